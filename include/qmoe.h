@@ -375,6 +375,48 @@ int qmoe_w8a16_gemv(const void* x, const void* w, const void* scale, void* y, in
 int qmoe_w8a16_gemm_mfma(const void* x, const void* w, const void* scale, void* y, int M, int K, int N,
                          int group_size, void* stream);
 
+/* ---- Norms around a block. n(v; w) = v * (mean(v^2) + eps)^(-1/2) * (offset + w) per row of
+ *      H <= 32768, in fp32 with one rounding per output (a sum of squares beyond the fp32
+ *      range is taken in 64 bits); eps >= 1e-30; offset 1 for weights stored as their distance
+ *      from one. Types are QMOE_BF16 / QMOE_F16 / QMOE_F32 (weights, gate: any of them); rows
+ *      are any number of elements apart (inputs may share rows: a step of 0), their elements
+ *      contiguous, at any alignment of the element. No counterpart among the reference's
+ *      kernels (its engine's RMSNorm is fnx/engine.py's own, outside the expert path). */
+#define QMOE_BF16 0
+#define QMOE_F16 1
+#define QMOE_F32 2
+/* Before a block: y = n(x; weight). ytype is xtype, or 16-bit for x in fp32. */
+int qmoe_block_norm(const void* x, long ldx, int xtype, const void* weight, int wtype, void* y, long ldy, int ytype,
+                    long rows, int H, float eps, float offset, void* stream);
+/* After a block: p = n(y; post_weight) (y itself for NULL), h = residual + scale * a(gate) * p,
+ * and for a next_weight the next block's input x = n(h; next_weight), normed from h before
+ * its rounding. a: the gate's value or, with gate_sigmoid, its sigmoid; gate NULL: 1. The gate
+ * of row r, column c is gate[r * gate_row_step + c * gate_column_step], gate_column_step 0 or
+ * 1 (one per row: 1 and 0; one per channel: 0 and 1). residual and h have rtype: ytype, or
+ * fp32; x has ytype. h may be the residual itself (same pointer and row step); no other
+ * output may overlap an input. next_weight and x go together. */
+int qmoe_block_residual(const void* y, long ldy, int ytype, const void* residual, long ldr, int rtype,
+                        const void* post_weight, int post_type, const void* gate, long gate_row_step,
+                        int gate_column_step, int gate_type, int gate_sigmoid, float scale, void* h, long ldh,
+                        const void* next_weight, int next_type, void* x, long ldx, long rows, int H, float eps,
+                        float offset, void* stream);
+
+/* ---- Log probabilities of given tokens, entropy and top alternatives, what follows the
+ *      lm_head projection (fnx/load.py:189-201). logits [T, V <= 2^30] of `type`, rows ld elements
+ *      apart at any alignment of the element; allowed: bytes [T, V], rows ld_allowed apart (0:
+ *      one row for all), 0 takes the token out whatever its logit holds, or NULL;
+ *      logprobs fp32 [T, m] = l - ln sum e^l of tokens int64 [T, m]; entropy fp32 [T]; the
+ *      `top` <= 32 largest logits (equal ones: lower id first) as top_ids int64 and
+ *      top_logprobs fp32 [T, top]. m = 0 and top = 0 leave their tensors out.
+ *      A token below 0 scores 0 (padding), one not allowed -inf, one from V on NaN. Fewer
+ *      than `top` tokens above -inf: id -1 and -inf fill up. A row with none at all: its tokens
+ *      -inf, entropy 0. A row with NaN or +inf at an allowed place: NaN, ids -1.
+ *      Workspace: qmoe_token_logprobs_workspace(T, V, type, top) bytes, 16-byte aligned. */
+size_t qmoe_token_logprobs_workspace(int T, int V, int type, int top);
+int qmoe_token_logprobs(const void* logits, long ld, int type, const void* tokens, int m, const void* allowed,
+                        long ld_allowed, int T, int V, void* logprobs, void* entropy, int top, void* top_ids,
+                        void* top_logprobs, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

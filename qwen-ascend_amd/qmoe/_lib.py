@@ -23,7 +23,10 @@ _SO = Path(__file__).with_name("libqmoe.so")
 P = ctypes.c_void_p
 I = ctypes.c_int
 L = ctypes.c_long
+F = ctypes.c_float
 Z = ctypes.c_size_t
+# QMOE_BF16, QMOE_F16 and QMOE_F32: the element types of the entry points that take several
+TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 EINVAL = -1  # QMOE_EINVAL: a shape or argument the entry point does not take
 
 # name -> (restype, argtypes); every entry point declared in include/qmoe.h
@@ -85,6 +88,10 @@ SIGNATURES = {
     "qmoe_w8a16_gemv_counters": (I, [I]),
     "qmoe_w8a16_gemv": (I, [P, P, P, P, I, I, I, I, P, Z, P, P]),
     "qmoe_w8a16_gemm_mfma": (I, [P, P, P, P, I, I, I, I, P]),
+    "qmoe_block_norm": (I, [P, L, I, P, I, P, L, I, L, I, F, F, P]),
+    "qmoe_block_residual": (I, [P, L, I, P, L, I, P, I, P, L, I, I, I, F, P, L, P, I, P, L, L, I, F, F, P]),
+    "qmoe_token_logprobs_workspace": (Z, [I, I, I, I]),
+    "qmoe_token_logprobs": (I, [P, L, I, P, I, P, L, I, I, P, P, I, P, P, P, Z, P]),
 }
 
 
@@ -129,6 +136,16 @@ def stream_of(t: torch.Tensor) -> int:
     if i < 0 or _RAW_STREAM is None:
         return torch.cuda.current_stream(t.device).cuda_stream  # raises for a tensor that is not on a GPU
     return _RAW_STREAM(i)
+
+
+def on_device_of(t: torch.Tensor, fn, *args):
+    """fn(*args), a launch on t's device: with that device current, as a launch on
+    its streams needs, where another one is."""
+    i = t.get_device()
+    if i == torch.cuda.current_device():
+        return fn(*args)
+    with torch.cuda.device(i):
+        return fn(*args)
 
 
 def ptr(t) -> int | None:

@@ -1,0 +1,93 @@
+"""Log probabilities of given tokens, with entropy and top alternatives.
+
+What follows the lm_head projection (a :class:`qmoe.DenseW8`, ``fnx/load.py:189-201``):
+the score of the tokens of a prompt, or of the ones sampled, beside the most likely ones.
+One pass over the logits with the running maximum and sums of the softmax, on the HIP kernels
+of libqmoe.so (``qmoe_token_logprobs``); nothing of the logits' size is written. Forward only:
+a tensor that requires a gradient is refused while gradients are recorded.
+"""
+from __future__ import annotations
+
+from typing import NamedTuple, Optional
+
+import torch
+
+from . import _lib
+from .norms import _check_tensors
+
+_TYPES = _lib.TYPES
+TOP_MAX = 32
+
+
+class TokenLogprobs(NamedTuple):
+    logprobs: Optional[torch.Tensor]      # fp32, the tokens' shape; None without tokens
+    entropy: torch.Tensor                 # fp32 [...]
+    top_ids: Optional[torch.Tensor]       # int64 [..., top]; None for top = 0
+    top_logprobs: Optional[torch.Tensor]  # fp32 [..., top]; None for top = 0
+
+
+def token_logprobs(logits, tokens=None, *, top=0, allowed=None):
+    """Scores of the softmax over rows of logits [..., V] (bfloat16, float16 or float32).
+
+    tokens int64 [...] or [..., m] (m given tokens for each row): their log
+    probabilities; a negative token scores 0 (padding), one that is not allowed -inf, one
+    from V on NaN. The entropy of each row. The ``top`` <= 32 most likely tokens in order
+    (equal logits: the lower id first) with their log probabilities; where fewer than ``top``
+    have a logit above -inf, id -1 and -inf fill up.
+
+    allowed: bool [V] or of the logits' shape; where it is False a token is out, whatever its
+    logit holds. A row with no token left: its tokens -inf, entropy 0. A row with NaN or +inf
+    at an allowed place has no distribution: NaN everywhere and ids -1. The sums are fp32:
+    log probabilities and entropies are exact to a few 2^-22 absolute.
+    """
+    if logits.dtype not in _TYPES:
+        raise RuntimeError("logits must be bfloat16, float16 or float32")
+    if logits.dim() < 1 or not 1 <= logits.shape[-1] <= 1 << 30:
+        raise RuntimeError("logits must be [..., V] with 1 <= V <= 2^30")
+    lead, V = logits.shape[:-1], logits.shape[-1]
+    top = int(top)
+    if not 0 <= top <= TOP_MAX:
+        raise RuntimeError(f"top must be 0..{TOP_MAX}")
+    m = 0
+    if tokens is not None:
+        if tokens.dtype != torch.int64:
+            raise RuntimeError("tokens must be int64")
+        if tokens.shape == lead:
+            m = 1
+        elif tokens.dim() == len(lead) + 1 and tokens.shape[:-1] == lead:
+            m = tokens.shape[-1]
+        else:
+            raise RuntimeError(f"tokens {tuple(tokens.shape)} do not match logits {tuple(logits.shape)}")
+    if allowed is not None and (allowed.dtype != torch.bool or allowed.shape not in ((V,), logits.shape)):
+        raise RuntimeError("allowed must be bool [V] or of the logits' shape")
+    _check_tensors(logits, tokens, allowed)
+    x = logits if logits.dim() == 2 else logits.reshape(-1, V)
+    if x.stride(1) != 1 and V != 1:
+        x = x.contiguous()
+    T, dev = x.shape[0], x.device
+    if T >= 1 << 31:
+        raise RuntimeError("logits must have fewer than 2^31 rows")
+    lda = 0
+    if allowed is not None:
+        if allowed.dim() > 1:
+            allowed = allowed if allowed.dim() == 2 else allowed.reshape(-1, V)
+            lda = allowed.stride(0)
+        if allowed.stride(-1) != 1 and V != 1:
+            allowed = allowed.contiguous()
+            lda = V if allowed.dim() > 1 else 0
+    if tokens is not None:
+        tokens = tokens.contiguous()
+    logprobs = None if tokens is None else torch.empty(tokens.shape, dtype=torch.float32, device=dev)
+    entropy = torch.empty(lead, dtype=torch.float32, device=dev)
+    top_ids = top_lp = None
+    if top:
+        top_ids = torch.empty((*lead, top), dtype=torch.int64, device=dev)
+        top_lp = torch.empty((*lead, top), dtype=torch.float32, device=dev)
+    L = _lib.lib()
+    kind, ptr = _TYPES[x.dtype], _lib.ptr
+    nbytes = L.qmoe_token_logprobs_workspace(T, V, kind, top)
+    ws = _lib.workspace(dev, nbytes) if nbytes else None
+    _lib.check(_lib.on_device_of(x, L.qmoe_token_logprobs, x.data_ptr(), x.stride(0), kind, ptr(tokens), m,
+                                 ptr(allowed), lda, T, V, ptr(logprobs), entropy.data_ptr(), top, ptr(top_ids),
+                                 ptr(top_lp), ptr(ws), nbytes, _lib.stream_of(x)), "token_logprobs")
+    return TokenLogprobs(logprobs, entropy, top_ids, top_lp)

@@ -1,0 +1,167 @@
+"""Norms around a block, with its gate and residual scale.
+
+A pre-norm layer calls, around each of its blocks (:func:`qmoe.shared.moe_block` here),
+
+    x = block_norm(h, w)                      # before the first block
+    y = block(x)
+    h, x = block_residual(y, h, next_weight=w)  # its residual sum and the next block's input
+
+RMS norm in fp32, n(v; w) = v * (mean(v^2) + eps)^(-1/2) * (offset + w), each output rounded
+once. HIP kernels of libqmoe.so (``qmoe_block_norm``, ``qmoe_block_residual``), one launch
+per call on the current stream of the tensors' device. Forward only: a tensor that requires a
+gradient is refused while gradients are recorded.
+"""
+from __future__ import annotations
+
+import torch
+
+from . import _lib
+from .ops import _same_device
+
+_TYPES = _lib.TYPES
+H_MAX = 32768
+
+
+def _rows(t, H):
+    """t [..., H] as rows [n, H] whose elements are contiguous (a view where it can be one)."""
+    if t.dim() != 2:
+        t = t.reshape(-1, H)
+    if t.stride(1) != 1 and H != 1:
+        t = t.contiguous()
+    return t
+
+
+def _check_weight(w, H, what):
+    if w.dtype not in _TYPES or w.shape != (H,):
+        raise RuntimeError(f"{what} must be a [{H}] tensor in bfloat16, float16 or float32")
+    return w if w.stride(0) == 1 or H == 1 else w.contiguous()
+
+
+def _check_row_tensor(t, what):
+    if t.dtype not in _TYPES:
+        raise RuntimeError(f"{what} must be bfloat16, float16 or float32")
+    if t.dim() < 1 or not 1 <= t.shape[-1] <= H_MAX:
+        raise RuntimeError(f"{what} must be [..., H] with 1 <= H <= {H_MAX}")
+
+
+def _check_tensors(*ts):
+    for t in ts:
+        if t is not None:
+            if not t.is_cuda:
+                raise RuntimeError("qmoe ops take device tensors")
+            if t.requires_grad and torch.is_grad_enabled():
+                raise RuntimeError("this operator has no backward pass: call it under torch.no_grad()")
+    _same_device(*ts)
+
+
+def block_norm(x, weight, *, eps=1e-6, offset=0.0, out_dtype=None):
+    """The norm before a block: n(x; weight) for rows x [..., H].
+
+    ``offset`` is added to the weight (1.0 for weights stored as their distance
+    from one). ``out_dtype`` is x's type, or bfloat16/float16 for a float32 x (a
+    32-bit residual stream normed to the block's type). ``eps`` >= 1e-30. Returns a
+    contiguous tensor of x's shape."""
+    _check_row_tensor(x, "x")
+    H = x.shape[-1]
+    out_dtype = x.dtype if out_dtype is None else out_dtype
+    if out_dtype not in _TYPES or (out_dtype != x.dtype and x.dtype != torch.float32):
+        raise RuntimeError("out_dtype must be x's type, or bfloat16 or float16 for a float32 x")
+    weight = _check_weight(weight, H, "weight")
+    _check_tensors(x, weight)
+    out = torch.empty(x.shape, dtype=out_dtype, device=x.device)
+    x = _rows(x, H)
+    _lib.check(_lib.on_device_of(x, _lib.lib().qmoe_block_norm, x.data_ptr(), x.stride(0), _TYPES[x.dtype],
+                                 weight.data_ptr(), _TYPES[weight.dtype], out.data_ptr(), H, _TYPES[out_dtype],
+                                 x.shape[0], H, eps, offset, _lib.stream_of(x)), "block_norm")
+    return out
+
+
+def _gate_steps(gate, shape, H):
+    """The gate as (tensor, row step, column step) of the rows of ``shape``."""
+    try:
+        g = gate.expand(shape)
+    except RuntimeError:
+        raise RuntimeError(f"gate {tuple(gate.shape)} does not broadcast to {tuple(shape)}") from None
+    if g.dim() != 2:
+        g = g.reshape(-1, H)
+    if H == 1 or g.stride(1) == 0:
+        return g, g.stride(0), 0
+    if g.stride(1) != 1:
+        g = g.contiguous()
+    return g, g.stride(0), 1
+
+
+def _span(t):
+    """Bytes [first, past the last) that a tensor's elements lie in."""
+    if t.numel() == 0:
+        return 0, 0
+    last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
+    return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+
+
+def _inplace_rows(residual, H, others):
+    """Rows of a residual that is written in place: a view of it, apart from each other and from
+    every other operand (y may be the residual itself)."""
+    rows = residual if residual.dim() == 2 else residual.view(-1, H)
+    if rows.shape[0] and ((rows.stride(1) != 1 and H != 1) or (rows.stride(0) < H and rows.shape[0] > 1)):
+        raise RuntimeError("inplace needs a residual of rows with contiguous elements that do not overlap")
+    lo, hi = _span(rows)
+    for t, same_is_fine in others:
+        if t is None:
+            continue
+        a, b = _span(t)
+        if a < hi and lo < b and not (same_is_fine and a == lo and t.dtype == rows.dtype
+                                      and t.stride() == residual.stride()):
+            raise RuntimeError("inplace: the residual overlaps another operand")
+    return rows
+
+
+def block_residual(y, residual, *, post_weight=None, gate=None, gate_act=None, scale=1.0, next_weight=None,
+                   eps=1e-6, offset=0.0, inplace=False):
+    """What follows a block: h = residual + scale * a(gate) * p, with p = n(y; post_weight)
+    (or y without one), and with ``next_weight`` the next block's input x = n(h; next_weight).
+
+    y [..., H]; residual of y's shape and type, or float32 beside a 16-bit y. gate: any
+    tensor that broadcasts to y (one value per row, per channel or per element), a: its value,
+    or its sigmoid for ``gate_act="sigmoid"``. The weights take ``offset`` as in
+    :func:`block_norm`. Returns h (contiguous, the residual's type), or (h, x) with x in y's
+    type; x is normed from h before h is rounded. ``inplace=True`` writes h over
+    ``residual`` and returns that tensor."""
+    _check_row_tensor(y, "y")
+    H = y.shape[-1]
+    if residual.shape != y.shape:
+        raise RuntimeError(f"residual {tuple(residual.shape)} and y {tuple(y.shape)} do not match")
+    if residual.dtype != y.dtype and residual.dtype != torch.float32:
+        raise RuntimeError("residual must have y's type or float32")
+    if gate_act not in (None, "sigmoid"):
+        raise RuntimeError("gate_act is None or 'sigmoid'")
+    if gate is not None and gate.dtype not in _TYPES:
+        raise RuntimeError("gate must be bfloat16, float16 or float32")
+    if gate is None and gate_act is not None:
+        raise RuntimeError("gate_act needs a gate")
+    if post_weight is not None:
+        post_weight = _check_weight(post_weight, H, "post_weight")
+    if next_weight is not None:
+        next_weight = _check_weight(next_weight, H, "next_weight")
+    _check_tensors(y, residual, post_weight, gate, next_weight)
+    g, g_row, g_col = (None, 0, 0) if gate is None else _gate_steps(gate, y.shape, H)
+    if inplace:
+        h = residual
+        res = hr = _inplace_rows(residual, H, ((y, True), (gate, False), (post_weight, False), (next_weight, False)))
+        ldr = ldh = res.stride(0) if res.shape[0] > 1 else H
+        if not residual.is_inference():
+            torch.autograd.graph.increment_version(residual)
+    else:
+        hr = h = torch.empty(residual.shape, dtype=residual.dtype, device=residual.device)
+        res = _rows(residual, H)
+        ldr, ldh = res.stride(0), H
+    x = None if next_weight is None else torch.empty(y.shape, dtype=y.dtype, device=y.device)
+    y = _rows(y, H)
+    ptr = _lib.ptr
+    _lib.check(_lib.on_device_of(
+        y, _lib.lib().qmoe_block_residual, y.data_ptr(), y.stride(0), _TYPES[y.dtype], res.data_ptr(), ldr,
+        _TYPES[res.dtype], ptr(post_weight), 0 if post_weight is None else _TYPES[post_weight.dtype], ptr(g), g_row,
+        g_col, 0 if g is None else _TYPES[g.dtype], int(gate_act == "sigmoid"), scale, hr.data_ptr(), ldh,
+        ptr(next_weight), 0 if next_weight is None else _TYPES[next_weight.dtype], ptr(x), H, y.shape[0], H, eps,
+        offset, _lib.stream_of(y)), "block_residual")
+    return h if x is None else (h, x)

@@ -1,0 +1,158 @@
+"""What the norm and log-probability operators refuse, and their references (CPU only)."""
+import math
+
+import pytest
+import torch
+
+import operators_ref as R
+
+BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
+
+
+def t(*shape, dtype=BF16):
+    return torch.zeros(shape, dtype=dtype)
+
+
+@pytest.mark.parametrize("call,says", [
+    (lambda q: q.block_norm(t(2, 8), t(8)), "device tensors"),
+    (lambda q: q.block_norm(t(2, 8), t(7)), "weight"),
+    (lambda q: q.block_norm(t(2, 8), t(8, dtype=torch.float64)), "weight"),
+    (lambda q: q.block_norm(t(2, 8, dtype=torch.int32), t(8)), "x must be"),
+    (lambda q: q.block_norm(t(2, 0), t(0)), "1 <= H"),
+    (lambda q: q.block_norm(t(2, 32769), t(32769)), "1 <= H"),
+    (lambda q: q.block_norm(torch.zeros((), dtype=BF16), t(1)), "1 <= H"),
+    (lambda q: q.block_norm(t(2, 8), t(8), out_dtype=F32), "out_dtype"),
+    (lambda q: q.block_norm(t(2, 8), t(8), out_dtype=F16), "out_dtype"),
+    (lambda q: q.block_residual(t(2, 8), t(2, 8)), "device tensors"),
+    (lambda q: q.block_residual(t(2, 8), t(8)), "do not match"),
+    (lambda q: q.block_residual(t(2, 8), t(2, 8, dtype=F16)), "residual must have"),
+    (lambda q: q.block_residual(t(2, 8, dtype=F32), t(2, 8)), "residual must have"),
+    (lambda q: q.block_residual(t(2, 8), t(2, 8), gate=t(2, 1), gate_act="tanh"), "gate_act"),
+    (lambda q: q.block_residual(t(2, 8), t(2, 8), gate_act="sigmoid"), "needs a gate"),
+    (lambda q: q.block_residual(t(2, 8), t(2, 8), gate=t(2, 1, dtype=torch.int8)), "gate must be"),
+    (lambda q: q.block_residual(t(2, 8), t(2, 8), post_weight=t(2, 8)), "post_weight"),
+    (lambda q: q.block_residual(t(2, 8), t(2, 8), next_weight=t(9)), "next_weight"),
+    (lambda q: q.token_logprobs(t(2, 8)), "device tensors"),
+    (lambda q: q.token_logprobs(t(2, 8, dtype=torch.int64)), "logits must be"),
+    (lambda q: q.token_logprobs(t(2, 0)), "1 <= V"),
+    (lambda q: q.token_logprobs(t(2, 8), top=33), "top"),
+    (lambda q: q.token_logprobs(t(2, 8), top=-1), "top"),
+    (lambda q: q.token_logprobs(t(2, 8), torch.zeros(2, dtype=torch.int32)), "int64"),
+    (lambda q: q.token_logprobs(t(2, 8), torch.zeros(3, dtype=torch.int64)), "do not match"),
+    (lambda q: q.token_logprobs(t(2, 8), torch.zeros((2, 3, 1), dtype=torch.int64)), "do not match"),
+    (lambda q: q.token_logprobs(t(2, 8), allowed=torch.ones((2, 7), dtype=torch.bool)), "allowed"),
+    (lambda q: q.token_logprobs(t(2, 8), allowed=torch.ones((2, 8), dtype=torch.uint8)), "allowed"),
+])
+def test_refusals(call, says):
+    import qmoe
+    with pytest.raises(RuntimeError, match=says):
+        call(qmoe)
+
+
+def test_gate_that_does_not_broadcast():
+    from qmoe.norms import _gate_steps
+    with pytest.raises(RuntimeError, match="does not broadcast"):
+        _gate_steps(t(3, 1), (2, 8), 8)
+    assert _gate_steps(t(2, 1), (2, 8), 8)[1:] == (1, 0)
+    assert _gate_steps(t(8), (2, 8), 8)[1:] == (0, 1)
+    assert _gate_steps(t(1, 1), (2, 8), 8)[2] == 0
+    assert _gate_steps(t(2, 3, 1), (2, 3, 8), 8)[1:] == (1, 0)
+    assert _gate_steps(t(8, 2).t(), (2, 8), 8)[1:] == (8, 1)     # columns first: copied
+    assert _gate_steps(t(2, 16)[:, :8], (2, 8), 8)[1:] == (16, 1)
+
+
+def test_inplace_overlap():
+    from qmoe.norms import _inplace_rows
+    base = t(64)
+    r = base[:32].view(4, 8)
+    assert _inplace_rows(r, 8, ((r, True), (None, False))).data_ptr() == r.data_ptr()
+    for other, fine in ((r, False), (base[8:40].view(4, 8), True), (base[31:39], False)):
+        with pytest.raises(RuntimeError, match="overlaps"):
+            _inplace_rows(r, 8, ((other, fine),))
+    _inplace_rows(r, 8, ((base[32:].view(4, 8), False),))
+    with pytest.raises(RuntimeError, match="do not overlap"):
+        _inplace_rows(t(1, 8).expand(4, 8), 8, ())
+    with pytest.raises(RuntimeError, match="do not overlap"):
+        _inplace_rows(base[:32].view(8, 4).t(), 8, ())
+
+
+def test_gradients_are_refused():
+    from qmoe.norms import _check_tensors
+
+    class Leaf:
+        is_cuda, requires_grad = True, True
+
+        def get_device(self):
+            return 0
+    with pytest.raises(RuntimeError, match="no backward pass"):
+        _check_tensors(Leaf())
+    with torch.no_grad():
+        _check_tensors(Leaf())
+
+
+def test_c_entries_refuse_before_any_launch():
+    from qmoe import _lib
+    L = _lib.lib()
+
+    def norm(rows=1, H=8, eps=1e-6, offset=0.0, xt=0, wt=0, yt=0, ldx=8, ldy=8, p=None):
+        return L.qmoe_block_norm(p, ldx, xt, p, wt, p, ldy, yt, rows, H, eps, offset, None)
+    assert norm(rows=0) == 0
+    for kw in (dict(rows=-1), dict(H=0), dict(H=32769, ldy=32769), dict(eps=0.0), dict(eps=-1.0), dict(eps=1e-31),
+               dict(eps=math.nan), dict(eps=math.inf), dict(offset=math.nan), dict(wt=3), dict(ldx=-1), dict(ldy=7)):
+        assert norm(**kw) == -1 and norm(**{"rows": 0, **kw}) == -1, kw
+    assert norm() == -1  # null pointers
+
+    def res(rows=1, H=8, yt=0, rt=0, gate=None, g_row=1, g_col=0, gt=0, scale=1.0, h=None, ldr=8, ldh=8, nxt=None,
+            x=None, ldx=8, r=None, y=None):
+        return L.qmoe_block_residual(y, 8, yt, r, ldr, rt, None, 0, gate, g_row, g_col, gt, 0, scale, h, ldh, nxt, 0,
+                                     x, ldx, rows, H, 1e-6, 0.0, None)
+    assert res(rows=0) == 0
+    for kw in (dict(rows=-1), dict(scale=math.inf), dict(gate=16, gt=7), dict(gate=16, g_col=2), dict(gate=16, g_row=-1),
+               dict(nxt=16), dict(x=16), dict(nxt=16, x=16, ldx=7), dict(ldr=-1), dict(ldh=7)):
+        assert res(**{"rows": 0, **kw}) == -1, kw
+    assert res() == -1
+    assert res(y=16, r=32, h=32, ldr=16, ldh=8) == -1       # in place with another row step
+    assert res(y=16, r=32, h=48, yt=0, rt=1) == -1          # types that do not go together
+    assert res(y=16, r=32, h=48, yt=2, rt=0) == -1
+
+    def lp(T=1, V=8, kind=0, m=0, top=0, ld=8, p=None, allowed=None, lda=0):
+        return L.qmoe_token_logprobs(p, ld, kind, p, m, allowed, lda, T, V, p, p, top, p, p, None, 0, None)
+    assert lp(T=0) == 0
+    for kw in (dict(T=-1), dict(V=0), dict(V=(1 << 30) + 1), dict(m=-1), dict(top=33), dict(top=-1), dict(ld=-1),
+               dict(allowed=16, lda=-1)):
+        assert lp(**kw) == -1, kw
+    assert lp() == -1
+
+
+def test_references():
+    """The references against hand-worked values and torch's own float64 functions."""
+    out, err = R.block_norm(torch.tensor([[3.0, 4.0]]), torch.tensor([1.0, 2.0]), eps=12.5)
+    assert torch.allclose(out, torch.tensor([[0.6, 1.6]], dtype=torch.float64)) and (err < 1e-5).all()
+    (h, _), (x, _) = R.block_residual(torch.tensor([[2.0, 0.0]]), torch.tensor([[1.0, 4.0]]), scale=0.5,
+                                      gate=torch.tensor([[4.0]]), next_weight=torch.tensor([1.0, 1.0]), eps=1e-9)
+    assert h.tolist() == [[5.0, 4.0]] and torch.allclose(x, h / math.sqrt(20.5))
+    g = torch.Generator().manual_seed(0)
+    l = torch.randn((3, 50), generator=g) * 3
+    l[1, 7:] = -float("inf")
+    tok = torch.tensor([[1, -1], [9, 50], [4, 4]])
+    (lp, _), (ent, _), ids, (tl, _) = R.token_logprobs(l, tok, top=8)
+    ref = l.double().log_softmax(1)
+    assert torch.allclose(lp[0, 0], ref[0, 1]) and lp[0, 1] == 0 and lp[1, 0] == -math.inf and lp[1, 1].isnan()
+    want = torch.distributions.Categorical(logits=l.double()[[0, 2]]).entropy()
+    assert torch.allclose(ent[[0, 2]], want)
+    assert ids[0].tolist() == torch.topk(l[0], 8)[1].tolist() and ids[1, 7] == -1 and tl[1, 7] == -math.inf
+    (_, _), (ent, _), ids, _ = R.token_logprobs(torch.tensor([[math.nan, 1.0], [-math.inf, -math.inf]]),
+                                                torch.tensor([0, 0]), top=1)
+    assert ent[0].isnan() and ent[1] == 0 and ids.tolist() == [[-1], [-1]]
+
+
+def test_planted_mistakes_are_seen():
+    """assert_close tells an exact value from one a step of the type away, and other infinities and NaN."""
+    e = torch.tensor([1.0, 100.0, 0.0, math.nan, -math.inf], dtype=torch.float64)
+    b = R.half_step(e, BF16)
+    R.assert_close(e.to(BF16), e, b, "same")
+    for at, v in ((0, 1.0 + 2 ** -7), (1, 100.5), (2, 1e-30), (3, 0.0), (4, math.inf), (0, math.nan)):
+        g = e.clone()
+        g[at] = v
+        with pytest.raises(AssertionError):
+            R.assert_close(g.to(BF16), e, b, "planted")
