@@ -33,6 +33,23 @@ def test_block_norm(device, T, H, xt, ot, wt, offset):
     R.assert_close(out, *R.block_norm(x, w, 1e-6, offset, ot), "block_norm")
 
 
+# more rows than workgroups stay resident: one wave a row, several, sixteen; short, odd, even
+MANY = [(20001, 64), (9001, 641), (5000, 1024), (5003, 1033), (3001, 2560), (1300, 4096), (1100, 8192), (601, 9001),
+        (800, 16384), (530, 16390)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,H", MANY)
+@pytest.mark.parametrize("xt,ot", [(BF16, BF16), (F32, F32), (F32, F16)])
+def test_block_norm_many_rows(device, T, H, xt, ot):
+    from qmoe import block_norm
+    log(f"block_norm T={T} H={H} {xt} {ot}")
+    n = gen(device, T + H)
+    x, w = n(T, H, std=3.0, dtype=xt), n(H, std=0.3)
+    x[T // 2, H // 2] = torch.finfo(xt).max  # this row's squares leave the fp32 range, the others' not
+    R.assert_close(block_norm(x, w, out_dtype=ot), *R.block_norm(x, w, 1e-6, 0.0, ot), "block_norm")
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("xt", [BF16, F32])
 def test_block_norm_layouts(device, xt):
@@ -129,6 +146,21 @@ def test_block_residual(device, T, H, c):
     again = block_residual(y, r, inplace=True, **kw)
     h = again[0] if isinstance(again, tuple) else again
     assert h is r and r._version > v
+    for a, b in zip(got if isinstance(got, tuple) else (got,), again if isinstance(again, tuple) else (again,)):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,H", MANY)
+@pytest.mark.parametrize("c", [COMBOS[0], COMBOS[3], COMBOS[5], COMBOS[6], COMBOS[7]])
+def test_block_residual_many_rows(device, T, H, c):
+    from qmoe import block_residual
+    log(f"block_residual T={T} H={H} {c}")
+    y, r, kw = operands(gen(device, T + 5 * H), T, H, c)
+    want = R.block_residual(y, r, **kw)
+    got = block_residual(y, r, **kw)
+    check_residual(got, want, "block_residual")
+    again = block_residual(y, r, inplace=True, **kw)
     for a, b in zip(got if isinstance(got, tuple) else (got,), again if isinstance(again, tuple) else (again,)):
         assert torch.equal(a, b)
 
