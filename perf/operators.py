@@ -168,8 +168,8 @@ def _own(s):
         return q.block_norm(s["x"], s["w"], offset=case["offset"], out_dtype=_TYPES[case["out"]])
     if case["op"] == "residual":
         return q.block_residual(s["y"], s["res"], post_weight=s["post"], gate=s["gate"],
-                                gate_act="sigmoid" if case["sigmoid"] else None, scale=case["scale"],
-                                next_weight=s["next"], offset=case["offset"])
+                                gate_act="sigmoid" if case["sigmoid"] and s["gate"] is not None else None,
+                                scale=case["scale"], next_weight=s["next"], offset=case["offset"])
     r = q.token_logprobs(s["x"], s["tokens"], top=case["top"], allowed=s["allowed"])
     if not case["top"]:
         return r.logprobs, r.entropy
