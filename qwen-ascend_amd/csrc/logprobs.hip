@@ -37,14 +37,39 @@ struct Part {
 // Base of the exponents: an empty part (m = -inf) takes 0, so its terms are e^-inf = 0.
 QMOE_DEV float base_of(float m) { return m == -INFINITY ? 0.f : m; }
 
-QMOE_DEV Part join(Part a, Part b) {
-  const float m = fmaxf(a.m, b.m), z = base_of(m);
-  const float da = (a.m - z) * LOG2E, db = (b.m - z) * LOG2E;
-  const float ca = __builtin_amdgcn_exp2f(da), cb = __builtin_amdgcn_exp2f(db);
-  Part r;
-  r.m = m;
-  r.s = ca * a.s + cb * b.s;
-  r.d = ca * (a.d + fmaxf(da, FAR) * a.s) + cb * (b.d + fmaxf(db, FAR) * b.s);
+QMOE_DEV float wave_max_f32(float v) {
+  v = fmaxf(v, QMOE_DPPF(v, 0xB1));
+  v = fmaxf(v, QMOE_DPPF(v, 0x4E));
+  v = fmaxf(v, QMOE_DPPF(v, 0x141));
+  v = fmaxf(v, QMOE_DPPF(v, 0x140));
+  const int i = __float_as_int(v);
+  return fmaxf(fmaxf(__int_as_float(__builtin_amdgcn_readlane(i, 0)), __int_as_float(__builtin_amdgcn_readlane(i, 16))),
+               fmaxf(__int_as_float(__builtin_amdgcn_readlane(i, 32)), __int_as_float(__builtin_amdgcn_readlane(i, 48))));
+}
+
+// p taken to the maximum m >= p.m
+QMOE_DEV Part moved(Part p, float m) {
+  const float shift = (p.m - base_of(m)) * LOG2E, c = __builtin_amdgcn_exp2f(shift);
+  return {m, c * p.s, c * (p.d + fmaxf(shift, FAR) * p.s)};
+}
+
+// The parts of a wave's lanes as one, the same in every lane.
+QMOE_DEV Part wave_join(Part p) {
+  p = moved(p, wave_max_f32(p.m));
+  return {p.m, wave_sum_f32(p.s), wave_sum_f32(p.d)};
+}
+
+// The parts of a workgroup's waves as one.
+QMOE_DEV Part join_waves(const Part* w) {
+  float m = w[0].m;
+#pragma unroll
+  for (int i = 1; i < WAVES; ++i) m = fmaxf(m, w[i].m);
+  Part r = {m, 0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < WAVES; ++i) {
+    const Part p = moved(w[i], m);
+    r.s += p.s, r.d += p.d;
+  }
   return r;
 }
 
@@ -60,67 +85,457 @@ QMOE_DEV float key_logit(uint64_t k) {
   return __uint_as_float((o & 0x80000000u) ? (o & 0x7fffffffu) : ~o);
 }
 
+// ---------------------------------------------------------------- one wave's stream
+
+// Candidates for the top alternatives that a wave keeps between compactions.
+constexpr int CAP = 256;
+constexpr int KEPT = CAP / 64;
+
+// Low bits of a logit's order key that its type leaves alike for all values of one sign.
 template <typename E>
-__global__ __launch_bounds__(THREADS) void logprob_rows_kernel(LogprobArgs a) {
-  __shared__ Part part[WAVES];
-  __shared__ uint64_t best[WAVES];
-  for (int t = blockIdx.x; t < a.T; t += gridDim.x) {
-    const auto* x = static_cast<const typename E::raw*>(a.logits) + (long)t * a.ld;
-    const uint8_t* ok = a.allowed ? a.allowed + (long)t * a.lda : nullptr;
-    auto logit = [&](int v) { return (ok && !ok[v]) ? -INFINITY : E::load(x[v]); };
-    Part p = {-INFINITY, 0.f, 0.f};
-    for (int v = threadIdx.x; v < a.V; v += THREADS) p = join(p, {logit(v), 1.f, 0.f});
+constexpr int KEY_SHIFT = 0;
+template <>
+constexpr int KEY_SHIFT<ElemBF16> = 16;
+template <>
+constexpr int KEY_SHIFT<ElemF16> = 13;
+
+QMOE_DEV uint32_t order_of(float l) { return (uint32_t)(key_of(l, 0) >> 32); }
+QMOE_DEV float order_logit(uint32_t o) { return key_logit((uint64_t)o << 32); }
+
+QMOE_DEV int lanes_below(uint64_t mask) {
+  return __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0));
+}
+
+// The k-th largest of one value per lane, bit by bit from the top.
+template <int BITS>
+QMOE_DEV uint32_t wave_kth(uint32_t v, int k) {
+  uint32_t r = 0;
 #pragma unroll
-    for (int o = 32; o; o >>= 1) p = join(p, {__shfl_xor(p.m, o), __shfl_xor(p.s, o), __shfl_xor(p.d, o)});
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = p;
-    __syncthreads();
-    p = part[0];
+  for (int b = BITS - 1; b >= 0; --b) {
+    const uint32_t c = r | (1u << b);
+    if (__popcll(__ballot(v >= c)) >= k) r = c;
+  }
+  return r;
+}
+
+// The k-th largest of one logit per lane.
+template <typename E>
+QMOE_DEV float wave_kth_logit(float l, int k) {
+  constexpr int SH = KEY_SHIFT<E>;
+  uint32_t o = wave_kth<32 - SH>(order_of(l) >> SH, k) << SH;
+  if (!(o & 0x80000000u)) o |= (1u << SH) - 1u;  // a negative value's low zeros are ones in its key
+  return order_logit(o);
+}
+
+// Keeps the k best of a wave's n candidates (n >= k) and returns the logit of the last of them.
+QMOE_DEV float compact(uint64_t* cand, int n, int k) {
+  const int lane = threadIdx.x & 63;
+  uint64_t key[KEPT];
 #pragma unroll
-    for (int w = 1; w < WAVES; ++w) p = join(p, part[w]);
-    const bool undefined = !(p.s >= 0.f);  // a NaN or +inf at an allowed place
-    const float log_s = logf(p.s);
-    if (threadIdx.x == 0) a.entropy[t] = p.s == 0.f ? 0.f : log_s - LN2 * p.d / p.s;
-    for (int j = threadIdx.x; j < a.m; j += THREADS) {
-      const int64_t tok = a.tokens[(long)t * a.m + j];
-      float r = 0.f;
-      if (tok >= a.V || undefined) r = NAN;
-      else if (tok >= 0) {
-        const float l = logit((int)tok);
-        r = l == -INFINITY ? l : (l - p.m) - log_s;
+  for (int q = 0; q < KEPT; ++q) key[q] = q * 64 + lane < n ? cand[q * 64 + lane] : 0;
+  uint64_t kth = 0;
+#pragma unroll 1
+  for (int b = 63; b >= 0; --b) {
+    const uint64_t c = kth | (1ull << b);
+    int count = 0;
+#pragma unroll
+    for (int q = 0; q < KEPT; ++q) count += __popcll(__ballot(key[q] >= c));
+    if (count >= k) kth = c;
+  }
+  int at = 0;
+#pragma unroll
+  for (int q = 0; q < KEPT; ++q) {
+    const bool keep = key[q] >= kth;
+    const uint64_t mask = __ballot(keep);
+    if (keep) cand[at + lanes_below(mask)] = key[q];
+    at += __popcll(mask);
+  }
+  return key_logit(kth);
+}
+
+// Each lane's largest logit so far, for all waves of the workgroup.
+struct Tops {
+  float v[WAVES][64];
+  QMOE_DEV void clear() { v[threadIdx.x >> 6][threadIdx.x & 63] = -INFINITY; }
+  // Stores this lane's value and returns the largest one of the same lane of all waves.
+  QMOE_DEV float raise(float mine) {
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    __hip_atomic_store(&v[wave][lane], mine, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+    return most(mine);
+  }
+  QMOE_DEV float most(float m) {
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w)
+      m = fmaxf(m, __hip_atomic_load(&v[w][threadIdx.x & 63], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP));
+    return m;
+  }
+};
+
+// A wave's running state: per lane the softmax sums and the largest logit of what it has read,
+// per wave the candidates for the top k and two bounds that a logit has to pass to become one:
+// - tau: k logits of this wave, at lower ids than what follows, are >= tau: only above it;
+// - floor: k logits of the workgroup, at any ids, are >= floor: from it on.
+// floor is the k-th largest of the 64 maxima over the same lane of all waves, which the waves
+// read from each other whenever they see a logit above their bounds; a value that another wave
+// has raised since is only a weaker bound.
+template <typename E, bool MASK, bool TOP>
+struct Stream {
+  bool infinite = MASK;
+  Part p = {-INFINITY, 0.f, 0.f};
+  float top = -INFINITY, tau = -INFINITY, floor = -INFINITY;
+  int count = 0;
+
+  // Adds the J pieces of P logits x.get(j, i). An infinite distance to the maximum would make D
+  // NaN (0 * inf): so long as none is met, nothing is done about it; from then on distances are
+  // taken no lower than FAR.
+  template <int P, int J, typename X>
+  QMOE_DEV void add(X& x, float most) {
+    p = moved(p, fmaxf(p.m, most));
+    const float z = base_of(p.m);
+    if (!infinite) {
+      float s = p.s, d = p.d;
+#pragma unroll
+      for (int j = 0; j < J; ++j) {
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+          const float l = (x.get(j, i) - z) * LOG2E, e = __builtin_amdgcn_exp2f(l);
+          s += e;
+          d += e * l;
+        }
+        __builtin_amdgcn_sched_barrier(0);  // a piece at a time: few registers, more waves
       }
-      a.logprobs[(long)t * a.m + j] = tok < 0 ? 0.f : r;
+      infinite = __any(d != d);
+      if (!infinite) {
+        p.s = s, p.d = d;
+        return;
+      }
     }
-    uint64_t last = ~0ull;
-    for (int j = 0; j < a.top; ++j) {
-      uint64_t k = 0;
-      for (int v = threadIdx.x; v < a.V; v += THREADS) {
-        const float l = logit(v);
-        const uint64_t q = l > -INFINITY ? key_of(l, v) : 0;
-        if (q < last && q > k) k = q;
-      }
+    x.pin();
 #pragma unroll
-      for (int o = 32; o; o >>= 1) k = max(k, (uint64_t)__shfl_xor((unsigned long long)k, o));
-      __syncthreads();
-      if ((threadIdx.x & 63) == 0) best[threadIdx.x >> 6] = k;
-      __syncthreads();
-      k = best[0];
+    for (int j = 0; j < J; ++j) {
 #pragma unroll
-      for (int w = 1; w < WAVES; ++w) k = max(k, best[w]);
-      last = k;
-      if (threadIdx.x == 0) {
-        const bool none = undefined || k == 0;
-        a.top_ids[(long)t * a.top + j] = none ? -1 : key_id(k);
-        a.top_logprobs[(long)t * a.top + j] = undefined ? NAN : k == 0 ? -INFINITY : (key_logit(k) - p.m) - log_s;
+      for (int i = 0; i < P; ++i) {
+        const float l = (x.get(j, i) - z) * LOG2E, e = __builtin_amdgcn_exp2f(l);
+        p.s += e;
+        p.d += e * fmaxf(l, FAR);
       }
+      __builtin_amdgcn_sched_barrier(0);
     }
   }
+
+  // The same pieces' logits as candidates, piece j from id first + j * stride on. logit(id)
+  // reads one of them from memory.
+  template <int P, int J, typename X, typename F>
+  QMOE_DEV void offer(X& x, const float (&piece_most)[J], float most, int first, int stride, Tops* tops, uint64_t* cand,
+                      int k, F logit) {
+    if (!__any(most > tau && most >= floor)) return;
+    x.pin();
+    top = fmaxf(top, most);
+    floor = fmaxf(floor, wave_kth_logit<E>(tops->raise(top), k));
+    // enough lanes of this wave reach the floor: what follows has to exceed it
+    float next_tau = __popcll(__ballot(top >= floor)) >= k ? floor : tau;
+    int n = count;
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      if (!__any(piece_most[j] > tau && piece_most[j] >= floor)) continue;
+#pragma unroll
+      for (int i = 0; i < P; ++i) {
+        const float l = x.get(j, i);
+        const bool in = l > tau && l >= floor;
+        const uint64_t mask = __ballot(in);
+        if (mask == 0) continue;
+        const int at = n + lanes_below(mask);
+        if (in && at < CAP) cand[at] = key_of(l, first + j * stride + i);
+        n += __popcll(mask);
+      }
+    }
+    if (n > CAP) {
+      // Too many at once (equal or ascending logits): once more, keeping the k best as it fills.
+      n = count;
+#pragma unroll 1
+      for (int e = 0; e < J * P; ++e) {
+        const int id = first + e / P * stride + e % P;
+        const float l = logit(id);
+        bool in = l > tau && l >= floor;
+        uint64_t mask = __ballot(in);
+        if (n + __popcll(mask) > CAP) {
+          const float kth = compact(cand, n, k);
+          floor = fmaxf(floor, kth);
+          next_tau = fmaxf(next_tau, kth);  // for what follows these logits, whose ids are in no order
+          n = k;
+          in = l > tau && l >= floor;
+          mask = __ballot(in);
+        }
+        if (in) cand[n + lanes_below(mask)] = key_of(l, id);
+        n += __popcll(mask);
+      }
+    }
+    count = n;
+    tau = next_tau;
+  }
+};
+
+// ---------------------------------------------------------------- a row's results
+
+QMOE_DEV void emit_top(const LogprobArgs& a, int t, int rank, uint64_t key, Part p, float log_s, bool undefined) {
+  const bool none = undefined || key == 0;
+  a.top_ids[(long)t * a.top + rank] = none ? -1 : key_id(key);
+  a.top_logprobs[(long)t * a.top + rank] = undefined ? NAN : key == 0 ? -INFINITY : (key_logit(key) - p.m) - log_s;
+}
+
+// A given token and its logit (-inf where it is not allowed), read before the row is.
+struct Given {
+  int64_t token;
+  float logit;
+};
+template <typename E>
+QMOE_DEV Given load_given(const LogprobArgs& a, int t, int j) {
+  Given g = {-1, -INFINITY};
+  if (j >= a.m) return g;
+  g.token = a.tokens[(long)t * a.m + j];
+  if (g.token >= 0 && g.token < a.V && (!a.allowed || a.allowed[(long)t * a.lda + g.token]))
+    g.logit = E::load(static_cast<const typename E::raw*>(a.logits)[(long)t * a.ld + g.token]);
+  return g;
 }
 
 template <typename E>
-int launch(const LogprobArgs& a, hipStream_t st) {
-  hipLaunchKernelGGL((logprob_rows_kernel<E>), dim3((unsigned)std::min(a.T, 1 << 20)), dim3(THREADS), 0, st, a);
+QMOE_DEV void emit_row(const LogprobArgs& a, int t, Given g, Part p, float log_s, bool undefined) {
+  if (threadIdx.x == 0) a.entropy[t] = p.s == 0.f ? 0.f : log_s - LN2 * p.d / p.s;
+  for (int j = threadIdx.x; j < a.m; j += THREADS) {
+    if (j >= THREADS) g = load_given<E>(a, t, j);
+    float r = 0.f;
+    if (g.token >= a.V || (g.token >= 0 && undefined)) r = NAN;
+    else if (g.token >= 0) r = g.logit == -INFINITY ? g.logit : (g.logit - p.m) - log_s;
+    a.logprobs[(long)t * a.m + j] = r;
+  }
+}
+
+// Ranks n candidates (distinct keys) by counting the greater ones, one wave; out(rank, key) for
+// the first k ranks, key 0 where there are fewer.
+template <typename F>
+QMOE_DEV void rank_top(const uint64_t* list, int n, int k, F out) {
+  const int lane = threadIdx.x & 63;
+  for (int c = 0; c < n; c += 64) {
+    const uint64_t mine = c + lane < n ? list[c + lane] : 0;
+    int rank = 0;
+#pragma unroll 8
+    for (int i = 0; i < n; ++i) rank += list[i] > mine;
+    if (mine && rank < k) out(rank, mine);
+  }
+  if (lane >= n && lane < k) out(lane, 0);
+}
+
+template <typename E>
+constexpr int PIECE = 16 / sizeof(typename E::raw);
+
+// -inf in a word of the type's values.
+template <typename E>
+constexpr uint32_t MINUS_INF = 0xff80ff80u;
+template <>
+constexpr uint32_t MINUS_INF<ElemF16> = 0xfc00fc00u;
+template <>
+constexpr uint32_t MINUS_INF<ElemF32> = 0xff800000u;
+
+// A thread's next PIECES pieces of a row and of its mask, as loaded; pieces from `end` on hold
+// -inf.
+template <typename E, bool MASK, int PIECES>
+struct Pieces {
+  static constexpr int N = PIECE<E>;
+  RawVec<N, sizeof(typename E::raw)> v[PIECES];
+  uint32_t allow[PIECES][N / 4];
+  QMOE_DEV void load(const typename E::raw* x, const uint8_t* ok, int piece, int end) {
+#pragma unroll
+    for (int j = 0; j < PIECES; ++j) {
+      const long c = piece + j * THREADS;
+#pragma unroll
+      for (int i = 0; i < v[j].WORDS; ++i) v[j].w[i] = MINUS_INF<E>;
+      if constexpr (MASK) {
+#pragma unroll
+        for (int i = 0; i < N / 4; ++i) allow[j][i] = 0;
+      }
+      if (c < end) {
+        v[j].load(x + c * N);
+        if constexpr (MASK) {
+#pragma unroll
+          for (int i = 0; i < N / 4; ++i) __builtin_memcpy(&allow[j][i], ok + c * N + 4 * i, 4);
+        }
+      }
+    }
+  }
+  // Unpacked again by what follows, not kept as 32-bit values.
+  QMOE_DEV void pin() {
+#pragma unroll
+    for (int j = 0; j < PIECES; ++j)
+#pragma unroll
+      for (int i = 0; i < v[j].WORDS; ++i) asm volatile("" : "+v"(v[j].w[i]));
+  }
+  QMOE_DEV float get(int j, int i) const {
+    const float l = v[j].template get<E>(i);
+    if constexpr (MASK) return ((allow[j][i / 4] >> (8 * (i & 3))) & 0xffu) ? l : -INFINITY;
+    return l;
+  }
+};
+
+// A workgroup takes one of `splits` parts of a row, in steps of PIECES pieces of 16 bytes per
+// thread; with one part it writes the row's results, with several its sums and its best
+// candidates for join_kernel.
+template <typename E, bool MASK, bool TOP, int PIECES>
+__global__ __launch_bounds__(THREADS) void logprob_kernel(LogprobArgs a, int splits, int pieces_per_split, Part* parts,
+                                                          uint64_t* keys) {
+  constexpr int N = PIECE<E>;
+  __shared__ uint64_t cand[TOP ? WAVES : 1][TOP ? CAP : 1], list[TOP ? WAVES * CAP : 1];
+  __shared__ Part wave_part[WAVES];
+  __shared__ Tops tops;
+  __shared__ int listed;
+  const int tid = threadIdx.x, wave = tid >> 6;
+  if constexpr (TOP) {
+    tops.clear();
+    __syncthreads();
+  }
+  for (long unit = blockIdx.x; unit < (long)a.T * splits; unit += gridDim.x) {
+    const int t = (int)(unit / splits), part = (int)(unit % splits);
+    const auto* x = static_cast<const typename E::raw*>(a.logits) + (long)t * a.ld;
+    const uint8_t* ok = MASK ? a.allowed + (long)t * a.lda : nullptr;
+    const int pieces = a.V / N, begin = part * pieces_per_split, end = min(pieces, begin + pieces_per_split);
+    const Given given = splits == 1 ? load_given<E>(a, t, tid) : Given{-1, 0.f};
+    Stream<E, MASK, TOP> st;
+    auto logit = [&](int v, int stop) { return v < stop && (!MASK || ok[v]) ? E::load(x[v]) : -INFINITY; };
+    for (int q = begin; q < end; q += THREADS * PIECES) {
+      Pieces<E, MASK, PIECES> now;
+      now.load(x, ok, q + tid, end);
+      float most = -INFINITY, piece_most[PIECES];
+#pragma unroll
+      for (int j = 0; j < PIECES; ++j) {
+        piece_most[j] = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < N; ++i) piece_most[j] = fmaxf(piece_most[j], now.get(j, i));
+        most = fmaxf(most, piece_most[j]);
+      }
+      now.pin();
+      st.template add<N, PIECES>(now, most);
+      if constexpr (TOP)
+        st.template offer<N, PIECES>(now, piece_most, most, (q + tid) * N, THREADS * N, &tops, cand[wave], a.top,
+                                     [&](int id) { return logit(id, end * N); });
+    }
+    if (part == splits - 1 && pieces * N < a.V) {  // the row's end, less than a piece
+      const int v = pieces * N + tid;
+      struct {
+        float l;
+        QMOE_DEV float get(int, int) const { return l; }
+        QMOE_DEV void pin() {}
+      } last = {logit(v, a.V)};
+      const float most[1] = {last.l};
+      st.template add<1, 1>(last, last.l);
+      if constexpr (TOP)
+        st.template offer<1, 1>(last, most, last.l, v, 0, &tops, cand[wave], a.top,
+                                [&](int id) { return logit(id, a.V); });
+    }
+    Part p = wave_join(st.p);
+    if ((tid & 63) == 0) wave_part[wave] = p;
+    if (tid == 0) listed = 0;
+    __syncthreads();
+    p = join_waves(wave_part);
+    const bool undefined = !(p.s >= 0.f);  // a NaN or +inf at an allowed place
+    const float log_s = logf(p.s);
+    if constexpr (TOP) {
+      const float floor = wave_kth_logit<E>(tops.most(st.top), a.top);
+      for (int i = tid & 63; i < st.count; i += 64) {
+        const uint64_t key = cand[wave][i];
+        if (key_logit(key) >= floor) list[atomicAdd(&listed, 1)] = key;
+      }
+      __syncthreads();
+      tops.clear();  // for the next row
+      if (wave == 0) {
+        if (splits == 1)
+          rank_top(list, listed, a.top, [&](int r, uint64_t k) { emit_top(a, t, r, k, p, log_s, undefined); });
+        else
+          rank_top(list, listed, a.top, [&](int r, uint64_t k) { keys[unit * a.top + r] = k; });
+      }
+    }
+    if (splits == 1) emit_row<E>(a, t, given, p, log_s, undefined);
+    else if (tid == 0) parts[unit] = p;
+    __syncthreads();  // the next row reuses the LDS
+  }
+}
+
+constexpr int MAX_SPLITS = 64;
+
+// Joins the parts of a row: their sums and their ordered best candidates.
+template <typename E, bool TOP>
+__global__ __launch_bounds__(THREADS) void join_kernel(LogprobArgs a, int splits, const Part* parts, const uint64_t* keys) {
+  constexpr int EACH = MAX_SPLITS * TOP_MAX / THREADS;
+  __shared__ uint64_t list[TOP ? MAX_SPLITS * TOP_MAX : 1];
+  __shared__ int listed;
+  const int t = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
+  const Given given = load_given<E>(a, t, tid);
+  Part p = {-INFINITY, 0.f, 0.f};
+  if (lane < splits) p = parts[(long)t * splits + lane];
+  uint64_t key[TOP ? EACH : 1];
+  uint32_t floor = 0;
+  if constexpr (TOP) {
+    const uint64_t* mine = keys + (long)t * splits * a.top;
+    // The parts' keys are in order, so where `lists` parts have an r-th key of at least a floor
+    // and r * lists >= k, k keys reach it.
+    const int r = (a.top + splits - 1) / splits, lists = (a.top + r - 1) / r;
+    const uint32_t rth = lane < splits ? (uint32_t)(mine[lane * a.top + r - 1] >> 32) : 0u;
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) key[i] = i * THREADS + tid < splits * a.top ? mine[i * THREADS + tid] : 0;
+    if (tid == 0) listed = 0;
+    constexpr int SH = KEY_SHIFT<E>;
+    floor = wave_kth<32 - SH>(rth >> SH, lists) << SH;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < EACH; ++i)
+      if (key[i] && (uint32_t)(key[i] >> 32) >= floor) list[atomicAdd(&listed, 1)] = key[i];
+    __syncthreads();
+  }
+  p = wave_join(p);
+  const bool undefined = !(p.s >= 0.f);
+  const float log_s = logf(p.s);
+  if constexpr (TOP) {
+    if (tid < 64) rank_top(list, listed, a.top, [&](int r, uint64_t k) { emit_top(a, t, r, k, p, log_s, undefined); });
+  }
+  emit_row<E>(a, t, given, p, log_s, undefined);
+}
+
+// Pieces per part of a row: whole steps of 4 pieces per thread, or one step of 2 or 1 where that
+// leaves too few workgroups, so that there are about 1024 of them, four per CU (V = 131072 in
+// bf16, top 20, in 1, 2, 4, 8, 16, 32, 64 parts: 48 rows 33.6, 26.3, 19.6, 16.1, 14.6, 14.9 and
+// 18.9 us; 256 rows 38.6, 32.5, 28.4, 32.2, 38.1, 42.2 and 61.8; 1024 rows 62.6, 71.5, 78.9 ...).
+// Without top alternatives 512 rows are enough (512 rows in one part: 29.7 us, in two 32.6).
+int part_pieces(int T, int V, int type, int top) {
+  const int pieces = V / (type == QMOE_F32 ? 4 : 8), full = 4 * THREADS;
+  const int want = T >= (top ? 1024 : 512) ? 1 : std::min(host_ceil_div(1024, T), MAX_SPLITS);
+  for (int per = THREADS; per < full; per *= 2)
+    if (host_ceil_div(pieces, per) <= want) return per;
+  return full * std::max(1, host_ceil_div(host_ceil_div(pieces, full), want));
+}
+int splits_for(int T, int V, int type, int top) {
+  return std::max(1, host_ceil_div(V / (type == QMOE_F32 ? 4 : 8), part_pieces(T, V, type, top)));
+}
+
+template <typename E, bool MASK, bool TOP>
+int launch(const LogprobArgs& a, int type, void* ws, hipStream_t st) {
+  const int splits = splits_for(a.T, a.V, type, a.top), per = part_pieces(a.T, a.V, type, a.top);
+  Part* parts = static_cast<Part*>(ws);
+  uint64_t* keys = nullptr;
+  if (splits > 1) keys = reinterpret_cast<uint64_t*>(static_cast<char*>(ws) + ((size_t)a.T * splits * sizeof(Part) + 15) / 16 * 16);
+  const unsigned grid = (unsigned)std::min<long>((long)a.T * splits, 1l << 20);
+  if (per == THREADS)
+    hipLaunchKernelGGL((logprob_kernel<E, MASK, TOP, 1>), dim3(grid), dim3(THREADS), 0, st, a, splits, per, parts, keys);
+  else if (per == 2 * THREADS)
+    hipLaunchKernelGGL((logprob_kernel<E, MASK, TOP, 2>), dim3(grid), dim3(THREADS), 0, st, a, splits, per, parts, keys);
+  else
+    hipLaunchKernelGGL((logprob_kernel<E, MASK, TOP, 4>), dim3(grid), dim3(THREADS), 0, st, a, splits, per, parts, keys);
+  if (splits > 1)
+    hipLaunchKernelGGL((join_kernel<E, TOP>), dim3(a.T), dim3(THREADS), 0, st, a, splits, parts, keys);
   return (int)hipGetLastError();
+}
+
+template <typename E>
+int dispatch(const LogprobArgs& a, int type, void* ws, hipStream_t st) {
+  if (a.allowed) return a.top ? launch<E, true, true>(a, type, ws, st) : launch<E, true, false>(a, type, ws, st);
+  return a.top ? launch<E, false, true>(a, type, ws, st) : launch<E, false, false>(a, type, ws, st);
 }
 
 }  // namespace
@@ -128,27 +543,29 @@ int launch(const LogprobArgs& a, hipStream_t st) {
 extern "C" {
 
 size_t qmoe_token_logprobs_workspace(int T, int V, int type, int top) {
-  (void)T, (void)V, (void)type, (void)top;
-  return 0;
+  if (T < 1 || V < 1 || top < 0 || top > TOP_MAX || !known_type(type)) return 0;
+  const size_t splits = splits_for(T, V, type, top);
+  return splits == 1 ? 0 : (T * splits * sizeof(Part) + 15) / 16 * 16 + T * splits * top * sizeof(uint64_t);
 }
 
 int qmoe_token_logprobs(const void* logits, long ld, int type, const void* tokens, int m, const void* allowed,
                         long ld_allowed, int T, int V, void* logprobs, void* entropy, int top, void* top_ids,
                         void* top_logprobs, void* workspace, size_t workspace_bytes, void* stream) {
-  if (T < 0 || V < 1 || V > (1 << 30) || m < 0 || top < 0 || top > TOP_MAX || ld < 0 || (allowed && ld_allowed < 0)) return QMOE_EINVAL;
+  if (T < 0 || V < 1 || V > (1 << 30) || m < 0 || top < 0 || top > TOP_MAX || ld < 0 || (allowed && ld_allowed < 0) ||
+      !known_type(type))
+    return QMOE_EINVAL;
   if (T == 0) return QMOE_OK;
   if (!logits || !entropy || (m && (!tokens || !logprobs)) || (top && (!top_ids || !top_logprobs))) return QMOE_EINVAL;
   const size_t need = qmoe_token_logprobs_workspace(T, V, type, top);
-  if (need && (!workspace || workspace_bytes < need)) return QMOE_EWORKSPACE;
+  if (need && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15))) return QMOE_EWORKSPACE;
   LogprobArgs a = {};
   a.logits = logits, a.ld = ld, a.tokens = (const int64_t*)tokens, a.m = m;
   a.allowed = (const uint8_t*)allowed, a.lda = ld_allowed, a.T = T, a.V = V;
   a.logprobs = (float*)logprobs, a.entropy = (float*)entropy;
   a.top = top, a.top_ids = (int64_t*)top_ids, a.top_logprobs = (float*)top_logprobs;
-  if (type == QMOE_BF16) return launch<ElemBF16>(a, (hipStream_t)stream);
-  if (type == QMOE_F16) return launch<ElemF16>(a, (hipStream_t)stream);
-  if (type == QMOE_F32) return launch<ElemF32>(a, (hipStream_t)stream);
-  return QMOE_EINVAL;
+  if (type == QMOE_BF16) return dispatch<ElemBF16>(a, type, workspace, (hipStream_t)stream);
+  if (type == QMOE_F16) return dispatch<ElemF16>(a, type, workspace, (hipStream_t)stream);
+  return dispatch<ElemF32>(a, type, workspace, (hipStream_t)stream);
 }
 
 }  // extern "C"
