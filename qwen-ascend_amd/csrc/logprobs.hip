@@ -127,25 +127,36 @@ QMOE_DEV float wave_kth_logit(float l, int k) {
   return order_logit(o);
 }
 
-// Keeps the k best of a wave's n candidates (n >= k) and returns the logit of the last of them.
-QMOE_DEV float compact(uint64_t* cand, int n, int k) {
-  const int lane = threadIdx.x & 63;
-  uint64_t key[KEPT];
-#pragma unroll
-  for (int q = 0; q < KEPT; ++q) key[q] = q * 64 + lane < n ? cand[q * 64 + lane] : 0;
+// A key that the k best of a wave's distinct keys, N per lane, reach and no other does; 0 where
+// there are no more than k.
+template <int N>
+QMOE_DEV uint64_t wave_kth_key(const uint64_t (&key)[N], int k) {
   uint64_t kth = 0;
 #pragma unroll 1
   for (int b = 63; b >= 0; --b) {
     const uint64_t c = kth | (1ull << b);
     int count = 0;
 #pragma unroll
-    for (int q = 0; q < KEPT; ++q) count += __popcll(__ballot(key[q] >= c));
-    if (count >= k) kth = c;
+    for (int q = 0; q < N; ++q) count += __popcll(__ballot(key[q] >= c));
+    if (count < k) continue;
+    kth = c;
+    if (count == k) break;
   }
+  return kth;
+}
+
+// Keeps the k best of a wave's n candidates (n >= k); the least logit of them is at least the
+// returned one.
+QMOE_DEV float compact(uint64_t* cand, int n, int k) {
+  const int lane = threadIdx.x & 63;
+  uint64_t key[KEPT];
+#pragma unroll
+  for (int q = 0; q < KEPT; ++q) key[q] = q * 64 + lane < n ? cand[q * 64 + lane] : 0;
+  const uint64_t kth = wave_kth_key(key, k);
   int at = 0;
 #pragma unroll
   for (int q = 0; q < KEPT; ++q) {
-    const bool keep = key[q] >= kth;
+    const bool keep = key[q] && key[q] >= kth;
     const uint64_t mask = __ballot(keep);
     if (keep) cand[at + lanes_below(mask)] = key[q];
     at += __popcll(mask);
@@ -250,23 +261,33 @@ struct Stream {
       }
     }
     if (n > CAP) {
-      // Too many at once (equal or ascending logits): once more, keeping the k best as it fills.
+      // Too many at once (equal or ascending logits): once more, from the k-th best of the lanes'
+      // best keys on, which tell equal logits apart; keeping the k best if it fills all the same.
+      uint64_t best[1] = {0};
+#pragma unroll 1
+      for (int e = 0; e < J * P; ++e) {
+        const int id = first + e / P * stride + e % P;
+        const float l = logit(id);
+        if (l > tau && l >= floor) best[0] = max(best[0], key_of(l, id));
+      }
+      const uint64_t from = wave_kth_key(best, k);
       n = count;
 #pragma unroll 1
       for (int e = 0; e < J * P; ++e) {
         const int id = first + e / P * stride + e % P;
         const float l = logit(id);
-        bool in = l > tau && l >= floor;
+        const uint64_t key = key_of(l, id);
+        bool in = l > tau && l >= floor && key >= from;
         uint64_t mask = __ballot(in);
         if (n + __popcll(mask) > CAP) {
           const float kth = compact(cand, n, k);
           floor = fmaxf(floor, kth);
           next_tau = fmaxf(next_tau, kth);  // for what follows these logits, whose ids are in no order
           n = k;
-          in = l > tau && l >= floor;
+          in = in && l >= floor;
           mask = __ballot(in);
         }
-        if (in) cand[n + lanes_below(mask)] = key_of(l, id);
+        if (in) cand[n + lanes_below(mask)] = key;
         n += __popcll(mask);
       }
     }
@@ -310,19 +331,18 @@ QMOE_DEV void emit_row(const LogprobArgs& a, int t, Given g, Part p, float log_s
   }
 }
 
-// Ranks n candidates (distinct keys) by counting the greater ones, one wave; out(rank, key) for
-// the first k ranks, key 0 where there are fewer.
+// Ranks n candidates (distinct keys) by counting the greater ones, the whole workgroup;
+// out(rank, key) for the first k ranks, key 0 where there are fewer.
 template <typename F>
 QMOE_DEV void rank_top(const uint64_t* list, int n, int k, F out) {
-  const int lane = threadIdx.x & 63;
-  for (int c = 0; c < n; c += 64) {
-    const uint64_t mine = c + lane < n ? list[c + lane] : 0;
+  for (int c = threadIdx.x; c < n; c += THREADS) {
+    const uint64_t mine = list[c];
     int rank = 0;
 #pragma unroll 8
     for (int i = 0; i < n; ++i) rank += list[i] > mine;
-    if (mine && rank < k) out(rank, mine);
+    if (rank < k) out(rank, mine);
   }
-  if (lane >= n && lane < k) out(lane, 0);
+  if ((int)threadIdx.x >= n && (int)threadIdx.x < k) out(threadIdx.x, 0);
 }
 
 template <typename E>
@@ -439,18 +459,25 @@ __global__ __launch_bounds__(THREADS) void logprob_kernel(LogprobArgs a, int spl
     const float log_s = logf(p.s);
     if constexpr (TOP) {
       const float floor = wave_kth_logit<E>(tops.most(st.top), a.top);
+      int above = 0;
+      for (int i = 0; i < st.count; i += 64) {
+        const int at = i + (tid & 63);
+        above += __popcll(__ballot(at < st.count && key_logit(cand[wave][min(at, CAP - 1)]) >= floor));
+      }
+      if (above > 2 * TOP_MAX) {  // ranking many equal logits would take long
+        compact(cand[wave], st.count, a.top);
+        st.count = a.top;
+      }
       for (int i = tid & 63; i < st.count; i += 64) {
         const uint64_t key = cand[wave][i];
         if (key_logit(key) >= floor) list[atomicAdd(&listed, 1)] = key;
       }
       __syncthreads();
       tops.clear();  // for the next row
-      if (wave == 0) {
-        if (splits == 1)
-          rank_top(list, listed, a.top, [&](int r, uint64_t k) { emit_top(a, t, r, k, p, log_s, undefined); });
-        else
-          rank_top(list, listed, a.top, [&](int r, uint64_t k) { keys[unit * a.top + r] = k; });
-      }
+      if (splits == 1)
+        rank_top(list, listed, a.top, [&](int r, uint64_t k) { emit_top(a, t, r, k, p, log_s, undefined); });
+      else
+        rank_top(list, listed, a.top, [&](int r, uint64_t k) { keys[unit * a.top + r] = k; });
     }
     if (splits == 1) emit_row<E>(a, t, given, p, log_s, undefined);
     else if (tid == 0) parts[unit] = p;
@@ -471,29 +498,33 @@ __global__ __launch_bounds__(THREADS) void join_kernel(LogprobArgs a, int splits
   Part p = {-INFINITY, 0.f, 0.f};
   if (lane < splits) p = parts[(long)t * splits + lane];
   uint64_t key[TOP ? EACH : 1];
-  uint32_t floor = 0;
   if constexpr (TOP) {
     const uint64_t* mine = keys + (long)t * splits * a.top;
     // The parts' keys are in order, so where `lists` parts have an r-th key of at least a floor
     // and r * lists >= k, k keys reach it.
     const int r = (a.top + splits - 1) / splits, lists = (a.top + r - 1) / r;
-    const uint32_t rth = lane < splits ? (uint32_t)(mine[lane * a.top + r - 1] >> 32) : 0u;
+    const uint64_t rth = lane < splits ? mine[lane * a.top + r - 1] : 0;
 #pragma unroll
     for (int i = 0; i < EACH; ++i) key[i] = i * THREADS + tid < splits * a.top ? mine[i * THREADS + tid] : 0;
     if (tid == 0) listed = 0;
     constexpr int SH = KEY_SHIFT<E>;
-    floor = wave_kth<32 - SH>(rth >> SH, lists) << SH;
+    uint64_t floor = (uint64_t)(wave_kth<32 - SH>((uint32_t)(rth >> 32) >> SH, lists) << SH) << 32;
+    int above = 0;
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) above += __popcll(__ballot(key[i] && key[i] >= floor));
+    // many equal or ascending logits: ranking all of them would take long
+    if (above > 2 * TOP_MAX) floor = max(floor, wave_kth_key(key, a.top));
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < EACH; ++i)
-      if (key[i] && (uint32_t)(key[i] >> 32) >= floor) list[atomicAdd(&listed, 1)] = key[i];
+      if (key[i] && key[i] >= floor) list[atomicAdd(&listed, 1)] = key[i];
     __syncthreads();
   }
   p = wave_join(p);
   const bool undefined = !(p.s >= 0.f);
   const float log_s = logf(p.s);
   if constexpr (TOP) {
-    if (tid < 64) rank_top(list, listed, a.top, [&](int r, uint64_t k) { emit_top(a, t, r, k, p, log_s, undefined); });
+    rank_top(list, listed, a.top, [&](int r, uint64_t k) { emit_top(a, t, r, k, p, log_s, undefined); });
   }
   emit_row<E>(a, t, given, p, log_s, undefined);
 }

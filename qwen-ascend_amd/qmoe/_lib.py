@@ -138,14 +138,23 @@ def stream_of(t: torch.Tensor) -> int:
     return _RAW_STREAM(i)
 
 
-def on_device_of(t: torch.Tensor, fn, *args):
-    """fn(*args), a launch on t's device: with that device current, as a launch on
-    its streams needs, where another one is."""
+def operands(t: torch.Tensor, *others) -> bool:
+    """Checks the operands of a forward-only operator (None: not given): device
+    tensors on one device, none of which asks for a gradient. False where that
+    device is not the current one, which a launch on its streams needs."""
     i = t.get_device()
-    if i == torch.cuda.current_device():
-        return fn(*args)
-    with torch.cuda.device(i):
-        return fn(*args)
+    graded = t.requires_grad
+    for o in others:
+        if o is not None:
+            if o.get_device() != i:
+                raise RuntimeError("qmoe ops take device tensors" if i < 0 or o.get_device() < 0 else
+                                   "all tensors must be on the same device")
+            graded = graded or o.requires_grad
+    if i < 0:
+        raise RuntimeError("qmoe ops take device tensors")
+    if graded and torch.is_grad_enabled():
+        raise RuntimeError("this operator has no backward pass: call it under torch.no_grad()")
+    return i == torch.cuda.current_device()
 
 
 def ptr(t) -> int | None:

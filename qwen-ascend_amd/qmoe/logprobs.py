@@ -13,7 +13,6 @@ from typing import NamedTuple, Optional
 import torch
 
 from . import _lib
-from .norms import _check_tensors
 
 _TYPES = _lib.TYPES
 TOP_MAX = 32
@@ -60,11 +59,13 @@ def token_logprobs(logits, tokens=None, *, top=0, allowed=None):
             raise RuntimeError(f"tokens {tuple(tokens.shape)} do not match logits {tuple(logits.shape)}")
     if allowed is not None and (allowed.dtype != torch.bool or allowed.shape not in ((V,), logits.shape)):
         raise RuntimeError("allowed must be bool [V] or of the logits' shape")
-    _check_tensors(logits, tokens, allowed)
+    if not _lib.operands(logits, tokens, allowed):
+        with torch.cuda.device(logits.device):
+            return token_logprobs(logits, tokens, top=top, allowed=allowed)
     x = logits if logits.dim() == 2 else logits.reshape(-1, V)
     if x.stride(1) != 1 and V != 1:
         x = x.contiguous()
-    T, dev = x.shape[0], x.device
+    T = x.shape[0]
     if T >= 1 << 31:
         raise RuntimeError("logits must have fewer than 2^31 rows")
     lda = 0
@@ -75,19 +76,20 @@ def token_logprobs(logits, tokens=None, *, top=0, allowed=None):
         if allowed.stride(-1) != 1 and V != 1:
             allowed = allowed.contiguous()
             lda = V if allowed.dim() > 1 else 0
+    logprobs = top_ids = top_lp = ws = None
     if tokens is not None:
         tokens = tokens.contiguous()
-    logprobs = None if tokens is None else torch.empty(tokens.shape, dtype=torch.float32, device=dev)
-    entropy = torch.empty(lead, dtype=torch.float32, device=dev)
-    top_ids = top_lp = None
+        logprobs = x.new_empty(tokens.shape, dtype=torch.float32)
+    entropy = x.new_empty(lead, dtype=torch.float32)
     if top:
-        top_ids = torch.empty((*lead, top), dtype=torch.int64, device=dev)
-        top_lp = torch.empty((*lead, top), dtype=torch.float32, device=dev)
+        top_ids = x.new_empty((*lead, top), dtype=torch.int64)
+        top_lp = x.new_empty((*lead, top), dtype=torch.float32)
     L = _lib.lib()
     kind, ptr = _TYPES[x.dtype], _lib.ptr
     nbytes = L.qmoe_token_logprobs_workspace(T, V, kind, top)
-    ws = _lib.workspace(dev, nbytes) if nbytes else None
-    _lib.check(_lib.on_device_of(x, L.qmoe_token_logprobs, x.data_ptr(), x.stride(0), kind, ptr(tokens), m,
-                                 ptr(allowed), lda, T, V, ptr(logprobs), entropy.data_ptr(), top, ptr(top_ids),
-                                 ptr(top_lp), ptr(ws), nbytes, _lib.stream_of(x)), "token_logprobs")
+    if nbytes:
+        ws = x.new_empty(nbytes, dtype=torch.uint8)  # from the caching allocator: aligned, its own in every graph
+    _lib.check(L.qmoe_token_logprobs(x.data_ptr(), x.stride(0), kind, ptr(tokens), m, ptr(allowed), lda, T, V,
+                                     ptr(logprobs), entropy.data_ptr(), top, ptr(top_ids), ptr(top_lp), ptr(ws), nbytes,
+                                     _lib.stream_of(x)), "token_logprobs")
     return TokenLogprobs(logprobs, entropy, top_ids, top_lp)

@@ -16,7 +16,6 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from .ops import _same_device
 
 _TYPES = _lib.TYPES
 H_MAX = 32768
@@ -44,16 +43,6 @@ def _check_row_tensor(t, what):
         raise RuntimeError(f"{what} must be [..., H] with 1 <= H <= {H_MAX}")
 
 
-def _check_tensors(*ts):
-    for t in ts:
-        if t is not None:
-            if not t.is_cuda:
-                raise RuntimeError("qmoe ops take device tensors")
-            if t.requires_grad and torch.is_grad_enabled():
-                raise RuntimeError("this operator has no backward pass: call it under torch.no_grad()")
-    _same_device(*ts)
-
-
 def block_norm(x, weight, *, eps=1e-6, offset=0.0, out_dtype=None):
     """The norm before a block: n(x; weight) for rows x [..., H].
 
@@ -62,22 +51,27 @@ def block_norm(x, weight, *, eps=1e-6, offset=0.0, out_dtype=None):
     32-bit residual stream normed to the block's type). ``eps`` >= 1e-30. Returns a
     contiguous tensor of x's shape."""
     _check_row_tensor(x, "x")
-    H = x.shape[-1]
-    out_dtype = x.dtype if out_dtype is None else out_dtype
-    if out_dtype not in _TYPES or (out_dtype != x.dtype and x.dtype != torch.float32):
+    H, xt = x.shape[-1], x.dtype
+    if out_dtype is None:
+        out_dtype = xt
+    elif out_dtype not in _TYPES or (out_dtype != xt and xt != torch.float32):
         raise RuntimeError("out_dtype must be x's type, or bfloat16 or float16 for a float32 x")
     weight = _check_weight(weight, H, "weight")
-    _check_tensors(x, weight)
-    out = torch.empty(x.shape, dtype=out_dtype, device=x.device)
+    if not _lib.operands(x, weight):
+        with torch.cuda.device(x.device):
+            return block_norm(x, weight, eps=eps, offset=offset, out_dtype=out_dtype)
+    out = x.new_empty(x.shape, dtype=out_dtype)
     x = _rows(x, H)
-    _lib.check(_lib.on_device_of(x, _lib.lib().qmoe_block_norm, x.data_ptr(), x.stride(0), _TYPES[x.dtype],
-                                 weight.data_ptr(), _TYPES[weight.dtype], out.data_ptr(), H, _TYPES[out_dtype],
-                                 x.shape[0], H, eps, offset, _lib.stream_of(x)), "block_norm")
+    _lib.check(_lib.lib().qmoe_block_norm(x.data_ptr(), x.stride(0), _TYPES[xt], weight.data_ptr(),
+                                          _TYPES[weight.dtype], out.data_ptr(), H, _TYPES[out_dtype], x.shape[0], H, eps,
+                                          offset, _lib.stream_of(x)), "block_norm")
     return out
 
 
 def _gate_steps(gate, shape, H):
     """The gate as (tensor, row step, column step) of the rows of ``shape``."""
+    if len(shape) == 2 and gate.shape == (shape[0], 1):  # one per row, the common one: no view made
+        return gate, gate.stride(0), 0
     try:
         g = gate.expand(shape)
     except RuntimeError:
@@ -99,6 +93,14 @@ def _span(t):
     return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
 
 
+def _other_columns(rows, t):
+    """Whether t's rows lie beside those of ``rows``, as columns of the same wider rows."""
+    if t.dim() != 2 or t.stride(0) != rows.stride(0) or t.dtype != rows.dtype or t.stride(1) not in (0, 1):
+        return False
+    column = (t.data_ptr() - rows.data_ptr()) // t.element_size() % rows.stride(0)
+    return column >= rows.shape[1] and column + (t.shape[1] if t.stride(1) else 1) <= rows.stride(0)
+
+
 def _inplace_rows(residual, H, others):
     """Rows of a residual that is written in place: a view of it, apart from each other and from
     every other operand (y may be the residual itself)."""
@@ -106,13 +108,14 @@ def _inplace_rows(residual, H, others):
     if rows.shape[0] and ((rows.stride(1) != 1 and H != 1) or (rows.stride(0) < H and rows.shape[0] > 1)):
         raise RuntimeError("inplace needs a residual of rows with contiguous elements that do not overlap")
     lo, hi = _span(rows)
-    for t, same_is_fine in others:
+    for t, itself_is_fine in others:
         if t is None:
             continue
         a, b = _span(t)
-        if a < hi and lo < b and not (same_is_fine and a == lo and t.dtype == rows.dtype
-                                      and t.stride() == residual.stride()):
-            raise RuntimeError("inplace: the residual overlaps another operand")
+        if a < hi and lo < b and not _other_columns(rows, t):
+            itself = a == lo and t.dtype == rows.dtype and t.shape == residual.shape and t.stride() == residual.stride()
+            if not (itself_is_fine and itself):
+                raise RuntimeError("inplace: the residual overlaps another operand")
     return rows
 
 
@@ -143,7 +146,10 @@ def block_residual(y, residual, *, post_weight=None, gate=None, gate_act=None, s
         post_weight = _check_weight(post_weight, H, "post_weight")
     if next_weight is not None:
         next_weight = _check_weight(next_weight, H, "next_weight")
-    _check_tensors(y, residual, post_weight, gate, next_weight)
+    if not _lib.operands(y, residual, post_weight, gate, next_weight):
+        with torch.cuda.device(y.device):
+            return block_residual(y, residual, post_weight=post_weight, gate=gate, gate_act=gate_act, scale=scale,
+                                  next_weight=next_weight, eps=eps, offset=offset, inplace=inplace)
     g, g_row, g_col = (None, 0, 0) if gate is None else _gate_steps(gate, y.shape, H)
     if inplace:
         h = residual
@@ -152,14 +158,14 @@ def block_residual(y, residual, *, post_weight=None, gate=None, gate_act=None, s
         if not residual.is_inference():
             torch.autograd.graph.increment_version(residual)
     else:
-        hr = h = torch.empty(residual.shape, dtype=residual.dtype, device=residual.device)
+        hr = h = residual.new_empty(residual.shape)
         res = _rows(residual, H)
         ldr, ldh = res.stride(0), H
-    x = None if next_weight is None else torch.empty(y.shape, dtype=y.dtype, device=y.device)
+    x = None if next_weight is None else y.new_empty(y.shape)
     y = _rows(y, H)
     ptr = _lib.ptr
-    _lib.check(_lib.on_device_of(
-        y, _lib.lib().qmoe_block_residual, y.data_ptr(), y.stride(0), _TYPES[y.dtype], res.data_ptr(), ldr,
+    _lib.check(_lib.lib().qmoe_block_residual(
+        y.data_ptr(), y.stride(0), _TYPES[y.dtype], res.data_ptr(), ldr,
         _TYPES[res.dtype], ptr(post_weight), 0 if post_weight is None else _TYPES[post_weight.dtype], ptr(g), g_row,
         g_col, 0 if g is None else _TYPES[g.dtype], int(gate_act == "sigmoid"), scale, hr.data_ptr(), ldh,
         ptr(next_weight), 0 if next_weight is None else _TYPES[next_weight.dtype], ptr(x), H, y.shape[0], H, eps,

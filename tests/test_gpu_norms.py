@@ -237,6 +237,38 @@ def test_next_norm_is_block_norm(device):
 
 
 @pytest.mark.gpu
+def test_inplace_beside_its_operands(device):
+    """y, the residual and a gate as columns of one tensor."""
+    from qmoe import block_residual
+    n = gen(device, 31)
+    wide = n(700, 1025 + 2 * 512)
+    y, r, gate = wide[:, :512], wide[:, 512:1024], wide[:, 1024:1025]
+    keep, want = wide.clone(), R.block_residual(y, r, gate=gate, gate_act="sigmoid")
+    check_residual(block_residual(y, r, gate=gate, gate_act="sigmoid", inplace=True), want, "beside")
+    assert torch.equal(wide[:, :512], keep[:, :512]) and torch.equal(wide[:, 1024:], keep[:, 1024:])
+
+
+@pytest.mark.gpu
+def test_other_device(device, monkeypatch):
+    """Tensors of a device that is not the current one: the call is made again with it current."""
+    from qmoe import _lib, block_norm, block_residual, token_logprobs
+    n = gen(device, 41)
+    x, w = n(5, 640), n(640)
+    tok = torch.zeros(5, dtype=torch.int64, device=device)
+    calls = (lambda: block_norm(x, w, offset=1.0), lambda: block_residual(x, x, post_weight=w, scale=0.5, next_weight=w),
+             lambda: token_logprobs(x, tok, top=3))
+    want = [c() for c in calls]
+    current = torch.cuda.current_device
+    for c, e in zip(calls, want):
+        answers = iter([1])
+        monkeypatch.setattr(torch.cuda, "current_device", lambda: next(answers, current()))
+        got = c()
+        assert next(answers, None) is None
+        for a, b in zip(got if isinstance(got, tuple) else (got,), e if isinstance(e, tuple) else (e,)):
+            assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
 def test_norms_with_gradients(device):
     from qmoe import block_norm, block_residual
     w = torch.ones(16, device=device, requires_grad=True)

@@ -70,24 +70,49 @@ def test_inplace_overlap():
         with pytest.raises(RuntimeError, match="overlaps"):
             _inplace_rows(r, 8, ((other, fine),))
     _inplace_rows(r, 8, ((base[32:].view(4, 8), False),))
+    wide = t(4, 20)                       # columns of the same rows, beside each other or not
+    r = wide[:, 2:10]
+    for cols, fine in ((slice(10, 18), True), (slice(12, 20), True), (slice(9, 17), False), (slice(0, 2), True),
+                       (slice(1, 3), False), (slice(18, 20), True)):
+        if fine:
+            _inplace_rows(r, 8, ((wide[:, cols], False),))
+        else:
+            with pytest.raises(RuntimeError, match="overlaps"):
+                _inplace_rows(r, 8, ((wide[:, cols], True),))
+    _inplace_rows(r, 8, ((wide[:, 19:].expand(4, 8), False),))      # one gate per row, beside the rows
+    with pytest.raises(RuntimeError, match="overlaps"):
+        _inplace_rows(r, 8, ((wide[:, 9:10].expand(4, 8), False),))
+    with pytest.raises(RuntimeError, match="overlaps"):             # wraps into the next row
+        _inplace_rows(r, 8, ((wide.view(-1)[18:18 + 60].view(3, 20)[:, :6], False),))
     with pytest.raises(RuntimeError, match="do not overlap"):
         _inplace_rows(t(1, 8).expand(4, 8), 8, ())
     with pytest.raises(RuntimeError, match="do not overlap"):
         _inplace_rows(base[:32].view(8, 4).t(), 8, ())
 
 
-def test_gradients_are_refused():
-    from qmoe.norms import _check_tensors
+class Operand:
+    def __init__(self, device=0, requires_grad=False):
+        self.device_index, self.requires_grad = device, requires_grad
 
-    class Leaf:
-        is_cuda, requires_grad = True, True
+    def get_device(self):
+        return self.device_index
 
-        def get_device(self):
-            return 0
-    with pytest.raises(RuntimeError, match="no backward pass"):
-        _check_tensors(Leaf())
+
+def test_operands(monkeypatch):
+    """Gradients, host tensors and two devices are refused; another device than the current one is
+    told apart."""
+    from qmoe import _lib
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    assert _lib.operands(Operand(), None, Operand()) is True
+    assert _lib.operands(Operand(1), Operand(1)) is False
+    for ops, says in (([Operand(-1)], "device tensors"), ([Operand(), Operand(-1)], "device tensors"),
+                      ([Operand(-1), Operand()], "device tensors"), ([Operand(), None, Operand(1)], "same device"),
+                      ([Operand(requires_grad=True)], "no backward pass"),
+                      ([Operand(), Operand(requires_grad=True)], "no backward pass")):
+        with pytest.raises(RuntimeError, match=says):
+            _lib.operands(*ops)
     with torch.no_grad():
-        _check_tensors(Leaf())
+        assert _lib.operands(Operand(requires_grad=True), Operand(requires_grad=True))
 
 
 def test_c_entries_refuse_before_any_launch():
