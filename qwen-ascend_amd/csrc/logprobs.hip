@@ -4,6 +4,15 @@
 //
 // over the allowed v, from m = max l, S = sum e^(l - m), D = sum e^(l - m) (l - m) (base 2
 // inside): logprob(v) = (l_v - m) - ln S, entropy = ln S - D / S. Sums in fp32.
+//
+// The logits are read once, 16 bytes per load; each lane keeps the running m, S and D of what it
+// has read, taken to a new maximum once per step of 4 loads. The top alternatives are found in the
+// same pass: a wave keeps as candidates only the logits that reach a bound which k logits of the
+// row are known to reach, and the few that are left at the end are ranked by counting. Many rows
+// are bound by HBM, with about ten vector operations per logit close behind (4096 x 131072 bf16:
+// 191 us, 5.6 TB/s, top 20 222 us; 1024 x 65536 fp32, top 20: 52 us, 5.2 TB/s); few rows are split
+// over the chip and joined by a second launch, bound by the two launches' latency (1 x 131072, top
+// 20: 9.4 us, none 4.9).
 #include "elem_types.h"
 
 #include <algorithm>
@@ -102,6 +111,12 @@ constexpr int KEY_SHIFT<ElemF16> = 13;
 QMOE_DEV uint32_t order_of(float l) { return (uint32_t)(key_of(l, 0) >> 32); }
 QMOE_DEV float order_logit(uint32_t o) { return key_logit((uint64_t)o << 32); }
 
+// The least float above a value below infinity.
+QMOE_DEV float just_above(float v) {
+  const int b = __float_as_int(v + 0.f);
+  return __int_as_float(b >= 0 ? b + 1 : b - 1);
+}
+
 QMOE_DEV int lanes_below(uint64_t mask) {
   return __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0));
 }
@@ -127,8 +142,8 @@ QMOE_DEV float wave_kth_logit(float l, int k) {
   return order_logit(o);
 }
 
-// A key that the k best of a wave's distinct keys, N per lane, reach and no other does; 0 where
-// there are no more than k.
+// A key that the k best of a wave's distinct keys, N per lane, reach and no other does (the
+// bits are tried from the top until exactly k are left); 0 where there are fewer than k.
 template <int N>
 QMOE_DEV uint64_t wave_kth_key(const uint64_t (&key)[N], int k) {
   uint64_t kth = 0;
@@ -145,8 +160,8 @@ QMOE_DEV uint64_t wave_kth_key(const uint64_t (&key)[N], int k) {
   return kth;
 }
 
-// Keeps the k best of a wave's n candidates (n >= k); the least logit of them is at least the
-// returned one.
+// Keeps the k best of a wave's n candidates (n >= k). Returns a bound that their logits reach
+// (the logit of no key, even NaN, where the bits end early: fmaxf with it is still a bound).
 QMOE_DEV float compact(uint64_t* cand, int n, int k) {
   const int lane = threadIdx.x & 63;
   uint64_t key[KEPT];
@@ -245,14 +260,15 @@ struct Stream {
     floor = fmaxf(floor, wave_kth_logit<E>(tops->raise(top), k));
     // enough lanes of this wave reach the floor: what follows has to exceed it
     float next_tau = __popcll(__ballot(top >= floor)) >= k ? floor : tau;
+    const float least = floor > tau ? floor : just_above(tau);
     int n = count;
 #pragma unroll
     for (int j = 0; j < J; ++j) {
-      if (!__any(piece_most[j] > tau && piece_most[j] >= floor)) continue;
+      if (!__any(piece_most[j] >= least)) continue;
 #pragma unroll
       for (int i = 0; i < P; ++i) {
         const float l = x.get(j, i);
-        const bool in = l > tau && l >= floor;
+        const bool in = l >= least;
         const uint64_t mask = __ballot(in);
         if (mask == 0) continue;
         const int at = n + lanes_below(mask);
@@ -268,7 +284,7 @@ struct Stream {
       for (int e = 0; e < J * P; ++e) {
         const int id = first + e / P * stride + e % P;
         const float l = logit(id);
-        if (l > tau && l >= floor) best[0] = max(best[0], key_of(l, id));
+        if (l >= least) best[0] = max(best[0], key_of(l, id));
       }
       const uint64_t from = wave_kth_key(best, k);
       n = count;
@@ -277,7 +293,7 @@ struct Stream {
         const int id = first + e / P * stride + e % P;
         const float l = logit(id);
         const uint64_t key = key_of(l, id);
-        bool in = l > tau && l >= floor && key >= from;
+        bool in = l >= least && key >= from;
         uint64_t mask = __ballot(in);
         if (n + __popcll(mask) > CAP) {
           const float kth = compact(cand, n, k);
@@ -485,7 +501,7 @@ __global__ __launch_bounds__(THREADS) void logprob_kernel(LogprobArgs a, int spl
   }
 }
 
-constexpr int MAX_SPLITS = 64;
+constexpr int MAX_SPLITS = 64;  // one part per lane of the joining wave
 
 // Joins the parts of a row: their sums and their ordered best candidates.
 template <typename E, bool TOP>
@@ -530,10 +546,11 @@ __global__ __launch_bounds__(THREADS) void join_kernel(LogprobArgs a, int splits
 }
 
 // Pieces per part of a row: whole steps of 4 pieces per thread, or one step of 2 or 1 where that
-// leaves too few workgroups, so that there are about 1024 of them, four per CU (V = 131072 in
-// bf16, top 20, in 1, 2, 4, 8, 16, 32, 64 parts: 48 rows 33.6, 26.3, 19.6, 16.1, 14.6, 14.9 and
-// 18.9 us; 256 rows 38.6, 32.5, 28.4, 32.2, 38.1, 42.2 and 61.8; 1024 rows 62.6, 71.5, 78.9 ...).
-// Without top alternatives 512 rows are enough (512 rows in one part: 29.7 us, in two 32.6).
+// leaves too few workgroups, so that there are about 1024 of them, four per CU. V = 131072 in
+// bf16, top 20, in 1, 2, 4, 8, 16, 32, 64 parts: 1 row 26.9, 20.9, 15.9, 12.5, 10.7, 9.9 and 9.4
+// us; 48 rows 31.2, 24.5, 18.3, 15.7, 14.4, 14.9 and 20.2; 256 rows 36.1, 31.4, 27.1, 30.2, 36.8,
+// 41.4 and 69.1; 1024 rows 62.6, 70.7, 77.5, 86.7, 110, 132 and 249. Without top alternatives
+// 512 rows are enough for whole ones (one part 29.8 us, two 32.6).
 int part_pieces(int T, int V, int type, int top) {
   const int pieces = V / (type == QMOE_F32 ? 4 : 8), full = 4 * THREADS;
   const int want = T >= (top ? 1024 : 512) ? 1 : std::min(host_ceil_div(1024, T), MAX_SPLITS);

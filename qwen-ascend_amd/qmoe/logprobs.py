@@ -36,7 +36,7 @@ def token_logprobs(logits, tokens=None, *, top=0, allowed=None):
 
     allowed: bool [V] or of the logits' shape; where it is False a token is out, whatever its
     logit holds. A row with no token left: its tokens -inf, entropy 0. A row with NaN or +inf
-    at an allowed place has no distribution: NaN everywhere and ids -1. The sums are fp32:
+    at an allowed place has no distribution: NaN (padding still 0) and ids -1. The sums are fp32:
     log probabilities and entropies are exact to a few 2^-22 absolute.
     """
     if logits.dtype not in _TYPES:
