@@ -68,18 +68,24 @@ QMOE_DEV T row_sum(T v, T* lds, int waves) {
 struct Rms {
   float pre, r;
 };
+template <typename T, int N>
+QMOE_DEV T squares(const float (&v)[N]) {
+  T s = 0;
+#pragma unroll
+  for (int i = 0; i < N; ++i) s += (T)v[i] * (T)v[i];
+  return s;
+}
+// mine(T()): the squares of this thread's places in T
+template <bool ONE_WAVE, typename F>
+QMOE_DEV Rms rms_of(F mine, int H, float eps, float* lds, double* lds64, int waves) {
+  const float s = row_sum<ONE_WAVE>(mine(0.f), lds, waves);
+  if (s <= FLT_MAX) return {1.f, 1.f / sqrtf(s / (float)H + eps)};
+  const double d = row_sum<ONE_WAVE>(mine(0.0), lds64, waves);
+  return {0x1p-60f, (float)(0x1p60 / sqrt(d / H + eps))};
+}
 template <bool ONE_WAVE, int N>
 QMOE_DEV Rms row_rms(const float (&v)[N], int H, float eps, float* lds, double* lds64, int waves) {
-  float s = 0.f;
-#pragma unroll
-  for (int i = 0; i < N; ++i) s += v[i] * v[i];
-  s = row_sum<ONE_WAVE>(s, lds, waves);
-  if (s <= FLT_MAX) return {1.f, 1.f / sqrtf(s / (float)H + eps)};
-  double d = 0.0;
-#pragma unroll
-  for (int i = 0; i < N; ++i) d += (double)v[i] * v[i];
-  d = row_sum<ONE_WAVE>(d, lds64, waves);
-  return {0x1p-60f, (float)(0x1p60 / sqrt(d / H + eps))};
+  return rms_of<ONE_WAVE>([&](auto zero) { return squares<decltype(zero)>(v); }, H, eps, lds, lds64, waves);
 }
 
 // N elements of a tensor whose type is known at run time only.
@@ -144,13 +150,14 @@ struct RowIn {
   AnyVec<N> g[MODE == SUM_GATED ? NV : 1];
   float y_end, r_end, g_end;
 
-  QMOE_DEV void load(const NormArgs& a, long row, int tpr, int tid, int whole) {
+  // Pieces from column `begin` on; the row's last elements with them where `ends`.
+  QMOE_DEV void load(const NormArgs& a, long row, int tpr, int tid, int whole, int begin = 0, bool ends = true) {
     const auto* yp = static_cast<const typename Y::raw*>(a.y) + row * a.ldy;
     const auto* rp = static_cast<const typename R::raw*>(a.r) + row * a.ldr;
     const long gp = row * a.ldg;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      const int c = (j * tpr + tid) * N;
+      const int c = begin + (j * tpr + tid) * N;
       r[j].zero();
       if constexpr (MODE != NORM) y[j].zero();
       if constexpr (MODE == SUM_GATED) g[j].v.zero();
@@ -162,13 +169,47 @@ struct RowIn {
     }
     y_end = r_end = g_end = 0.f;
     const int last = whole + tid;
-    if (last < a.H) {
+    if (ends && last < a.H) {
       r_end = R::load(rp[last]);
       if constexpr (MODE != NORM) y_end = Y::load(yp[last]);
       if constexpr (MODE == SUM_GATED) g_end = load_typed(a.gate, gp + last, a.gate_type);
     }
     if constexpr (MODE == SUM)
       if (a.gate) g_end = load_typed(a.gate, gp, a.gate_type);
+  }
+
+  // What is normed first: y, or the residual where there is no y.
+  QMOE_DEV void unpack(float (&v)[NV * N + 1]) const {
+#pragma unroll
+    for (int i = 0; i < NV * N; ++i) {
+      if constexpr (MODE == NORM) v[i] = r[i / N].template get<R>(i % N);
+      else v[i] = y[i / N].template get<Y>(i % N);
+    }
+    v[NV * N] = MODE == NORM ? r_end : y_end;
+  }
+
+  // v, the block's (normed) output, becomes r + scale * a(gate) * v.
+  QMOE_DEV void sum(const NormArgs& a, float (&v)[NV * N + 1]) const {
+    float scale = a.scale;
+    if constexpr (MODE == SUM) {
+      if (a.gate) scale *= a.gate_sigmoid ? sigmoid(g_end) : g_end;
+    } else {
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        float f[N];
+        g[j].unpack(f, a.gate_type);
+        if (a.gate_sigmoid) {
+#pragma unroll
+          for (int i = 0; i < N; ++i) f[i] = sigmoid(f[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[j * N + i] *= f[i];
+      }
+      v[NV * N] *= a.gate_sigmoid ? sigmoid(g_end) : g_end;
+    }
+#pragma unroll
+    for (int i = 0; i < NV * N; ++i) v[i] = r[i / N].template get<R>(i % N) + scale * v[i];
+    v[NV * N] = r_end + scale * v[NV * N];
   }
 };
 
@@ -177,14 +218,14 @@ template <int NV, int N>
 struct Weights {
   AnyVec<N> w[NV];
   float end;
-  QMOE_DEV void load(const void* p, int type, int H, int tpr, int tid, int whole) {
+  QMOE_DEV void load(const void* p, int type, int H, int tpr, int tid, int whole, int begin = 0, bool ends = true) {
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      const int c = (j * tpr + tid) * N;
+      const int c = begin + (j * tpr + tid) * N;
       w[j].v.zero();
       if (c < whole) w[j].load(p, c, type);
     }
-    end = whole + tid < H ? load_typed(p, whole + tid, type) : 0.f;
+    end = ends && whole + tid < H ? load_typed(p, whole + tid, type) : 0.f;
   }
   // v = v * m * (offset + w)
   QMOE_DEV void apply(float (&v)[NV * N + 1], const Rms m, float offset, int type) {
@@ -201,13 +242,14 @@ struct Weights {
 };
 
 template <typename E, int NV, int N>
-QMOE_DEV void store_row(const float (&v)[NV * N + 1], typename E::raw* p, int H, int tpr, int tid, int whole) {
+QMOE_DEV void store_row(const float (&v)[NV * N + 1], typename E::raw* p, int H, int tpr, int tid, int whole, int begin = 0,
+                        bool ends = true) {
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
-    const int c = (j * tpr + tid) * N;
+    const int c = begin + (j * tpr + tid) * N;
     if (c < whole) store_piece<E, N>(v + j * N, p + c);
   }
-  if (whole + tid < H) p[whole + tid] = E::store(v[NV * N]);
+  if (ends && whole + tid < H) p[whole + tid] = E::store(v[NV * N]);
 }
 
 // Places behind the row hold zeros and stay zero through all of it (or turn NaN only where a
@@ -234,35 +276,10 @@ __global__ __launch_bounds__(MAX_WAVES == 1 ? 256 : 64 * MAX_WAVES) void norm_ro
     RowIn<Y, R, NV, MODE> ahead;
     if (AHEAD && following < a.rows) ahead.load(a, following, tpr, tid, whole);
     float v[L + 1];
-    if constexpr (MODE == NORM) {
-#pragma unroll
-      for (int i = 0; i < L; ++i) v[i] = in.r[i / N].template get<R>(i % N);
-      v[L] = in.r_end;
-    } else {
-#pragma unroll
-      for (int i = 0; i < L; ++i) v[i] = in.y[i / N].template get<Y>(i % N);
-      v[L] = in.y_end;
+    in.unpack(v);
+    if constexpr (MODE != NORM) {
       if (a.post) post.apply(v, row_rms<ONE_WAVE>(v, a.H, a.eps, lds[0], lds64[0], waves), a.offset, a.post_type);
-      float scale = a.scale;
-      if constexpr (MODE == SUM) {
-        if (a.gate) scale *= a.gate_sigmoid ? sigmoid(in.g_end) : in.g_end;
-      } else {
-#pragma unroll
-        for (int j = 0; j < NV; ++j) {
-          float g[N];
-          in.g[j].unpack(g, a.gate_type);
-          if (a.gate_sigmoid) {
-#pragma unroll
-            for (int i = 0; i < N; ++i) g[i] = sigmoid(g[i]);
-          }
-#pragma unroll
-          for (int i = 0; i < N; ++i) v[j * N + i] *= g[i];
-        }
-        v[L] *= a.gate_sigmoid ? sigmoid(in.g_end) : in.g_end;
-      }
-#pragma unroll
-      for (int i = 0; i < L; ++i) v[i] = in.r[i / N].template get<R>(i % N) + scale * v[i];
-      v[L] = in.r_end + scale * v[L];
+      in.sum(a, v);
       store_row<R, NV, N>(v, static_cast<typename R::raw*>(a.h) + row * a.ldh, a.H, tpr, tid, whole);
     }
     if (a.next) {
@@ -277,55 +294,62 @@ __global__ __launch_bounds__(MAX_WAVES == 1 ? 256 : 64 * MAX_WAVES) void norm_ro
   }
 }
 
-// Rows longer than a workgroup's registers hold: each pass over the row reads it again.
+// Rows longer than a workgroup's registers hold: the same in steps of a piece per thread, each
+// pass over the row reading it again (from the caches; 2048 x 32768 bf16: norm 62.9 us, 4.3 TB/s,
+// the whole step after a block 157 us, 3.4 TB/s).
 constexpr int WIDE_THREADS = 1024;
-template <typename F>
-QMOE_DEV Rms wide_rms(F value, int H, float eps, float* lds, double* lds64) {
-  float s = 0.f;
-  for (int i = threadIdx.x; i < H; i += WIDE_THREADS) {
-    const float v = value(i);
-    s += v * v;
-  }
-  s = row_sum<false>(s, lds, WIDE_THREADS / 64);
-  if (s <= FLT_MAX) return {1.f, 1.f / sqrtf(s / (float)H + eps)};
-  double d = 0.0;
-  for (int i = threadIdx.x; i < H; i += WIDE_THREADS) {
-    const double v = value(i);
-    d += v * v;
-  }
-  d = row_sum<false>(d, lds64, WIDE_THREADS / 64);
-  return {0x1p-60f, (float)(0x1p60 / sqrt(d / H + eps))};
-}
-
-template <typename Y, typename R>
+template <typename Y, typename R, int MODE>
 __global__ __launch_bounds__(WIDE_THREADS) void norm_wide_kernel(NormArgs a) {
-  __shared__ float lds[2][16];
-  __shared__ double lds64[2][16];
+  constexpr int N = VE<Y>, SPAN = WIDE_THREADS * N, WAVES = WIDE_THREADS / 64;
+  __shared__ float lds[2][WAVES];
+  __shared__ double lds64[2][WAVES];
+  const int tid = threadIdx.x, whole = a.H / N * N;
   for (long row = blockIdx.x; row < a.rows; row += gridDim.x) {
-    const auto* y = static_cast<const typename Y::raw*>(a.y) + row * a.ldy;
-    const auto* r = static_cast<const typename R::raw*>(a.r) + row * a.ldr;
-    Rms post = {1.f, 1.f}, next = {1.f, 1.f};
-    if (a.post) post = wide_rms([&](int i) { return Y::load(y[i]); }, a.H, a.eps, lds[0], lds64[0]);
-    auto sum = [&](int i) {
-      const float res = R::load(r[i]);
-      if (!a.y) return res;
-      float p = Y::load(y[i]);
-      if (a.post) p = p * post.pre * post.r * (a.offset + load_typed(a.post, i, a.post_type));
-      float scale = a.scale;
-      if (a.gate) {
-        const float g = load_typed(a.gate, row * a.ldg + (long)i * a.gate_step, a.gate_type);
-        scale *= a.gate_sigmoid ? sigmoid(g) : g;
+    RowIn<Y, R, 1, MODE> in;
+    Weights<1, N> w;
+    float v[N + 1];
+    Rms post = {1.f, 1.f};
+    auto each = [&](auto f) {
+      for (int c = 0; c < whole; c += SPAN) {
+        const bool ends = c + SPAN >= whole;
+        in.load(a, row, WIDE_THREADS, tid, whole, c, ends);
+        in.unpack(v);
+        f(c, ends);
       }
-      return res + scale * p;
     };
-    if (a.next) next = wide_rms(sum, a.H, a.eps, lds[1], lds64[1]);
-    for (int i = threadIdx.x; i < a.H; i += WIDE_THREADS) {  // h may overwrite r: each place by its own thread
-      const float h = sum(i);
-      if (a.h) static_cast<typename R::raw*>(a.h)[row * a.ldh + i] = R::store(h);
-      if (a.next)
-        static_cast<typename Y::raw*>(a.x)[row * a.ldx + i] =
-            Y::store(h * next.pre * next.r * (a.offset + load_typed(a.next, i, a.next_type)));
-    }
+    auto sum = [&](int c, bool ends) {
+      if constexpr (MODE != NORM) {
+        if (a.post) {
+          w.load(a.post, a.post_type, a.H, WIDE_THREADS, tid, whole, c, ends);
+          w.apply(v, post, a.offset, a.post_type);
+        }
+        in.sum(a, v);
+      }
+    };
+    if (MODE != NORM && a.post)
+      post = rms_of<false>([&](auto s) {
+        each([&](int, bool) { s += squares<decltype(s)>(v); });
+        return s;
+      }, a.H, a.eps, lds[0], lds64[0], WAVES);
+    Rms next = {1.f, 1.f};
+    if (a.next)
+      next = rms_of<false>([&](auto s) {
+        each([&](int c, bool ends) {
+          sum(c, ends);
+          s += squares<decltype(s)>(v);
+        });
+        return s;
+      }, a.H, a.eps, lds[1], lds64[1], WAVES);
+    each([&](int c, bool ends) {  // h may overwrite r: each place read and written by one thread
+      sum(c, ends);
+      if constexpr (MODE != NORM)
+        store_row<R, 1, N>(v, static_cast<typename R::raw*>(a.h) + row * a.ldh, a.H, WIDE_THREADS, tid, whole, c, ends);
+      if (a.next) {
+        w.load(a.next, a.next_type, a.H, WIDE_THREADS, tid, whole, c, ends);
+        w.apply(v, next, a.offset, a.next_type);
+        store_row<Y, 1, N>(v, static_cast<typename Y::raw*>(a.x) + row * a.ldx, a.H, WIDE_THREADS, tid, whole, c, ends);
+      }
+    });
     barrier_lds();
   }
 }
@@ -365,8 +389,8 @@ int launch_mode(const NormArgs& a, hipStream_t st) {
   if (waves(2) <= 16) return launch_rows<Y, R, 2, MODE, 16, false>(a, waves(2), st);
   if constexpr (VE<Y> == 4)
     if (waves(4) <= 16) return launch_rows<Y, R, 4, MODE, 16, false>(a, waves(4), st);
-  hipLaunchKernelGGL((norm_wide_kernel<Y, R>), dim3((unsigned)std::min<long>(a.rows, 1 << 20)), dim3(WIDE_THREADS), 0, st,
-                     a);
+  hipLaunchKernelGGL((norm_wide_kernel<Y, R, MODE>), dim3((unsigned)std::min<long>(a.rows, 1 << 20)), dim3(WIDE_THREADS),
+                     0, st, a);
   return (int)hipGetLastError();
 }
 
