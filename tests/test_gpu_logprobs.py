@@ -48,6 +48,7 @@ def check(logits, tokens=None, top=0, allowed=None):
                                        (300, 1000, 1, 8), (7, 50003, 4, 20), (1, 131072, 1, 20), (33, 131072, 1, 0),
                                        (1, 262147, 1, 32), (1200, 4099, 1, 20), (600, 20001, 0, 5), (2, 1000003, 1, 20),
                                        (100, 60000, 1, 32), (400, 33011, 1, 20), (1023, 17000, 1, 5), (511, 40000, 2, 0),
+                                       (3, 32768, 1, 20), (3, 32769, 1, 20), (3, 32776, 1, 20), (5, 16391, 1, 20),
                                        (48, 70001, 300, 8), (1100000, 9, 1, 3)])
 def test_token_logprobs(device, T, V, m, top, dtype):
     log(f"token_logprobs T={T} V={V} m={m} top={top} {dtype}")
