@@ -372,29 +372,47 @@ constexpr uint32_t MINUS_INF<ElemF16> = 0xfc00fc00u;
 template <>
 constexpr uint32_t MINUS_INF<ElemF32> = 0xff800000u;
 
-// A thread's next PIECES pieces of a row and of its mask, as loaded; pieces from `end` on hold
-// -inf.
+// A thread's next PIECES pieces of a row, as loaded; pieces from `end` on and places that the mask
+// takes out hold -inf.
 template <typename E, bool MASK, int PIECES>
 struct Pieces {
   static constexpr int N = PIECE<E>;
   RawVec<N, sizeof(typename E::raw)> v[PIECES];
-  uint32_t allow[PIECES][N / 4];
   QMOE_DEV void load(const typename E::raw* x, const uint8_t* ok, int piece, int end) {
+    uint32_t allow[PIECES][N / 4];
 #pragma unroll
     for (int j = 0; j < PIECES; ++j) {
       const long c = piece + j * THREADS;
 #pragma unroll
       for (int i = 0; i < v[j].WORDS; ++i) v[j].w[i] = MINUS_INF<E>;
-      if constexpr (MASK) {
 #pragma unroll
-        for (int i = 0; i < N / 4; ++i) allow[j][i] = 0;
-      }
+      for (int i = 0; i < N / 4; ++i) allow[j][i] = 0;
       if (c < end) {
         v[j].load(x + c * N);
         if constexpr (MASK) {
 #pragma unroll
           for (int i = 0; i < N / 4; ++i) __builtin_memcpy(&allow[j][i], ok + c * N + 4 * i, 4);
         }
+      }
+    }
+    if constexpr (MASK) {
+#pragma unroll
+      for (int j = 0; j < PIECES; ++j)
+#pragma unroll
+        for (int i = 0; i < N / 4; ++i) take_out(v[j].w + i * v[j].WORDS / (N / 4), allow[j][i]);
+    }
+  }
+  // -inf for those of 4 logits whose byte is 0, two 16-bit values at a time.
+  QMOE_DEV static void take_out(uint32_t* w, uint32_t allow) {
+    if constexpr (sizeof(typename E::raw) == 4) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] = (allow >> (8 * i)) & 0xffu ? w[i] : MINUS_INF<E>;
+    } else {
+      const uint32_t one = ((((allow & 0x7f7f7f7fu) + 0x7f7f7f7fu) | allow) >> 7) & 0x01010101u;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const uint32_t keep = __umul24(__builtin_amdgcn_perm(0u, one, i ? 0x0c030c02u : 0x0c010c00u), 0xffffu);
+        w[i] = (w[i] & keep) | (MINUS_INF<E> & ~keep);
       }
     }
   }
@@ -405,11 +423,7 @@ struct Pieces {
 #pragma unroll
       for (int i = 0; i < v[j].WORDS; ++i) asm volatile("" : "+v"(v[j].w[i]));
   }
-  QMOE_DEV float get(int j, int i) const {
-    const float l = v[j].template get<E>(i);
-    if constexpr (MASK) return ((allow[j][i / 4] >> (8 * (i & 3))) & 0xffu) ? l : -INFINITY;
-    return l;
-  }
+  QMOE_DEV float get(int j, int i) const { return v[j].template get<E>(i); }
 };
 
 // A workgroup takes one of `splits` parts of a row, in steps of PIECES pieces of 16 bytes per

@@ -81,6 +81,14 @@ def test_allowed(device, T, V, dtype):
         one = allowed[0].clone()
         check(torch.where(one, x, junk), tokens, 20, one)
         check(torch.where(one, x, junk), tokens, 4, one.expand(T, V))
+    # any byte but 0 allows, in a mask made of bytes
+    some = torch.randint(0, 3, (V,), generator=g, device=device) * 127
+    some = torch.where(some == 254, 255, some).to(torch.uint8)
+    check(x, tokens, 5, some.ne(0))
+    from qmoe import token_logprobs
+    for a, b in zip(token_logprobs(x, tokens, top=5, allowed=some.view(torch.bool)),
+                    token_logprobs(x, tokens, top=5, allowed=some.ne(0))):
+        assert torch.equal(a, b)
 
 
 @pytest.mark.gpu
