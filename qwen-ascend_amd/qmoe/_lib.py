@@ -138,6 +138,20 @@ def stream_of(t: torch.Tensor) -> int:
     return _RAW_STREAM(i)
 
 
+# The current device's index without the wrapper around it (0.25 us a call); not a public name.
+_CURRENT_DEVICE = getattr(torch._C, "_cuda_getDevice", None)
+
+
+def current_device() -> int:
+    return torch.cuda.current_device() if _CURRENT_DEVICE is None else _CURRENT_DEVICE()
+
+
+def contiguous_like(t: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
+    """An uninitialised contiguous tensor of t's shape (empty_like, where its result is
+    contiguous, takes 0.6 us less than the other calls)."""
+    return torch.empty_like(t, dtype=dtype) if t.is_contiguous() else t.new_empty(t.shape, dtype=dtype)
+
+
 def operands(t: torch.Tensor, *others) -> bool:
     """Checks the operands of a forward-only operator (None: not given): device
     tensors on one device, none of which asks for a gradient. False where that
@@ -154,7 +168,7 @@ def operands(t: torch.Tensor, *others) -> bool:
         raise RuntimeError("qmoe ops take device tensors")
     if graded and torch.is_grad_enabled():
         raise RuntimeError("this operator has no backward pass: call it under torch.no_grad()")
-    return i == torch.cuda.current_device()
+    return i == current_device()
 
 
 def ptr(t) -> int | None:

@@ -79,11 +79,11 @@ def token_logprobs(logits, tokens=None, *, top=0, allowed=None):
     logprobs = top_ids = top_lp = ws = None
     if tokens is not None:
         tokens = tokens.contiguous()
-        logprobs = x.new_empty(tokens.shape, dtype=torch.float32)
+        logprobs = torch.empty_like(tokens, dtype=torch.float32)
     entropy = x.new_empty(lead, dtype=torch.float32)
     if top:
         top_ids = x.new_empty((*lead, top), dtype=torch.int64)
-        top_lp = x.new_empty((*lead, top), dtype=torch.float32)
+        top_lp = torch.empty_like(top_ids, dtype=torch.float32)
     L = _lib.lib()
     kind, ptr = _TYPES[x.dtype], _lib.ptr
     nbytes = L.qmoe_token_logprobs_workspace(T, V, kind, top)

@@ -60,7 +60,7 @@ def block_norm(x, weight, *, eps=1e-6, offset=0.0, out_dtype=None):
     if not _lib.operands(x, weight):
         with torch.cuda.device(x.device):
             return block_norm(x, weight, eps=eps, offset=offset, out_dtype=out_dtype)
-    out = x.new_empty(x.shape, dtype=out_dtype)
+    out = _lib.contiguous_like(x, out_dtype)
     x = _rows(x, H)
     _lib.check(_lib.lib().qmoe_block_norm(x.data_ptr(), x.stride(0), _TYPES[xt], weight.data_ptr(),
                                           _TYPES[weight.dtype], out.data_ptr(), H, _TYPES[out_dtype], x.shape[0], H, eps,
@@ -158,10 +158,10 @@ def block_residual(y, residual, *, post_weight=None, gate=None, gate_act=None, s
         if not residual.is_inference():
             torch.autograd.graph.increment_version(residual)
     else:
-        hr = h = residual.new_empty(residual.shape)
+        hr = h = _lib.contiguous_like(residual, residual.dtype)
         res = _rows(residual, H)
         ldr, ldh = res.stride(0), H
-    x = None if next_weight is None else y.new_empty(y.shape)
+    x = None if next_weight is None else _lib.contiguous_like(y, y.dtype)
     y = _rows(y, H)
     ptr = _lib.ptr
     _lib.check(_lib.lib().qmoe_block_residual(

@@ -102,7 +102,7 @@ def test_operands(monkeypatch):
     """Gradients, host tensors and two devices are refused; another device than the current one is
     told apart."""
     from qmoe import _lib
-    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    monkeypatch.setattr(_lib, "current_device", lambda: 0)
     assert _lib.operands(Operand(), None, Operand()) is True
     assert _lib.operands(Operand(1), Operand(1)) is False
     for ops, says in (([Operand(-1)], "device tensors"), ([Operand(), Operand(-1)], "device tensors"),
