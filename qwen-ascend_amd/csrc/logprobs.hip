@@ -211,15 +211,16 @@ struct Stream {
   float top = -INFINITY, tau = -INFINITY, floor = -INFINITY;
   int count = 0;
 
-  // Adds the J pieces of P logits x.get(j, i). An infinite distance to the maximum would make D
-  // NaN (0 * inf): so long as none is met, nothing is done about it; from then on distances are
-  // taken no lower than FAR.
+  // Adds the J pieces of P logits x.get(j, i), their sums first, so that the terms of a long row
+  // are added in two levels. An infinite distance to the maximum would make D NaN (0 * inf): so
+  // long as none is met, nothing is done about it; from then on distances are taken no lower than
+  // FAR.
   template <int P, int J, typename X>
   QMOE_DEV void add(X& x, float most) {
     p = moved(p, fmaxf(p.m, most));
     const float z = base_of(p.m);
     if (!infinite) {
-      float s = p.s, d = p.d;
+      float s = 0.f, d = 0.f;
 #pragma unroll
       for (int j = 0; j < J; ++j) {
 #pragma unroll
@@ -232,21 +233,23 @@ struct Stream {
       }
       infinite = __any(d != d);
       if (!infinite) {
-        p.s = s, p.d = d;
+        p.s += s, p.d += d;
         return;
       }
     }
     x.pin();
+    float s = 0.f, d = 0.f;
 #pragma unroll
     for (int j = 0; j < J; ++j) {
 #pragma unroll
       for (int i = 0; i < P; ++i) {
         const float l = (x.get(j, i) - z) * LOG2E, e = __builtin_amdgcn_exp2f(l);
-        p.s += e;
-        p.d += e * fmaxf(l, FAR);
+        s += e;
+        d += e * fmaxf(l, FAR);
       }
       __builtin_amdgcn_sched_barrier(0);
     }
+    p.s += s, p.d += d;
   }
 
   // The same pieces' logits as candidates, piece j from id first + j * stride on. logit(id)

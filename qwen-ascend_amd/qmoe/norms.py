@@ -95,7 +95,8 @@ def _span(t):
 
 def _other_columns(rows, t):
     """Whether t's rows lie beside those of ``rows``, as columns of the same wider rows."""
-    if t.dim() != 2 or t.stride(0) != rows.stride(0) or t.dtype != rows.dtype or t.stride(1) not in (0, 1):
+    if (t.dim() != 2 or t.dtype != rows.dtype or t.stride(1) not in (0, 1) or t.stride(0) != rows.stride(0)
+            or rows.stride(0) < rows.shape[1]):
         return False
     column = (t.data_ptr() - rows.data_ptr()) // t.element_size() % rows.stride(0)
     return column >= rows.shape[1] and column + (t.shape[1] if t.stride(1) else 1) <= rows.stride(0)

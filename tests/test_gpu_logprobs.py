@@ -190,6 +190,30 @@ def test_same_bits_again(device):
 
 
 @pytest.mark.gpu
+def test_longest_row(device):
+    """2^30 logits in one row, the most that is taken: all equal but a few."""
+    import math
+    from qmoe import token_logprobs
+    V = 1 << 30
+    log("longest row")
+    x = torch.zeros(V, dtype=BF16, device=device)
+    at = [V - 1, 0, V // 2 + 3, 77777, V - 9]
+    for i, v in enumerate(at):
+        x[v] = 9.0 - i
+    z = V - len(at) + sum(math.exp(9.0 - i) for i in range(len(at)))
+    got = token_logprobs(x, torch.tensor([5, V - 1], device=device), top=7)
+    first = [v for v in range(2, 10) if v not in at][:2]
+    # a lane adds its 65536 equal terms in steps of 32: 32 + 2048 additions, then the tree
+    tol = (32 + 2048 + 64) * R.U + 2 * R.U * math.log(z)
+    assert got.top_ids.tolist() == at + [1, 2] == at + [1] + first[:1]
+    want = [9.0 - i - math.log(z) for i in range(len(at))] + [-math.log(z)] * 2
+    assert all(abs(a - b) <= tol for a, b in zip(got.top_logprobs.tolist(), want))
+    assert abs(got.logprobs[0].item() + math.log(z)) <= tol and abs(got.logprobs[1].item() - want[0]) <= tol
+    ent = math.log(z) - sum(math.exp(9.0 - i) * (9.0 - i) for i in range(len(at))) / z
+    assert abs(got.entropy.item() - ent) <= tol * (1 + math.log(z))
+
+
+@pytest.mark.gpu
 def test_far_offsets(device):
     """Elements beyond 2^32 of a tensor (rows of a 9 GiB buffer, the last ones looked at)."""
     from qmoe import block_norm, token_logprobs

@@ -84,6 +84,10 @@ def test_inplace_overlap():
         _inplace_rows(r, 8, ((wide[:, 9:10].expand(4, 8), False),))
     with pytest.raises(RuntimeError, match="overlaps"):             # wraps into the next row
         _inplace_rows(r, 8, ((wide.view(-1)[18:18 + 60].view(3, 20)[:, :6], False),))
+    one = base.as_strided((1, 8), (0, 1))  # a single row may have any step
+    _inplace_rows(one, 8, ((base.as_strided((1, 8), (0, 1), 8), False), (one, True)))
+    with pytest.raises(RuntimeError, match="overlaps"):
+        _inplace_rows(one, 8, ((base.as_strided((1, 8), (0, 1), 4), True),))
     with pytest.raises(RuntimeError, match="do not overlap"):
         _inplace_rows(t(1, 8).expand(4, 8), 8, ())
     with pytest.raises(RuntimeError, match="do not overlap"):
