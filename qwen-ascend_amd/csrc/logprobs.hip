@@ -563,17 +563,20 @@ __global__ __launch_bounds__(THREADS) void join_kernel(LogprobArgs a, int splits
 }
 
 // Pieces per part of a row: whole steps of 4 pieces per thread, or one step of 2 or 1 where that
-// leaves too few workgroups, so that there are about 1024 of them, four per CU. V = 131072 in
+// leaves too few workgroups, so that there are up to 1024 of them, four per CU. V = 131072 in
 // bf16, top 20, in 1, 2, 4, 8, 16, 32, 64 parts: 1 row 26.9, 20.9, 15.9, 12.5, 10.7, 9.9 and 9.4
 // us; 48 rows 31.2, 24.5, 18.3, 15.7, 14.4, 14.9 and 20.2; 256 rows 36.1, 31.4, 27.1, 30.2, 36.8,
-// 41.4 and 69.1; 1024 rows 62.6, 70.7, 77.5, 86.7, 110, 132 and 249. From 512 rows on (43.0, 40.1,
-// 44.4 us ...; without top alternatives 29.8, 32.6, 32.1) and for rows of up to four steps a row is
-// one part, which also saves the second launch (V = 32768, top 8, in parts and whole: 1 row 8.4
-// and 9.6 us, 64 rows 11.3 and 11.7, 256 rows 14.0 and 12.4; V = 8192: 8.2 and 5.6, 9.2 and 6.2,
-// 11.5 and 7.0; V = 65536: 8.4 and 14.0, 12.2 and 17.1, 18.3 and 20.2).
+// 41.4 and 69.1; 1024 rows 62.6, 70.7, 77.5, 86.7, 110, 132 and 249.
+// A row is one part, which also saves the second launch,
+// - from 512 rows on (43.0, 40.1, 44.4 us ...; without top alternatives 29.8, 32.6, 32.1);
+// - for rows of up to four steps (V = 32768, top 8, in parts and whole: 1 row 8.4 and 9.6 us, 64
+//   rows 11.3 and 11.7, 256 rows 14.0 and 12.4; V = 8192: 8.2 and 5.6, 9.2 and 6.2, 11.5 and 7.0);
+// - for rows of up to eight steps beyond 256 rows (V = 65536: 256 rows 18.1 and 20.1, 333 rows
+//   22.9 and 22.8, 400 rows 25.9 and 23.4; V = 50003: 18.5 and 18.8, 23.5 and 21.8, 25.4 and 22.2).
 int part_pieces(int T, int V, int type) {
   const int pieces = V / (type == QMOE_F32 ? 4 : 8), full = 4 * THREADS;
-  const int want = T >= 512 || pieces <= 4 * full ? 1 : std::min(host_ceil_div(1024, T), MAX_SPLITS);
+  const bool whole = T >= 512 || pieces <= 4 * full || (T > 256 && pieces <= 8 * full);
+  const int want = whole ? 1 : std::min(1024 / T, MAX_SPLITS);
   for (int per = THREADS; per < full; per *= 2)
     if (host_ceil_div(pieces, per) <= want) return per;
   return full * std::max(1, host_ceil_div(host_ceil_div(pieces, full), want));
