@@ -10,9 +10,9 @@
 // same pass: a wave keeps as candidates only the logits that reach a bound which k logits of the
 // row are known to reach, and the few that are left at the end are ranked by counting. Many rows
 // are bound by HBM, with about ten vector operations per logit close behind (4096 x 131072 bf16:
-// 191 us, 5.6 TB/s, top 20 222 us; 1024 x 65536 fp32, top 20: 52 us, 5.2 TB/s); few rows are split
-// over the chip and joined by a second launch, bound by the two launches' latency (1 x 131072, top
-// 20: 9.4 us, none 4.9).
+// 184 us, 5.8 TB/s, top 8 198 us; 1024 x 65536 fp32, top 20: 52 us, 5.2 TB/s). Fewer rows than CUs are
+// bound by a workgroup's own steps; the longest of them are split and joined by a second launch
+// (1 x 131072, top 20: 9.3 us, none 4.7).
 #include "elem_types.h"
 
 #include <algorithm>
@@ -20,7 +20,7 @@
 namespace {
 
 constexpr int TOP_MAX = 32;
-constexpr int THREADS = 256, WAVES = THREADS / 64;
+constexpr int JOIN_THREADS = 256;
 constexpr float LOG2E = 1.44269504088896341f, LN2 = 0.693147180559945309f;
 // e^(l - m) is zero in fp32 below this distance (base 2); l - m is not taken lower in D,
 // where an infinite distance would meet the zero.
@@ -66,20 +66,6 @@ QMOE_DEV Part moved(Part p, float m) {
 QMOE_DEV Part wave_join(Part p) {
   p = moved(p, wave_max_f32(p.m));
   return {p.m, wave_sum_f32(p.s), wave_sum_f32(p.d)};
-}
-
-// The parts of a workgroup's waves as one.
-QMOE_DEV Part join_waves(const Part* w) {
-  float m = w[0].m;
-#pragma unroll
-  for (int i = 1; i < WAVES; ++i) m = fmaxf(m, w[i].m);
-  Part r = {m, 0.f, 0.f};
-#pragma unroll
-  for (int i = 0; i < WAVES; ++i) {
-    const Part p = moved(w[i], m);
-    r.s += p.s, r.d += p.d;
-  }
-  return r;
 }
 
 // Distinct 64-bit selection keys: larger logit, then lower id (-0 counts as 0). 0: none.
@@ -133,11 +119,11 @@ QMOE_DEV uint32_t wave_kth(uint32_t v, int k) {
   return r;
 }
 
-// The k-th largest of one logit per lane.
+// The logit of the k-th largest of one order key per lane.
 template <typename E>
-QMOE_DEV float wave_kth_logit(float l, int k) {
+QMOE_DEV float wave_kth_logit(uint32_t order, int k) {
   constexpr int SH = KEY_SHIFT<E>;
-  uint32_t o = wave_kth<32 - SH>(order_of(l) >> SH, k) << SH;
+  uint32_t o = wave_kth<32 - SH>(order >> SH, k) << SH;
   if (!(o & 0x80000000u)) o |= (1u << SH) - 1u;  // a negative value's low zeros are ones in its key
   return order_logit(o);
 }
@@ -179,21 +165,16 @@ QMOE_DEV float compact(uint64_t* cand, int n, int k) {
   return key_logit(kth);
 }
 
-// Each lane's largest logit so far, for all waves of the workgroup.
+// The order key of the largest logit that the same lane of all waves has seen.
 struct Tops {
-  float v[WAVES][64];
-  QMOE_DEV void clear() { v[threadIdx.x >> 6][threadIdx.x & 63] = -INFINITY; }
-  // Stores this lane's value and returns the largest one of the same lane of all waves.
-  QMOE_DEV float raise(float mine) {
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    __hip_atomic_store(&v[wave][lane], mine, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
-    return most(mine);
+  uint32_t v[64];
+  QMOE_DEV void clear() {
+    if (threadIdx.x < 64) v[threadIdx.x] = 0;
   }
-  QMOE_DEV float most(float m) {
-#pragma unroll
-    for (int w = 0; w < WAVES; ++w)
-      m = fmaxf(m, __hip_atomic_load(&v[w][threadIdx.x & 63], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP));
-    return m;
+  // Brings this lane's largest logit in and returns the key of the largest of all.
+  QMOE_DEV uint32_t raise(float mine) {
+    const uint32_t o = order_of(mine);
+    return max(o, __hip_atomic_fetch_max(&v[threadIdx.x & 63], o, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP));
   }
 };
 
@@ -201,9 +182,9 @@ struct Tops {
 // per wave the candidates for the top k and two bounds that a logit has to pass to become one:
 // - tau: k logits of this wave, at lower ids than what follows, are >= tau: only above it;
 // - floor: k logits of the workgroup, at any ids, are >= floor: from it on.
-// floor is the k-th largest of the 64 maxima over the same lane of all waves, which the waves
-// read from each other whenever they see a logit above their bounds; a value that another wave
-// has raised since is only a weaker bound.
+// floor is the k-th largest of the 64 maxima over the same lane of all waves, which a wave looks
+// up whenever it sees a logit above its bounds; what other waves bring in later only makes the
+// bound weaker than it could be.
 template <typename E, bool MASK, bool TOP>
 struct Stream {
   bool infinite = MASK;
@@ -338,7 +319,7 @@ QMOE_DEV Given load_given(const LogprobArgs& a, int t, int j) {
   return g;
 }
 
-template <typename E>
+template <typename E, int THREADS>
 QMOE_DEV void emit_row(const LogprobArgs& a, int t, Given g, Part p, float log_s, bool undefined) {
   if (threadIdx.x == 0) a.entropy[t] = p.s == 0.f ? 0.f : log_s - LN2 * p.d / p.s;
   for (int j = threadIdx.x; j < a.m; j += THREADS) {
@@ -352,7 +333,7 @@ QMOE_DEV void emit_row(const LogprobArgs& a, int t, Given g, Part p, float log_s
 
 // Ranks n candidates (distinct keys) by counting the greater ones, the whole workgroup;
 // out(rank, key) for the first k ranks, key 0 where there are fewer.
-template <typename F>
+template <int THREADS, typename F>
 QMOE_DEV void rank_top(const uint64_t* list, int n, int k, F out) {
   for (int c = threadIdx.x; c < n; c += THREADS) {
     const uint64_t mine = list[c];
@@ -377,7 +358,7 @@ constexpr uint32_t MINUS_INF<ElemF32> = 0xff800000u;
 
 // A thread's next PIECES pieces of a row, as loaded; pieces from `end` on and places that the mask
 // takes out hold -inf.
-template <typename E, bool MASK, int PIECES>
+template <typename E, bool MASK, int PIECES, int THREADS>
 struct Pieces {
   static constexpr int N = PIECE<E>;
   RawVec<N, sizeof(typename E::raw)> v[PIECES];
@@ -429,13 +410,13 @@ struct Pieces {
   QMOE_DEV float get(int j, int i) const { return v[j].template get<E>(i); }
 };
 
-// A workgroup takes one of `splits` parts of a row, in steps of PIECES pieces of 16 bytes per
-// thread; with one part it writes the row's results, with several its sums and its best
+// A workgroup of WAVES waves takes one of `n_parts` parts of a row, in steps of PIECES pieces of 16
+// bytes per thread; with one part it writes the row's results, with several its sums and its best
 // candidates for join_kernel.
-template <typename E, bool MASK, bool TOP, int PIECES>
-__global__ __launch_bounds__(THREADS) void logprob_kernel(LogprobArgs a, int splits, int pieces_per_split, Part* parts,
-                                                          uint64_t* keys) {
-  constexpr int N = PIECE<E>;
+template <typename E, bool MASK, bool TOP, int PIECES, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void logprob_kernel(LogprobArgs a, int n_parts, int pieces_per_part, Part* parts,
+                                                             uint64_t* keys) {
+  constexpr int N = PIECE<E>, THREADS = 64 * WAVES;
   __shared__ uint64_t cand[TOP ? WAVES : 1][TOP ? CAP : 1], list[TOP ? WAVES * CAP : 1];
   __shared__ Part wave_part[WAVES];
   __shared__ Tops tops;
@@ -445,16 +426,16 @@ __global__ __launch_bounds__(THREADS) void logprob_kernel(LogprobArgs a, int spl
     tops.clear();
     __syncthreads();
   }
-  for (long unit = blockIdx.x; unit < (long)a.T * splits; unit += gridDim.x) {
-    const int t = (int)(unit / splits), part = (int)(unit % splits);
+  for (long unit = blockIdx.x; unit < (long)a.T * n_parts; unit += gridDim.x) {
+    const int t = (int)(unit / n_parts), part = (int)(unit % n_parts);
     const auto* x = static_cast<const typename E::raw*>(a.logits) + (long)t * a.ld;
     const uint8_t* ok = MASK ? a.allowed + (long)t * a.lda : nullptr;
-    const int pieces = a.V / N, begin = part * pieces_per_split, end = min(pieces, begin + pieces_per_split);
-    const Given given = splits == 1 ? load_given<E>(a, t, tid) : Given{-1, 0.f};
+    const int pieces = a.V / N, begin = part * pieces_per_part, end = min(pieces, begin + pieces_per_part);
+    const Given given = n_parts == 1 ? load_given<E>(a, t, tid) : Given{-1, 0.f};
     Stream<E, MASK, TOP> st;
     auto logit = [&](int v, int stop) { return v < stop && (!MASK || ok[v]) ? E::load(x[v]) : -INFINITY; };
     for (int q = begin; q < end; q += THREADS * PIECES) {
-      Pieces<E, MASK, PIECES> now;
+      Pieces<E, MASK, PIECES, THREADS> now;
       now.load(x, ok, q + tid, end);
       float most = -INFINITY, piece_most[PIECES];
 #pragma unroll
@@ -470,7 +451,7 @@ __global__ __launch_bounds__(THREADS) void logprob_kernel(LogprobArgs a, int spl
         st.template offer<N, PIECES>(now, piece_most, most, (q + tid) * N, THREADS * N, &tops, cand[wave], a.top,
                                      [&](int id) { return logit(id, end * N); });
     }
-    if (part == splits - 1 && pieces * N < a.V) {  // the row's end, less than a piece
+    if (part == n_parts - 1 && pieces * N < a.V) {  // the row's end, less than a piece
       const int v = pieces * N + tid;
       struct {
         float l;
@@ -487,11 +468,11 @@ __global__ __launch_bounds__(THREADS) void logprob_kernel(LogprobArgs a, int spl
     if ((tid & 63) == 0) wave_part[wave] = p;
     if (tid == 0) listed = 0;
     __syncthreads();
-    p = join_waves(wave_part);
+    p = wave_join((tid & 63) < WAVES ? wave_part[tid & 63] : Part{-INFINITY, 0.f, 0.f});
     const bool undefined = !(p.s >= 0.f);  // a NaN or +inf at an allowed place
     const float log_s = logf(p.s);
     if constexpr (TOP) {
-      const float floor = wave_kth_logit<E>(tops.most(st.top), a.top);
+      const float floor = wave_kth_logit<E>(tops.raise(st.top), a.top);
       int above = 0;
       for (int i = 0; i < st.count; i += 64) {
         const int at = i + (tid & 63);
@@ -507,38 +488,40 @@ __global__ __launch_bounds__(THREADS) void logprob_kernel(LogprobArgs a, int spl
       }
       __syncthreads();
       tops.clear();  // for the next row
-      if (splits == 1)
-        rank_top(list, listed, a.top, [&](int r, uint64_t k) { emit_top(a, t, r, k, p, log_s, undefined); });
+      if (n_parts == 1)
+        rank_top<THREADS>(list, listed, a.top, [&](int r, uint64_t k) { emit_top(a, t, r, k, p, log_s, undefined); });
       else
-        rank_top(list, listed, a.top, [&](int r, uint64_t k) { keys[unit * a.top + r] = k; });
+        rank_top<THREADS>(list, listed, a.top, [&](int r, uint64_t k) { keys[unit * a.top + r] = k; });
     }
-    if (splits == 1) emit_row<E>(a, t, given, p, log_s, undefined);
+    if (n_parts == 1) emit_row<E, THREADS>(a, t, given, p, log_s, undefined);
     else if (tid == 0) parts[unit] = p;
     __syncthreads();  // the next row reuses the LDS
   }
 }
 
-constexpr int MAX_SPLITS = 64;  // one part per lane of the joining wave
+constexpr int MAX_PARTS = 64;  // one part per lane of the joining wave
 
 // Joins the parts of a row: their sums and their ordered best candidates.
 template <typename E, bool TOP>
-__global__ __launch_bounds__(THREADS) void join_kernel(LogprobArgs a, int splits, const Part* parts, const uint64_t* keys) {
-  constexpr int EACH = MAX_SPLITS * TOP_MAX / THREADS;
-  __shared__ uint64_t list[TOP ? MAX_SPLITS * TOP_MAX : 1];
+__global__ __launch_bounds__(JOIN_THREADS) void join_kernel(LogprobArgs a, int n_parts, const Part* parts,
+                                                            const uint64_t* keys) {
+  constexpr int THREADS = JOIN_THREADS;
+  constexpr int EACH = MAX_PARTS * TOP_MAX / THREADS;
+  __shared__ uint64_t list[TOP ? MAX_PARTS * TOP_MAX : 1];
   __shared__ int listed;
   const int t = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
   const Given given = load_given<E>(a, t, tid);
   Part p = {-INFINITY, 0.f, 0.f};
-  if (lane < splits) p = parts[(long)t * splits + lane];
+  if (lane < n_parts) p = parts[(long)t * n_parts + lane];
   uint64_t key[TOP ? EACH : 1];
   if constexpr (TOP) {
-    const uint64_t* mine = keys + (long)t * splits * a.top;
+    const uint64_t* mine = keys + (long)t * n_parts * a.top;
     // The parts' keys are in order, so where `lists` parts have an r-th key of at least a floor
     // and r * lists >= k, k keys reach it.
-    const int r = (a.top + splits - 1) / splits, lists = (a.top + r - 1) / r;
-    const uint64_t rth = lane < splits ? mine[lane * a.top + r - 1] : 0;
+    const int r = (a.top + n_parts - 1) / n_parts, lists = (a.top + r - 1) / r;
+    const uint64_t rth = lane < n_parts ? mine[lane * a.top + r - 1] : 0;
 #pragma unroll
-    for (int i = 0; i < EACH; ++i) key[i] = i * THREADS + tid < splits * a.top ? mine[i * THREADS + tid] : 0;
+    for (int i = 0; i < EACH; ++i) key[i] = i * THREADS + tid < n_parts * a.top ? mine[i * THREADS + tid] : 0;
     if (tid == 0) listed = 0;
     constexpr int SH = KEY_SHIFT<E>;
     uint64_t floor = (uint64_t)(wave_kth<32 - SH>((uint32_t)(rth >> 32) >> SH, lists) << SH) << 32;
@@ -557,56 +540,78 @@ __global__ __launch_bounds__(THREADS) void join_kernel(LogprobArgs a, int splits
   const bool undefined = !(p.s >= 0.f);
   const float log_s = logf(p.s);
   if constexpr (TOP) {
-    rank_top(list, listed, a.top, [&](int r, uint64_t k) { emit_top(a, t, r, k, p, log_s, undefined); });
+    rank_top<JOIN_THREADS>(list, listed, a.top, [&](int r, uint64_t k) { emit_top(a, t, r, k, p, log_s, undefined); });
   }
-  emit_row<E>(a, t, given, p, log_s, undefined);
+  emit_row<E, JOIN_THREADS>(a, t, given, p, log_s, undefined);
 }
 
-// Pieces per part of a row: whole steps of 4 pieces per thread, or one step of 2 or 1 where that
-// leaves too few workgroups, so that there are up to 1024 of them, four per CU. V = 131072 in
-// bf16, top 20, in 1, 2, 4, 8, 16, 32, 64 parts: 1 row 26.9, 20.9, 15.9, 12.5, 10.7, 9.9 and 9.4
-// us; 48 rows 31.2, 24.5, 18.3, 15.7, 14.4, 14.9 and 20.2; 256 rows 36.1, 31.4, 27.1, 30.2, 36.8,
-// 41.4 and 69.1; 1024 rows 62.6, 70.7, 77.5, 86.7, 110, 132 and 249.
-// A row is one part, which also saves the second launch,
-// - from 512 rows on (43.0, 40.1, 44.4 us ...; without top alternatives 29.8, 32.6, 32.1);
-// - for rows of up to four steps (V = 32768, top 8, in parts and whole: 1 row 8.4 and 9.6 us, 64
-//   rows 11.3 and 11.7, 256 rows 14.0 and 12.4; V = 8192: 8.2 and 5.6, 9.2 and 6.2, 11.5 and 7.0);
-// - for rows of up to eight steps beyond 256 rows (V = 65536: 256 rows 18.1 and 20.1, 333 rows
-//   22.9 and 22.8, 400 rows 25.9 and 23.4; V = 50003: 18.5 and 18.8, 23.5 and 21.8, 25.4 and 22.2).
-int part_pieces(int T, int V, int type) {
-  const int pieces = V / (type == QMOE_F32 ? 4 : 8), full = 4 * THREADS;
-  const bool whole = T >= 512 || pieces <= 4 * full || (T > 256 && pieces <= 8 * full);
-  const int want = whole ? 1 : std::min(1024 / T, MAX_SPLITS);
-  for (int per = THREADS; per < full; per *= 2)
-    if (host_ceil_div(pieces, per) <= want) return per;
-  return full * std::max(1, host_ceil_div(host_ceil_div(pieces, full), want));
+// How a call's rows go over workgroups.
+struct Plan {
+  int parts;   // of a row; more than one are joined by a second launch
+  int pieces;  // of 16 bytes per part
+  int waves;   // per workgroup
+};
+
+// Whole rows wherever they fill the chip or are short, which also saves the second launch;
+// otherwise parts of whole steps of 4 pieces per thread (or one step of 2 or 1), up to 1024
+// workgroups of 4 waves. V in bf16, top 8, split and whole on 16 waves: 1 row of 65536 8.4 and 9.7
+// us, of 131072 8.5 and 14.3; 64 rows 12.0 and 10.8, 13.9 and 15.8; 128 rows 14.1 and 11.2, 18.4 and
+// 17.3; 192 rows of 131072 21.7 and 17.7. Parts of 131072, top 20: 1, 2, 4, 8, 16, 32, 64 of them
+// take 26.9, 20.9, 15.9, 12.5, 10.7, 9.9 and 9.4 us for 1 row, 31.2, 24.5, 18.3, 15.7, 14.4, 14.9 and
+// 20.2 for 48.
+// Waves for whole rows: 16 with up to a row per CU and enough in it, 8 with up to two rows per CU or
+// short rows, 4 for more rows, where the waves of several rows hide each other's latency. Top 8, 4, 8
+// and 16 waves: 64 x 32768 11.6, 8.9 and 8.1; 64 x 8192 6.2, 5.7 and 6.4; 333 x 32768 14.7, 12.3 and
+// 15.6; 333 x 8192 7.5, 7.6 and 11.6; 1024 x 32768 20.5, 23.1 and 30.4. Without top alternatives, whose
+// candidates each wave pays for, 8 waves win for many rows as well (2048 x 65536 55.7 and 52.6;
+// 4096 x 131072 194 and 184; but 1024 x 131072 52.8 and 54.8).
+Plan plan_for(int T, int V, int type, int top) {
+  const int pieces = V / (type == QMOE_F32 ? 4 : 8);
+  if (pieces <= 4096 || T >= 160 || pieces <= 128 * T) {
+    int waves = 4;
+    if (T <= 256) waves = pieces >= 4096 ? 16 : 8;
+    else if (T <= 512) waves = pieces >= 2048 ? 8 : 4;
+    else if (T > 1024 && !top) waves = pieces >= 4096 ? 8 : 4;
+    return {1, std::max(pieces, 1), waves};
+  }
+  constexpr int STEP = 256;
+  const int want = std::min(1024 / T, MAX_PARTS);
+  for (int per = STEP; per < 4 * STEP; per *= 2)
+    if (host_ceil_div(pieces, per) <= want) return {host_ceil_div(pieces, per), per, 4};
+  const int per = 4 * STEP * host_ceil_div(host_ceil_div(pieces, 4 * STEP), want);
+  return {host_ceil_div(pieces, per), per, 4};
 }
-int splits_for(int T, int V, int type) {
-  return std::max(1, host_ceil_div(V / (type == QMOE_F32 ? 4 : 8), part_pieces(T, V, type)));
+
+size_t parts_bytes(int T, const Plan& p) { return ((size_t)T * p.parts * sizeof(Part) + 15) / 16 * 16; }
+
+template <typename E, bool MASK, bool TOP, int STEP, int WAVES>
+void launch_rows(const LogprobArgs& a, const Plan& p, Part* parts, uint64_t* keys, hipStream_t st) {
+  const unsigned grid = (unsigned)std::min<long>((long)a.T * p.parts, 1l << 20);
+  hipLaunchKernelGGL((logprob_kernel<E, MASK, TOP, STEP, WAVES>), dim3(grid), dim3(64 * WAVES), 0, st, a, p.parts, p.pieces,
+                     parts, keys);
 }
 
 template <typename E, bool MASK, bool TOP>
-int launch(const LogprobArgs& a, int type, void* ws, hipStream_t st) {
-  const int splits = splits_for(a.T, a.V, type), per = part_pieces(a.T, a.V, type);
+int launch(const LogprobArgs& a, const Plan& p, void* ws, hipStream_t st) {
   Part* parts = static_cast<Part*>(ws);
-  uint64_t* keys = nullptr;
-  if (splits > 1) keys = reinterpret_cast<uint64_t*>(static_cast<char*>(ws) + ((size_t)a.T * splits * sizeof(Part) + 15) / 16 * 16);
-  const unsigned grid = (unsigned)std::min<long>((long)a.T * splits, 1l << 20);
-  if (per == THREADS)
-    hipLaunchKernelGGL((logprob_kernel<E, MASK, TOP, 1>), dim3(grid), dim3(THREADS), 0, st, a, splits, per, parts, keys);
-  else if (per == 2 * THREADS)
-    hipLaunchKernelGGL((logprob_kernel<E, MASK, TOP, 2>), dim3(grid), dim3(THREADS), 0, st, a, splits, per, parts, keys);
-  else
-    hipLaunchKernelGGL((logprob_kernel<E, MASK, TOP, 4>), dim3(grid), dim3(THREADS), 0, st, a, splits, per, parts, keys);
-  if (splits > 1)
-    hipLaunchKernelGGL((join_kernel<E, TOP>), dim3(a.T), dim3(THREADS), 0, st, a, splits, parts, keys);
+  uint64_t* keys = p.parts > 1 ? reinterpret_cast<uint64_t*>(static_cast<char*>(ws) + parts_bytes(a.T, p)) : nullptr;
+  const int each = host_ceil_div(p.pieces, 64 * p.waves);  // pieces per thread
+  if (p.waves == 16) launch_rows<E, MASK, TOP, 4, 16>(a, p, parts, keys, st);
+  else if (p.waves == 8 && each == 1) launch_rows<E, MASK, TOP, 1, 8>(a, p, parts, keys, st);
+  else if (p.waves == 8 && each == 2) launch_rows<E, MASK, TOP, 2, 8>(a, p, parts, keys, st);
+  else if (p.waves == 8) launch_rows<E, MASK, TOP, 4, 8>(a, p, parts, keys, st);
+  else if (each == 1) launch_rows<E, MASK, TOP, 1, 4>(a, p, parts, keys, st);
+  else if (each == 2) launch_rows<E, MASK, TOP, 2, 4>(a, p, parts, keys, st);
+  else launch_rows<E, MASK, TOP, 4, 4>(a, p, parts, keys, st);
+  if (p.parts > 1)
+    hipLaunchKernelGGL((join_kernel<E, TOP>), dim3(a.T), dim3(JOIN_THREADS), 0, st, a, p.parts, parts, keys);
   return (int)hipGetLastError();
 }
 
 template <typename E>
-int dispatch(const LogprobArgs& a, int type, void* ws, hipStream_t st) {
-  if (a.allowed) return a.top ? launch<E, true, true>(a, type, ws, st) : launch<E, true, false>(a, type, ws, st);
-  return a.top ? launch<E, false, true>(a, type, ws, st) : launch<E, false, false>(a, type, ws, st);
+int dispatch(const LogprobArgs& a, const Plan& p, void* ws, hipStream_t st) {
+  if (a.allowed) return a.top ? launch<E, true, true>(a, p, ws, st) : launch<E, true, false>(a, p, ws, st);
+  return a.top ? launch<E, false, true>(a, p, ws, st) : launch<E, false, false>(a, p, ws, st);
 }
 
 }  // namespace
@@ -615,8 +620,8 @@ extern "C" {
 
 size_t qmoe_token_logprobs_workspace(int T, int V, int type, int top) {
   if (T < 1 || V < 1 || top < 0 || top > TOP_MAX || !known_type(type)) return 0;
-  const size_t splits = splits_for(T, V, type);
-  return splits == 1 ? 0 : (T * splits * sizeof(Part) + 15) / 16 * 16 + T * splits * top * sizeof(uint64_t);
+  const Plan p = plan_for(T, V, type, top);
+  return p.parts == 1 ? 0 : parts_bytes(T, p) + (size_t)T * p.parts * top * sizeof(uint64_t);
 }
 
 int qmoe_token_logprobs(const void* logits, long ld, int type, const void* tokens, int m, const void* allowed,
@@ -634,9 +639,10 @@ int qmoe_token_logprobs(const void* logits, long ld, int type, const void* token
   a.allowed = (const uint8_t*)allowed, a.lda = ld_allowed, a.T = T, a.V = V;
   a.logprobs = (float*)logprobs, a.entropy = (float*)entropy;
   a.top = top, a.top_ids = (int64_t*)top_ids, a.top_logprobs = (float*)top_logprobs;
-  if (type == QMOE_BF16) return dispatch<ElemBF16>(a, type, workspace, (hipStream_t)stream);
-  if (type == QMOE_F16) return dispatch<ElemF16>(a, type, workspace, (hipStream_t)stream);
-  return dispatch<ElemF32>(a, type, workspace, (hipStream_t)stream);
+  const Plan p = plan_for(T, V, type, top);
+  if (type == QMOE_BF16) return dispatch<ElemBF16>(a, p, workspace, (hipStream_t)stream);
+  if (type == QMOE_F16) return dispatch<ElemF16>(a, p, workspace, (hipStream_t)stream);
+  return dispatch<ElemF32>(a, p, workspace, (hipStream_t)stream);
 }
 
 }  // extern "C"

@@ -49,7 +49,12 @@ def check(logits, tokens=None, top=0, allowed=None):
                                        (1, 262147, 1, 32), (1200, 4099, 1, 20), (600, 20001, 0, 5), (2, 1000003, 1, 20),
                                        (100, 60000, 1, 32), (400, 33011, 1, 20), (1023, 17000, 1, 5), (511, 40000, 2, 0),
                                        (3, 32768, 1, 20), (3, 32769, 1, 20), (3, 32776, 1, 20), (5, 16391, 1, 20),
-                                       (48, 70001, 300, 8), (1100000, 9, 1, 3)])
+                                       (48, 70001, 1100, 8), (1100000, 9, 1, 3),
+                                       # whole rows on 16, 8 and 4 waves, one and more steps, ends on and off them
+                                       (200, 131072, 1, 20), (161, 140001, 1, 32), (64, 65543, 3, 5), (256, 32768, 1, 20),
+                                       (257, 32768, 1, 20), (500, 16384, 1, 32), (500, 16383, 1, 5), (9, 4096, 1, 20),
+                                       (9, 4104, 1, 20), (9, 8193, 1, 32), (1100, 33000, 1, 0), (1100, 33000, 1, 2),
+                                       (513, 40000, 1, 20), (127, 131077, 1, 20), (70, 80000, 1, 7)])
 def test_token_logprobs(device, T, V, m, top, dtype):
     log(f"token_logprobs T={T} V={V} m={m} top={top} {dtype}")
     g = gen(device, T + V)
@@ -61,7 +66,7 @@ def test_token_logprobs(device, T, V, m, top, dtype):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [BF16, F16, F32])
-@pytest.mark.parametrize("T,V", [(1, 100), (9, 3001), (3, 131072), (700, 9000)])
+@pytest.mark.parametrize("T,V", [(1, 100), (9, 3001), (3, 131072), (700, 9000), (100, 40001), (300, 20000)])
 def test_allowed(device, T, V, dtype):
     """Masks by row and for all rows, whatever the masked places hold; rows with one token left and
     with none."""

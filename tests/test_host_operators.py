@@ -155,8 +155,9 @@ def test_c_entries_refuse_before_any_launch():
 
 @pytest.mark.parametrize("T,V,kind,parts", [
     (1, 131072, 0, 64), (1, 32768, 0, 1), (1, 32776, 0, 17), (1, 1 << 30, 0, 64), (16, 131072, 0, 64), (48, 131072, 0, 16),
-    (128, 131072, 1, 8), (256, 65536, 0, 4), (257, 65536, 0, 1), (257, 65544, 0, 3), (342, 131072, 0, 2), (511, 131072, 0, 2),
-    (512, 131072, 0, 1), (512, 1 << 30, 2, 1), (1, 16384, 2, 1), (1, 16388, 2, 17), (3, 7, 0, 1), (2, 1000003, 0, 62),
+    (64, 65536, 0, 1), (63, 65536, 0, 16), (64, 131072, 0, 16), (100, 131072, 1, 8), (127, 131072, 1, 8),
+    (128, 131072, 1, 1), (159, 262144, 0, 6), (160, 1 << 30, 2, 1), (512, 1 << 30, 2, 1), (1, 16384, 2, 1),
+    (1, 16388, 2, 17), (3, 7, 0, 1), (2, 1000003, 0, 62),
 ])
 def test_parts_of_rows(T, V, kind, parts):
     """How token_logprobs splits rows over workgroups, by its workspace: 12 bytes of sums and 8 bytes per
