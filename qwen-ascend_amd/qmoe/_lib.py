@@ -152,6 +152,12 @@ def contiguous_like(t: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
     return torch.empty_like(t, dtype=dtype) if t.is_contiguous() else t.new_empty(t.shape, dtype=dtype)
 
 
+def as_stored(t: torch.Tensor) -> torch.Tensor:
+    """t with its values in memory: a lazily negated view (the imaginary part of a conjugate),
+    whose memory holds the other sign, is copied."""
+    return t.resolve_neg() if t.is_neg() else t
+
+
 def operands(t: torch.Tensor, *others) -> bool:
     """Checks the operands of a forward-only operator (None: not given): device
     tensors on one device, none of which asks for a gradient. False where that

@@ -63,7 +63,8 @@ def token_logprobs(logits, tokens=None, *, top=0, allowed=None):
     if not _lib.operands(logits, tokens, allowed):
         with torch.cuda.device(logits.device):
             return token_logprobs(logits, tokens, top=top, allowed=allowed)
-    x = logits if logits.dim() == 2 else logits.reshape(-1, V)
+    x = _lib.as_stored(logits)
+    x = x if x.dim() == 2 else x.reshape(-1, V)
     if x.stride(1) != 1 and V != 1:
         x = x.contiguous()
     T = x.shape[0]

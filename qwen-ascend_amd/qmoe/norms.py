@@ -23,6 +23,7 @@ H_MAX = 32768
 
 def _rows(t, H):
     """t [..., H] as rows [n, H] whose elements are contiguous (a view where it can be one)."""
+    t = _lib.as_stored(t)
     if t.dim() != 2:
         t = t.reshape(-1, H)
     if t.stride(1) != 1 and H != 1:
@@ -33,6 +34,7 @@ def _rows(t, H):
 def _check_weight(w, H, what):
     if w.dtype not in _TYPES or w.shape != (H,):
         raise RuntimeError(f"{what} must be a [{H}] tensor in bfloat16, float16 or float32")
+    w = _lib.as_stored(w)
     return w if w.stride(0) == 1 or H == 1 else w.contiguous()
 
 
@@ -70,6 +72,7 @@ def block_norm(x, weight, *, eps=1e-6, offset=0.0, out_dtype=None):
 
 def _gate_steps(gate, shape, H):
     """The gate as (tensor, row step, column step) of the rows of ``shape``."""
+    gate = _lib.as_stored(gate)
     if len(shape) == 2 and gate.shape == (shape[0], 1):  # one per row, the common one: no view made
         return gate, gate.stride(0), 0
     try:
@@ -105,6 +108,8 @@ def _other_columns(rows, t):
 def _inplace_rows(residual, H, others):
     """Rows of a residual that is written in place: a view of it, apart from each other and from
     every other operand (y may be the residual itself)."""
+    if residual.is_neg():  # its memory holds the other sign
+        raise RuntimeError("inplace needs a residual that is not a lazily negated view (resolve_neg())")
     rows = residual if residual.dim() == 2 else residual.view(-1, H)
     if rows.shape[0] and ((rows.stride(1) != 1 and H != 1) or (rows.stride(0) < H and rows.shape[0] > 1)):
         raise RuntimeError("inplace needs a residual of rows with contiguous elements that do not overlap")

@@ -282,3 +282,34 @@ def test_norms_with_gradients(device):
     with torch.inference_mode():
         r = x.clone()
         assert block_residual(x, r, inplace=True) is r
+
+
+@pytest.mark.gpu
+def test_negated_views(device):
+    """Imaginary parts of conjugates, whose memory holds the other sign, as every operand that can be one."""
+    from qmoe import block_norm, block_residual, token_logprobs
+    n = gen(device, 51)
+
+    def view(*shape):
+        v = torch.imag(torch.complex(n(*shape, dtype=F32), n(*shape, dtype=F32)).conj())
+        assert v.is_neg()
+        return v
+    for T, H in ((5, 1), (1, 1), (4, 77)):
+        log(f"negated T={T} H={H}")
+        x, w, y, r, gate = view(T, H), view(H), view(T, H), view(T, H), view(T, 1)
+        R.assert_close(block_norm(x, w), *R.block_norm(x, w), "block_norm")
+        kw = dict(post_weight=w, gate=gate, scale=0.5, next_weight=w)
+        check_residual(block_residual(y, r, **kw), R.block_residual(y, r, **kw), "block_residual")
+        wide = gate.expand(T, H)
+        check_residual(block_residual(y, r, gate=wide), R.block_residual(y, r, gate=wide), "expanded gate")
+        with pytest.raises(RuntimeError, match="negated"):
+            block_residual(y, r, inplace=True)
+        keep = y.clone()
+        plain = r.clone().resolve_neg()
+        want = R.block_residual(y, plain, gate=gate)
+        check_residual(block_residual(y, plain, gate=gate, inplace=True), want, "in place")
+        assert torch.equal(y, keep)
+        got, want = token_logprobs(x, top=3), R.token_logprobs(x, top=3)
+        assert torch.equal(got.top_ids, want[2])
+        R.assert_close(got.entropy, *want[1], "entropy")
+        R.assert_close(got.top_logprobs, *want[3], "top_logprobs")

@@ -201,3 +201,29 @@ def test_planted_mistakes_are_seen():
         g[at] = v
         with pytest.raises(AssertionError):
             R.assert_close(g.to(BF16), e, b, "planted")
+
+
+def negated(*shape, dtype=torch.complex64):
+    """A view with the values -1, -2, ... and the memory 1, 2, ... (a step of 2 apart)."""
+    n = math.prod(shape)
+    z = torch.complex(*(torch.arange(1.0, n + 1).view(shape).to(F16 if dtype == torch.complex32 else F32),) * 2)
+    return torch.imag(z.conj())
+
+
+@pytest.mark.parametrize("dtype", [torch.complex64, torch.complex32])
+def test_negated_views(dtype):
+    """Operands whose memory holds the other sign are handed on with their values in memory."""
+    from qmoe import _lib
+    from qmoe.norms import _check_weight, _gate_steps, _inplace_rows, _rows
+    v = negated(4, 1, dtype=dtype)
+    assert v.is_neg()
+    want = [-1.0, -2.0, -3.0, -4.0]
+    for got in (_rows(v, 1), _rows(v.view(2, 2, 1), 1), _gate_steps(v, (4, 8), 8)[0],
+                _gate_steps(v, (4, 1), 1)[0], _gate_steps(v.view(2, 2, 1), (2, 2, 8), 8)[0][:, :1]):
+        assert not got.is_neg() and got.flatten().tolist() == want
+    for got in (_check_weight(v[:1, 0], 1, "weight"), _check_weight(v[:, 0], 4, "weight")):
+        assert not got.is_neg() and got.tolist() == want[:got.numel()]
+    plain = torch.ones(3, 4)
+    assert _lib.as_stored(plain) is plain and not _lib.as_stored(v).is_neg()
+    with pytest.raises(RuntimeError, match="negated"):
+        _inplace_rows(v, 1, ())
