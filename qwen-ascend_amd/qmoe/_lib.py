@@ -15,6 +15,7 @@ import threading
 from pathlib import Path
 
 import torch
+from torch.autograd import forward_ad
 
 _LIB = None
 _LOCK = threading.Lock()
@@ -152,6 +153,12 @@ def contiguous_like(t: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
     return torch.empty_like(t, dtype=dtype) if t.is_contiguous() else t.new_empty(t.shape, dtype=dtype)
 
 
+def _dual_level() -> int:
+    """The forward-mode level that is entered (-1: none); not a public name, so without it every
+    operand is looked at."""
+    return getattr(forward_ad, "_current_level", 0)
+
+
 def as_stored(t: torch.Tensor) -> torch.Tensor:
     """t with its values in memory: a lazily negated view (the imaginary part of a conjugate),
     whose memory holds the other sign, is copied."""
@@ -160,8 +167,9 @@ def as_stored(t: torch.Tensor) -> torch.Tensor:
 
 def operands(t: torch.Tensor, *others) -> bool:
     """Checks the operands of a forward-only operator (None: not given): device
-    tensors on one device, none of which asks for a gradient. False where that
-    device is not the current one, which a launch on its streams needs."""
+    tensors on one device, none of which asks for a gradient or carries a
+    forward-mode tangent. False where that device is not the current one, which a
+    launch on its streams needs."""
     i = t.get_device()
     graded = t.requires_grad
     for o in others:
@@ -174,6 +182,8 @@ def operands(t: torch.Tensor, *others) -> bool:
         raise RuntimeError("qmoe ops take device tensors")
     if graded and torch.is_grad_enabled():
         raise RuntimeError("this operator has no backward pass: call it under torch.no_grad()")
+    if _dual_level() >= 0 and any(o is not None and forward_ad.unpack_dual(o).tangent is not None for o in (t, *others)):
+        raise RuntimeError("this operator has no forward-mode derivative: call it on the primal tensors")
     return i == current_device()
 
 

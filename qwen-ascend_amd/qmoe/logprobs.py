@@ -4,7 +4,8 @@ What follows the lm_head projection (a :class:`qmoe.DenseW8`, ``fnx/load.py:189-
 the score of the tokens of a prompt, or of the ones sampled, beside the most likely ones.
 One pass over the logits with the running maximum and sums of the softmax, on the HIP kernels
 of libqmoe.so (``qmoe_token_logprobs``); nothing of the logits' size is written. Forward only:
-a tensor that requires a gradient is refused while gradients are recorded.
+a tensor that requires a gradient is refused while gradients are recorded, and one with a
+forward-mode tangent.
 """
 from __future__ import annotations
 

@@ -9,7 +9,7 @@ A pre-norm layer calls, around each of its blocks (:func:`qmoe.shared.moe_block`
 RMS norm in fp32, n(v; w) = v * (mean(v^2) + eps)^(-1/2) * (offset + w), each output rounded
 once. HIP kernels of libqmoe.so (``qmoe_block_norm``, ``qmoe_block_residual``), one launch
 per call on the current stream of the tensors' device. Forward only: a tensor that requires a
-gradient is refused while gradients are recorded.
+gradient is refused while gradients are recorded, and one with a forward-mode tangent.
 """
 from __future__ import annotations
 

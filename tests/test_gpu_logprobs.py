@@ -342,3 +342,21 @@ def test_logprobs_with_gradients(device):
         token_logprobs(x)
     with torch.no_grad():
         assert token_logprobs(x).entropy.shape == (2,)
+
+
+@pytest.mark.gpu
+def test_forward_mode(device):
+    """Operands with a forward-mode tangent are refused; their primal values are taken."""
+    from torch.autograd import forward_ad
+    from qmoe import block_norm, block_residual, token_logprobs
+    x, w = torch.ones((2, 8), device=device), torch.ones(8, device=device)
+    want = block_norm(x, w), block_residual(x, x, next_weight=w)[1], token_logprobs(x).entropy
+    with forward_ad.dual_level():
+        d, dw = forward_ad.make_dual(x, x), forward_ad.make_dual(w, w)
+        for call in (lambda: block_norm(d, w), lambda: block_norm(x, dw), lambda: block_residual(x, d),
+                     lambda: block_residual(x, x, gate=d), lambda: token_logprobs(d)):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call()
+        p = forward_ad.unpack_dual(d).primal
+        got = block_norm(p, w), block_residual(p, p, next_weight=w)[1], token_logprobs(p).entropy
+    assert all(torch.equal(a, b) for a, b in zip(got, want))

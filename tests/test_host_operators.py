@@ -227,3 +227,28 @@ def test_negated_views(dtype):
     assert _lib.as_stored(plain) is plain and not _lib.as_stored(v).is_neg()
     with pytest.raises(RuntimeError, match="negated"):
         _inplace_rows(v, 1, ())
+
+
+def test_forward_mode_tangents_are_refused(monkeypatch):
+    """A dual tensor does not require a gradient, and its tangent would be lost."""
+    from torch.autograd import forward_ad
+    from qmoe import _lib
+    monkeypatch.setattr(_lib, "current_device", lambda: 0)
+    monkeypatch.setattr(torch.Tensor, "get_device", lambda self: 0)
+    x = torch.ones(2, 8)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, x)
+        assert not dual.requires_grad
+        for ops in ((dual,), (x, None, dual)):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                _lib.operands(*ops)
+            with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
+                _lib.operands(*ops)
+        assert _lib.operands(x, None, forward_ad.unpack_dual(dual).primal) is True
+        with monkeypatch.context() as m:  # without the name that tells whether a level is entered
+            m.delattr(forward_ad, "_current_level")
+            m.setattr(forward_ad, "unpack_dual", lambda t, f=forward_ad.unpack_dual: f(t, level=0))
+            assert _lib.operands(x) is True
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                _lib.operands(dual)
+    assert _lib.operands(x, dual) is True
