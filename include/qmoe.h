@@ -405,7 +405,7 @@ int qmoe_block_residual(const void* y, long ldy, int ytype, const void* residual
  *      lm_head projection (fnx/load.py:189-201). logits [T, V <= 2^30] of `type`, rows ld elements
  *      apart at any alignment of the element; allowed: bytes [T, V], rows ld_allowed apart (0:
  *      one row for all), 0 takes the token out whatever its logit holds, or NULL;
- *      logprobs fp32 [T, m] = l - ln sum e^l of tokens int64 [T, m]; entropy fp32 [T]; the
+ *      logprobs fp32 [T, m] = l - ln sum e^l of tokens int64 [T, m <= 2^30]; entropy fp32 [T]; the
  *      `top` <= 32 largest logits (equal ones: lower id first) as top_ids int64 and
  *      top_logprobs fp32 [T, top]. m = 0 and top = 0 leave their tensors out.
  *      A token below 0 scores 0 (padding), one not allowed -inf, one from V on NaN. Fewer

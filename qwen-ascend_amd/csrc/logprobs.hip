@@ -20,6 +20,7 @@
 namespace {
 
 constexpr int TOP_MAX = 32;
+constexpr int V_MAX = 1 << 30, M_MAX = 1 << 30;  // with a workgroup's stride on top they stay within an int
 constexpr int JOIN_THREADS = 256;
 constexpr float LOG2E = 1.44269504088896341f, LN2 = 0.693147180559945309f;
 // e^(l - m) is zero in fp32 below this distance (base 2); l - m is not taken lower in D,
@@ -627,8 +628,8 @@ size_t qmoe_token_logprobs_workspace(int T, int V, int type, int top) {
 int qmoe_token_logprobs(const void* logits, long ld, int type, const void* tokens, int m, const void* allowed,
                         long ld_allowed, int T, int V, void* logprobs, void* entropy, int top, void* top_ids,
                         void* top_logprobs, void* workspace, size_t workspace_bytes, void* stream) {
-  if (T < 0 || V < 1 || V > (1 << 30) || m < 0 || top < 0 || top > TOP_MAX || ld < 0 || (allowed && ld_allowed < 0) ||
-      !known_type(type))
+  if (T < 0 || V < 1 || V > V_MAX || m < 0 || m > M_MAX || top < 0 || top > TOP_MAX || ld < 0 ||
+      (allowed && ld_allowed < 0) || !known_type(type))
     return QMOE_EINVAL;
   if (T == 0) return QMOE_OK;
   if (!logits || !entropy || (m && (!tokens || !logprobs)) || (top && (!top_ids || !top_logprobs))) return QMOE_EINVAL;

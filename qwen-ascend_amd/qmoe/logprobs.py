@@ -29,7 +29,7 @@ class TokenLogprobs(NamedTuple):
 def token_logprobs(logits, tokens=None, *, top=0, allowed=None):
     """Scores of the softmax over rows of logits [..., V] (bfloat16, float16 or float32).
 
-    tokens int64 [...] or [..., m] (m given tokens for each row): their log
+    tokens int64 [...] or [..., m] (m <= 2^30 given tokens for each row): their log
     probabilities; a negative token scores 0 (padding), one that is not allowed -inf, one
     from V on NaN. The entropy of each row. The ``top`` <= 32 most likely tokens in order
     (equal logits: the lower id first) with their log probabilities; where fewer than ``top``
@@ -59,6 +59,8 @@ def token_logprobs(logits, tokens=None, *, top=0, allowed=None):
             m = tokens.shape[-1]
         else:
             raise RuntimeError(f"tokens {tuple(tokens.shape)} do not match logits {tuple(logits.shape)}")
+        if m > 1 << 30:
+            raise RuntimeError("tokens must be at most 2^30 for each row")
     if allowed is not None and (allowed.dtype != torch.bool or allowed.shape not in ((V,), logits.shape)):
         raise RuntimeError("allowed must be bool [V] or of the logits' shape")
     if not _lib.operands(logits, tokens, allowed):

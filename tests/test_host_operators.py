@@ -252,3 +252,21 @@ def test_forward_mode_tangents_are_refused(monkeypatch):
             with pytest.raises(RuntimeError, match="forward-mode"):
                 _lib.operands(dual)
     assert _lib.operands(x, dual) is True
+
+
+def test_many_tokens_per_row():
+    """More than 2^30 tokens for a row are refused: the kernels count them in 32 bits, a workgroup's
+    stride on top (checked before anything is read; the pointers are not real)."""
+    import qmoe
+    from qmoe import _lib
+    L = _lib.lib()
+    for m in ((1 << 30) + 1, (1 << 31) - 256, (1 << 31) - 1):
+        for T in (0, 1):
+            assert L.qmoe_token_logprobs(16, 8, 0, 16, m, None, 0, T, 8, 16, 16, 0, None, None, None, 0, None) == -1, m
+    assert L.qmoe_token_logprobs(16, 8, 0, 16, 1 << 30, None, 0, 0, 8, 16, 16, 0, None, None, None, 0, None) == 0
+    one = torch.zeros((), dtype=torch.int64)
+    for m in ((1 << 30) + 1, 1 << 31, (1 << 32) + 5):
+        with pytest.raises(RuntimeError, match="2.30 for each row"):
+            qmoe.token_logprobs(t(2, 8), one.expand(2, m))
+    with pytest.raises(RuntimeError, match="device tensors"):
+        qmoe.token_logprobs(t(2, 8), one.expand(2, 1 << 30))
