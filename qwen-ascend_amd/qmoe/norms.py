@@ -8,8 +8,10 @@ A pre-norm layer calls, around each of its blocks (:func:`qmoe.shared.moe_block`
 
 RMS norm in fp32, n(v; w) = v * (mean(v^2) + eps)^(-1/2) * (offset + w), each output rounded
 once. HIP kernels of libqmoe.so (``qmoe_block_norm``, ``qmoe_block_residual``), one launch
-per call on the current stream of the tensors' device. Forward only: a tensor that requires a
-gradient is refused while gradients are recorded, and one with a forward-mode tangent.
+per call on the current stream of the tensors' device; operands that are no rows of contiguous
+elements (strided columns, dimensions that do not merge into rows, lazily negated views) are
+copied first. Forward only: a tensor that requires a gradient is refused while gradients are
+recorded, and one with a forward-mode tangent.
 """
 from __future__ import annotations
 
@@ -79,10 +81,11 @@ def _gate_steps(gate, shape, H):
         g = gate.expand(shape)
     except RuntimeError:
         raise RuntimeError(f"gate {tuple(gate.shape)} does not broadcast to {tuple(shape)}") from None
+    if H == 1 or g.stride(-1) == 0:  # one per row: of a batch of sequences, a copy of a value per row at most
+        g = g[..., :1].reshape(-1, 1)
+        return g, g.stride(0), 0
     if g.dim() != 2:
         g = g.reshape(-1, H)
-    if H == 1 or g.stride(1) == 0:
-        return g, g.stride(0), 0
     if g.stride(1) != 1:
         g = g.contiguous()
     return g, g.stride(0), 1
@@ -131,8 +134,9 @@ def block_residual(y, residual, *, post_weight=None, gate=None, gate_act=None, s
     (or y without one), and with ``next_weight`` the next block's input x = n(h; next_weight).
 
     y [..., H]; residual of y's shape and type, or float32 beside a 16-bit y. gate: any
-    tensor that broadcasts to y (one value per row, per channel or per element), a: its value,
-    or its sigmoid for ``gate_act="sigmoid"``. The weights take ``offset`` as in
+    tensor that broadcasts to y (one value per row, per channel or per element; one per
+    sequence and channel, [B, 1, H], is written out for every row first), a: its value, or its
+    sigmoid for ``gate_act="sigmoid"``. The weights take ``offset`` as in
     :func:`block_norm`. Returns h (contiguous, the residual's type), or (h, x) with x in y's
     type; x is normed from h before h is rounded. ``inplace=True`` writes h over
     ``residual`` and returns that tensor."""

@@ -313,3 +313,19 @@ def test_negated_views(device):
         assert torch.equal(got.top_ids, want[2])
         R.assert_close(got.entropy, *want[1], "entropy")
         R.assert_close(got.top_logprobs, *want[3], "top_logprobs")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B,S,H", [(3, 5, 333), (1, 4, 64), (4, 1, 64), (2, 3, 1), (70, 11, 2560)])
+def test_gates_per_sequence(device, B, S, H):
+    """Gates of a batch of sequences: one value for each of them, each and channel, each position of
+    all, each channel, one in all."""
+    from qmoe import block_residual
+    n = gen(device, B * S + H)
+    y, r, w = n(B, S, H), n(B, S, H, dtype=F32), n(H)
+    for shape in ((B, 1, 1), (B, 1, H), (1, S, 1), (S, 1), (1, S, H), (1, 1, H), (H,), (1,), ()):
+        log(f"gate {shape} of {(B, S, H)}")
+        gate = n(*shape)
+        for act in (None, "sigmoid"):
+            want = R.block_residual(y, r, gate=gate, gate_act=act, next_weight=w)
+            check_residual(block_residual(y, r, gate=gate, gate_act=act, next_weight=w), want, f"gate {shape}")

@@ -270,3 +270,16 @@ def test_many_tokens_per_row():
             qmoe.token_logprobs(t(2, 8), one.expand(2, m))
     with pytest.raises(RuntimeError, match="device tensors"):
         qmoe.token_logprobs(t(2, 8), one.expand(2, 1 << 30))
+
+
+def test_gates_of_a_batch():
+    """One value per sequence stays one value per row; only as many values as rows are ever copied."""
+    from qmoe.norms import _gate_steps
+    for shape, of, want in (((2, 1, 1), (2, 5, 8), [0] * 5 + [1] * 5), ((1, 5, 1), (2, 5, 8), [0, 1, 2, 3, 4] * 2),
+                            ((5, 1), (2, 5, 8), [0, 1, 2, 3, 4] * 2), ((), (2, 5, 8), [0] * 10), ((1,), (8,), [0]),
+                            ((2, 1, 2, 1), (2, 3, 2, 8), [0, 1] * 3 + [2, 3] * 3), ((2, 5, 1), (2, 5, 1), list(range(10))),
+                            ((2, 1, 1), (2, 0, 8), [])):
+        gate = torch.arange(float(math.prod(shape))).view(shape)
+        g, row, column = _gate_steps(gate, of, of[-1])
+        assert column == 0 and g.untyped_storage().nbytes() <= 4 * max(gate.numel(), len(want)), shape
+        assert g.as_strided((len(want),), (row,)).tolist() == want, shape
