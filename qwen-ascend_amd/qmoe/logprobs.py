@@ -38,8 +38,11 @@ def token_logprobs(logits, tokens=None, *, top=0, allowed=None):
     allowed: bool [V] or of the logits' shape; where it is False a token is out, whatever its
     logit holds. A row with no token left: its tokens -inf, entropy 0. A row with NaN or +inf
     at an allowed place has no distribution: NaN (padding still 0) and ids -1. The sums are fp32,
-    in two levels: rounding moves a row's sum by at most V / 4096 + 64 half steps (2^-24 of it),
-    and by far less as a rule; log probabilities and entropies move by as much, absolute.
+    in two levels. With B = V / 1024 + 128 half steps (2^-24 each), to first order: a row's sum is
+    off by at most B of it, a log probability by at most B and four half steps of its own size, an
+    entropy E by at most (1 + 5 E) B; by far less as a rule. (V / 1024 is the cost of a maximum that
+    rises all along the row, at most four roundings a step of at least 4096 logits; where it comes
+    early it is V / 4096.)
     """
     if logits.dtype not in _TYPES:
         raise RuntimeError("logits must be bfloat16, float16 or float32")
