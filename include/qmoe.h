@@ -411,7 +411,9 @@ int qmoe_block_residual(const void* y, long ldy, int ytype, const void* residual
  *      A token below 0 scores 0 (padding), one not allowed -inf, one from V on NaN. Fewer
  *      than `top` tokens above -inf: id -1 and -inf fill up. A row with none at all: its tokens
  *      -inf, entropy 0. A row with NaN or +inf at an allowed place: NaN, ids -1.
- *      Workspace: qmoe_token_logprobs_workspace(T, V, type, top) bytes, 16-byte aligned. */
+ *      Workspace: qmoe_token_logprobs_workspace(T, V, type, top) bytes, 16-byte aligned. Asked for
+ *      each call's own sizes: the need does not grow with T or V (127 rows of 131072 are split, 128
+ *      are not). */
 size_t qmoe_token_logprobs_workspace(int T, int V, int type, int top);
 int qmoe_token_logprobs(const void* logits, long ld, int type, const void* tokens, int m, const void* allowed,
                         long ld_allowed, int T, int V, void* logprobs, void* entropy, int top, void* top_ids,

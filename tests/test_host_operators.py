@@ -283,3 +283,25 @@ def test_gates_of_a_batch():
         g, row, column = _gate_steps(gate, of, of[-1])
         assert column == 0 and g.untyped_storage().nbytes() <= 4 * max(gate.numel(), len(want)), shape
         assert g.as_strided((len(want),), (row,)).tolist() == want, shape
+
+
+def test_workspace_is_checked_before_any_launch():
+    """Split rows need their workspace: none, one that is too short or off its alignment is refused (no
+    pointer here is real). The need does not grow with the rows: a size is good for its own call only."""
+    from qmoe import _lib
+    L = _lib.lib()
+    size = L.qmoe_token_logprobs_workspace
+    EWORKSPACE = -2
+
+    def call(T, V, top, ws, nbytes, kind=0):
+        return L.qmoe_token_logprobs(16, V, kind, 16, 1, None, 0, T, V, 16, 16, top, 16, 16, ws, nbytes, None)
+    for T, V, top, kind in ((1, 131072, 20, 0), (1, 131072, 0, 0), (48, 131072, 8, 1), (127, 131072, 32, 0), (159, 262144, 5, 0),
+                            (1, 16388, 1, 2), (3, 1 << 30, 20, 0)):
+        need = size(T, V, kind, top)
+        assert need > 0 and need % 8 == 0
+        for ws, nbytes in ((None, need), (None, 0), (4096, need - 1), (4096, 0), (4096 + 8, need), (4096 + 1, need + 64)):
+            assert call(T, V, top, ws, nbytes, kind) == EWORKSPACE, (T, V, top, ws, nbytes)
+    assert size(127, 131072, 0, 20) > size(128, 131072, 0, 20) == 0
+    assert size(16, 131072, 0, 20) > size(17, 131072, 0, 20) and size(1, 131072, 0, 20) > size(1, 131080, 0, 20)
+    assert call(127, 131072, 20, 4096, size(128, 131072, 0, 20)) == EWORKSPACE
+    assert call(127, 131072, 20, 4096, size(127, 131072, 0, 8)) == EWORKSPACE
