@@ -385,7 +385,7 @@ int qmoe_w8a16_gemm_mfma(const void* x, const void* w, const void* scale, void* 
 #define QMOE_BF16 0
 #define QMOE_F16 1
 #define QMOE_F32 2
-/* Before a block: y = n(x; weight). ytype is xtype, or 16-bit for x in fp32. */
+/* Before a block: y = n(x; weight). ytype is xtype, or 16-bit for x in fp32. y does not overlap x. */
 int qmoe_block_norm(const void* x, long ldx, int xtype, const void* weight, int wtype, void* y, long ldy, int ytype,
                     long rows, int H, float eps, float offset, void* stream);
 /* After a block: p = n(y; post_weight) (y itself for NULL), h = residual + scale * a(gate) * p,

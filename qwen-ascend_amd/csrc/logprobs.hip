@@ -10,9 +10,12 @@
 // same pass: a wave keeps as candidates only the logits that reach a bound which k logits of the
 // row are known to reach, and the few that are left at the end are ranked by counting. Many rows
 // are bound by HBM, with about ten vector operations per logit close behind (4096 x 131072 bf16:
-// 184 us, 5.8 TB/s, top 8 198 us; 1024 x 65536 fp32, top 20: 52 us, 5.2 TB/s). Fewer rows than CUs are
+// 182 us, 5.9 TB/s, top 8 189 us; 1024 x 65536 fp32, top 20: 52 us, 5.2 TB/s). Fewer rows than CUs are
 // bound by a workgroup's own steps; the longest of them are split and joined by a second launch
-// (1 x 131072, top 20: 9.3 us, none 4.7).
+// (1 x 131072, top 20: 9.2 us, none 4.5; 48 rows, top 8: 12.8, none 8.4, under a mask 15.3 and 10.6).
+// An unfinished last step costs as much as a whole one (333 x 50003, top 5: 19.9 us, 1.2 ps per
+// logit, 131072 of them 28.2 us, 0.65 ps; 4096 rows, none: 98 us, 0.48 ps, and 181 us, 0.34 ps). Times
+// are those of graphs over several states.
 #include "elem_types.h"
 
 #include <algorithm>
@@ -196,7 +199,8 @@ struct Stream {
   // Adds the J pieces of P logits x.get(j, i), their sums first, so that the terms of a long row
   // are added in two levels. An infinite distance to the maximum would make D NaN (0 * inf): so
   // long as none is met, nothing is done about it; from then on distances are taken no lower than
-  // FAR.
+  // FAR. A row's places past its end are such distances: waves that hold some in its last step do
+  // that step twice.
   template <int P, int J, typename X>
   QMOE_DEV void add(X& x, float most) {
     p = moved(p, fmaxf(p.m, most));

@@ -33,7 +33,8 @@ struct NormArgs {
 // workgroup with more than one row loads the next one while it works on this one.
 // 4096 x 2560 bf16: 10.9 us for the norm (42 MB), 20.8 for the whole step after a block (84
 // MB); copies of the same bytes take 10.0 and 17.7. 8192 x 4096 with a 32-bit stream: 77.9 us,
-// 5.2 TB/s.
+// 5.2 TB/s. All in fp32: norm 4096 x 2560 15.9 us, 5.3 TB/s, 2048 x 16384 53 us, 5.0 TB/s; the whole
+// step, gate per row 40.8 and 114 us, 4.1 and 4.7 TB/s, gate per element 55.2 and 188 us.
 template <typename Y>
 constexpr int VE = 16 / sizeof(typename Y::raw);
 
@@ -356,9 +357,15 @@ __global__ __launch_bounds__(WIDE_THREADS) void norm_wide_kernel(NormArgs a) {
 
 template <typename Y, typename R, int NV, int MODE, int MAX_WAVES, bool AHEAD>
 int launch_rows(const NormArgs& a, int waves, hipStream_t st) {
-  // With rows ahead: as many workgroups as stay resident with 16 waves per CU, the rows in
-  // even rounds over them (4096 x 2560 norm: 10.9 us; 12 waves 13.0, 20 waves 11.0). The
-  // others take a row each and leave the order to the dispatcher.
+  // With rows ahead: as many workgroups as 16 waves per CU make, the rows in even rounds over
+  // them. That is what stays resident up to 128 registers. Above, fewer do, and part of the
+  // grid waits: 12 waves with a gate per row beside fp32 (153 to 156) and per element in bf16
+  // (164), 8 per element in fp16 (170) and beside fp32 (186 to 189). Grids of 8, 12, 16 and 20
+  // waves, us: 4096 x 2560 norm 13.0, 10.0, 10.0, 10.1; bf16 sum, gate per row 24.7, 18.8, 18.8,
+  // 20.3; per channel beside fp32 33.4, 34.7, 34.6, 37.8; 8192 x 4096, gate per element fp16
+  // 65.9, 73.3, 65.4, 71.9, beside fp32 88.9, 103, 89.0, 96.7. Against 16 stand rows of three and
+  // eight waves beside fp32: 8192 x 1536 per channel 34.6, 45.5, 42.6, 42.6, 3000 x 8192 62.9,
+  // 62.8, 65.4, 65.2. The other forms take a row each and leave the order to the dispatcher.
   const int rows_per = MAX_WAVES == 1 ? 4 : 1, wg_waves = MAX_WAVES == 1 ? 4 : waves;
   const long groups = (a.rows + rows_per - 1) / rows_per, most = AHEAD ? 256l * (16 / wg_waves) : 1l << 20;
   const long rounds = (groups + most - 1) / most;
@@ -373,6 +380,20 @@ int launch_rows(const NormArgs& a, int waves, hipStream_t st) {
 // 8192 x 1536: 22.8 and 24.0), and the next row on its way, where the registers hold it: not for
 // 16 waves with 32-bit sums or a gate per element (2048 x 16384 sum in bf16: 59.9 us, without
 // the row ahead 68.1; in fp16, with nine words spilled, 66.0 and 70.4).
+// Where few rows end depends on the form; 512 is one limit for all. One piece and two with the
+// row ahead, us:
+//   norm bf16                400 x 4096   4.1 /  4.0     1003 x 2048  4.1 /  4.1    1003 x 4096   5.9 /  5.6
+//   sum, gate per row, bf16  400 x 2048   4.9 /  5.2      513 x 2048  5.3 /  5.6    2048 x 4096  15.1 / 13.5
+//   gate per element, fp16   400 x 2048   5.2 /  6.4      777 x 2048  7.4 /  7.6    1003 x 2048   7.9 /  8.1
+//                           2048 x 2048  11.7 / 13.9     4096 x 2048 17.4 / 23.2    2048 x 8192  45.6 / 40.9
+//   per channel beside fp32  400 x 2048   5.5 /  6.5     2048 x 2048 14.3 / 17.9    2048 x 8192  55.0 / 46.3
+// So two pieces win from the limit on for long rows and for all norms and gates per row, but not for
+// rows of about 2048 under a gate per element or channel, which lose up to a quarter there; with up to
+// two rows per workgroup the row ahead is hardly ever loaded. Below the limit rows of 8192 under a gate per
+// row lose as much (400: 10.9 / 8.4).
+// Forms that spill: a gate per element on 16 waves in fp32 with four pieces, 24 words (2048 x 16384:
+// 188 us, 3.6 TB/s; a gate per row, without spills, 114 us, 4.7), fp16 beside fp32 4 words and bf16
+// beside fp32 1 (117 and 112 us, 4.0 and 4.2 TB/s; a gate per row 96 us, 4.2).
 template <typename Y, typename R, int MODE>
 int launch_mode(const NormArgs& a, hipStream_t st) {
   const int pieces = host_ceil_div(a.H, VE<Y>);
