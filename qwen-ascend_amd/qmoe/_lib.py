@@ -153,16 +153,9 @@ def contiguous_like(t: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
     return torch.empty_like(t, dtype=dtype) if t.is_contiguous() else t.new_empty(t.shape, dtype=dtype)
 
 
-def _dual_level() -> int:
-    """The forward-mode level that is entered (-1: none); not a public name, so without it every
-    operand is looked at."""
-    return getattr(forward_ad, "_current_level", 0)
-
-
-def as_stored(t: torch.Tensor) -> torch.Tensor:
-    """t with its values in memory: a lazily negated view (the imaginary part of a conjugate),
-    whose memory holds the other sign, is copied."""
-    return t.resolve_neg() if t.is_neg() else t
+# _current_level: the forward-mode level that is entered (-1: none); not a public name, so without it
+# every operand is looked at.
+_FORWARD_AD = vars(forward_ad)
 
 
 def operands(t: torch.Tensor, *others) -> bool:
@@ -182,7 +175,8 @@ def operands(t: torch.Tensor, *others) -> bool:
         raise RuntimeError("qmoe ops take device tensors")
     if graded and torch.is_grad_enabled():
         raise RuntimeError("this operator has no backward pass: call it under torch.no_grad()")
-    if _dual_level() >= 0 and any(o is not None and forward_ad.unpack_dual(o).tangent is not None for o in (t, *others)):
+    if _FORWARD_AD.get("_current_level", 0) >= 0 and any(
+            o is not None and forward_ad.unpack_dual(o).tangent is not None for o in (t, *others)):
         raise RuntimeError("this operator has no forward-mode derivative: call it on the primal tensors")
     return i == current_device()
 

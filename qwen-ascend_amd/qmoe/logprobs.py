@@ -69,8 +69,9 @@ def token_logprobs(logits, tokens=None, *, top=0, allowed=None):
     if not _lib.operands(logits, tokens, allowed):
         with torch.cuda.device(logits.device):
             return token_logprobs(logits, tokens, top=top, allowed=allowed)
-    x = _lib.as_stored(logits)
-    x = x if x.dim() == 2 else x.reshape(-1, V)
+    x = logits if logits.dim() == 2 else logits.reshape(-1, V)
+    if x.is_neg():  # the imaginary part of a conjugate: its memory holds the other sign
+        x = x.resolve_neg()
     if x.stride(1) != 1 and V != 1:
         x = x.contiguous()
     T = x.shape[0]

@@ -25,7 +25,8 @@ H_MAX = 32768
 
 def _rows(t, H):
     """t [..., H] as rows [n, H] whose elements are contiguous (a view where it can be one)."""
-    t = _lib.as_stored(t)
+    if t.is_neg():  # the imaginary part of a conjugate: its memory holds the other sign
+        t = t.resolve_neg()
     if t.dim() != 2:
         t = t.reshape(-1, H)
     if t.stride(1) != 1 and H != 1:
@@ -36,7 +37,8 @@ def _rows(t, H):
 def _check_weight(w, H, what):
     if w.dtype not in _TYPES or w.shape != (H,):
         raise RuntimeError(f"{what} must be a [{H}] tensor in bfloat16, float16 or float32")
-    w = _lib.as_stored(w)
+    if w.is_neg():
+        w = w.resolve_neg()
     return w if w.stride(0) == 1 or H == 1 else w.contiguous()
 
 
@@ -74,7 +76,8 @@ def block_norm(x, weight, *, eps=1e-6, offset=0.0, out_dtype=None):
 
 def _gate_steps(gate, shape, H):
     """The gate as (tensor, row step, column step) of the rows of ``shape``."""
-    gate = _lib.as_stored(gate)
+    if gate.is_neg():
+        gate = gate.resolve_neg()
     if len(shape) == 2 and gate.shape == (shape[0], 1):  # one per row, the common one: no view made
         return gate, gate.stride(0), 0
     try:
