@@ -359,12 +359,13 @@ template <typename Y, typename R, int NV, int MODE, int MAX_WAVES, bool AHEAD>
 int launch_rows(const NormArgs& a, int waves, hipStream_t st) {
   // With rows ahead: as many workgroups as 16 waves per CU make, the rows in even rounds over
   // them. That is what stays resident up to 128 registers. Above, fewer do, and part of the
-  // grid waits: 12 waves with a gate per row beside fp32 (153 to 156) and per element in bf16
-  // (164), 8 per element in fp16 (170) and beside fp32 (186 to 189). Grids of 8, 12, 16 and 20
+  // grid waits: 12 waves with a gate per row in fp16 (137 to 140), in bf16 with rows of one wave
+  // (130) and beside fp32 (153 to 156), and with one per element in bf16 (164), 8 with one per
+  // element in fp16 (170) and beside fp32 (186 to 189). Grids of 8, 12, 16 and 20
   // waves, us: 4096 x 2560 norm 13.0, 10.0, 10.0, 10.1; bf16 sum, gate per row 24.7, 18.8, 18.8,
   // 20.3; per channel beside fp32 33.4, 34.7, 34.6, 37.8; 8192 x 4096, gate per element fp16
-  // 65.9, 73.3, 65.4, 71.9, beside fp32 88.9, 103, 89.0, 96.7. Against 16 stand rows of three and
-  // eight waves beside fp32: 8192 x 1536 per channel 34.6, 45.5, 42.6, 42.6, 3000 x 8192 62.9,
+  // 65.9, 73.3, 65.4, 71.9, beside fp32 88.9, 103, 89.0, 96.7. Against 16 stand rows of two and
+  // of eight waves beside fp32: 8192 x 1536 per channel 34.6, 45.5, 42.6, 42.6, 3000 x 8192 62.9,
   // 62.8, 65.4, 65.2. The other forms take a row each and leave the order to the dispatcher.
   const int rows_per = MAX_WAVES == 1 ? 4 : 1, wg_waves = MAX_WAVES == 1 ? 4 : waves;
   const long groups = (a.rows + rows_per - 1) / rows_per, most = AHEAD ? 256l * (16 / wg_waves) : 1l << 20;
