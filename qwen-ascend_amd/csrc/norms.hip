@@ -390,9 +390,9 @@ int launch_rows(const NormArgs& a, int waves, hipStream_t st) {
 //   per channel beside fp32  400 x 2048   5.5 /  6.5     2048 x 2048 14.3 / 17.9    2048 x 8192  55.0 / 46.3
 //   gate per row, fp16      1003 x 2048   6.8 /  6.8     4096 x 2048 13.6 / 16.4    2048 x 4096  15.4 / 15.8
 // So two pieces win from the limit on for norms, for a gate per row in bf16 and for rows of 8192, but not for
-// rows of 2048 to 4096 in fp16 or under a gate per element or channel, which lose up to a quarter there; with
-// up to two rows per workgroup the row ahead is hardly ever loaded. Below the limit rows of 8192 under a gate
-// per row in bf16 lose as much (400: 10.9 / 8.4).
+// rows of 2048 in fp16 or under a gate per element or channel, which lose up to a quarter there, nor for rows
+// of 4096 in fp16 or per channel beside fp32 (up to a seventh); with up to two rows per workgroup the row ahead
+// is hardly ever loaded. Below the limit rows of 8192 under a gate per row in bf16 lose a quarter (400: 10.9 / 8.4).
 // Forms that spill: a gate per element on 16 waves in fp32 with four pieces, 24 words (2048 x 16384:
 // 188 us, 3.6 TB/s; a gate per row, without spills, 114 us, 4.7), fp16 beside fp32 4 words and bf16
 // beside fp32 1 (117 and 112 us, 4.0 and 4.2 TB/s; a gate per row 96 us, 4.2).
