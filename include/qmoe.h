@@ -419,6 +419,50 @@ int qmoe_token_logprobs(const void* logits, long ld, int type, const void* token
                         long ld_allowed, int T, int V, void* logprobs, void* entropy, int top, void* top_ids,
                         void* top_logprobs, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---- An attention layer over a paged cache: rotary positions, the new tokens' keys and values
+ *      stored, attention over them. No counterpart among the reference's kernels on this path (its
+ *      engine's RoPE, KV store and attention are fnx/engine.py's own, outside the expert path).
+ *      Rows [T, heads, D] are given by their element steps (token, head), a cache [n_pages, page,
+ *      Hkv, D] by its own (page, slot, head); the D elements of a head are contiguous.
+ *      The batch of B sequences: starts int32 [B + 1], ascending from 0: rows [starts[b], starts[b + 1])
+ *      are the new tokens of sequence b, its last ones (NULL: T == B, one row each); lengths int32
+ *      [B]: its tokens, the new ones among them; table int32 [B, table_width], rows table_ld apart:
+ *      entry p / page names the page of position p. An entry outside [0, n_pages) is no page, and
+ *      positions past the table have none. Nothing is read or written out of range whatever
+ *      these hold; two tokens must not be stored at one place. */
+/* The first rd elements of every head turned by its token's position, the rest copied. Pair i is
+ * (x[i], x[i + rd/2]), or (x[2i], x[2i+1]) for interleaved; frequencies: uint64 [rd/2], turns per
+ * position times 2^64; cosine and sine are multiplied by `turn`. positions [T]: int32, or int64
+ * for positions64; they may be negative. D <= 1024; QMOE_BF16, QMOE_F16 or QMOE_F32. y may be x
+ * itself with the same steps, and overlap it no other way. */
+int qmoe_rotate(const void* x, long x_token, long x_head, void* y, long y_token, long y_head, int type,
+                const void* positions, int positions64, const void* frequencies, int rd, int interleaved, float turn,
+                int T, int heads, int D, void* stream);
+/* Keys (turned, for rd > 0) and values of the new tokens written to their places; a token without
+ * a page, or behind the last sequence, is not. q [T, Hq, D], turned alike, to q_out, contiguous
+ * (Hq 0, both NULL: none; behind the last sequence as at position 0). positions NULL: a token's position in
+ * its sequence. Inputs must not overlap the caches. */
+int qmoe_append_kv(const void* k, long k_token, long k_head, const void* v, long v_token, long v_head, const void* q,
+                   long q_token, long q_head, void* q_out, int type, void* k_cache, long k_page, long k_slot,
+                   long k_cache_head, void* v_cache, long v_page, long v_slot, long v_cache_head, const void* table,
+                   long table_ld, int table_width, const void* lengths, const void* starts, const void* positions,
+                   int positions64, const void* frequencies, int rd, int interleaved, float turn, int T, int B, int Hq,
+                   int Hkv, int D, int page, long n_pages, void* stream);
+/* Attention of the new tokens: row (t, h) at position p sees keys j <= p (with a window > 0, those
+ * with j > p - window) that lie on a page; out [T, Hq, D], contiguous, = sum e^(s_j - m) v_j / sum
+ * e^(s_j - m), s_j = scale q.k_j, m = max s_j, in fp32 with one rounding (and the e^(s_j - m) rounded
+ * to `type` for the product with v). Query heads [h G, h G + G) share key head h, G = Hq / Hkv <= 64.
+ * A row that sees no key, or only scores of -inf, and every row behind the last sequence gives 0;
+ * what lies at places that a row does not see (NaN too) does not reach it. QMOE_BF16 or QMOE_F16; D <= 256 a
+ * multiple of 8, cache steps too, caches 16-byte aligned. Workspace: qmoe_paged_attention_workspace()
+ * bytes for the call's own sizes, 16-byte aligned (one_each: starts is NULL). */
+size_t qmoe_paged_attention_workspace(int T, int B, int Hq, int Hkv, int D, int page, int table_width, int one_each);
+int qmoe_paged_attention(const void* q, long q_token, long q_head, const void* k_cache, long k_page, long k_slot,
+                         long k_head, const void* v_cache, long v_page, long v_slot, long v_head, int type,
+                         const void* table, long table_ld, int table_width, const void* lengths, const void* starts,
+                         void* out, int T, int B, int Hq, int Hkv, int D, int page, long n_pages, float scale,
+                         int window, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

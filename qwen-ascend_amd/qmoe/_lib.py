@@ -93,6 +93,11 @@ SIGNATURES = {
     "qmoe_block_residual": (I, [P, L, I, P, L, I, P, I, P, L, I, I, I, F, P, L, P, I, P, L, L, I, F, F, P]),
     "qmoe_token_logprobs_workspace": (Z, [I, I, I, I]),
     "qmoe_token_logprobs": (I, [P, L, I, P, I, P, L, I, I, P, P, I, P, P, P, Z, P]),
+    "qmoe_rotate": (I, [P, L, L, P, L, L, I, P, I, P, I, I, F, I, I, I, P]),
+    "qmoe_append_kv": (I, [P, L, L, P, L, L, P, L, L, P, I, P, L, L, L, P, L, L, L, P, L, I, P, P, P, I, P, I, I, F, I, I, I,
+                           I, I, I, L, P]),
+    "qmoe_paged_attention_workspace": (Z, [I, I, I, I, I, I, I, I]),
+    "qmoe_paged_attention": (I, [P, L, L, P, L, L, L, P, L, L, L, I, P, L, I, P, P, P, I, I, I, I, I, I, L, F, I, P, Z, P]),
 }
 
 
