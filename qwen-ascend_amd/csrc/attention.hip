@@ -2,13 +2,46 @@
 //
 // Row (t, h) at position p of its sequence sees the keys j with p - window < j <= p that lie on a
 // page of the cache:  o = sum_j e^(s_j - m) v_j / sum_j e^(s_j - m),  s_j = scale * q.k_j,
-// m = max_j s_j. Scores, sums and the output's sums in fp32, one rounding at the end. A row that
-// sees no key, or whose scores are all -inf, gives 0.
+// m = max_j s_j. Scores, sums and the output's sums in fp32; the weights e^(s_j - m) are rounded
+// to the tensors' type for the matrix product with v, each output once. A row that sees no key, or whose scores
+// are all -inf, gives 0.
+//
+// One pass over the keys with a running maximum and sum. The rows that share a key head (a sequence's
+// tokens times the query heads of the group) are one matrix; a wave holds 32 of them. It takes
+// S^T = K Q^T and O^T += V^T P^T on 32 x 32 x 16 MFMAs: a lane then holds scores of one row only (lane & 31),
+// so that maximum and sum are sums over its own registers and one exchange with lane ^ 32, and the
+// weights lie in registers just as the second product reads them, once the keys of 16 are taken in the
+// order 4 half + (i & 3) + 8 (i >> 2). V's columns for it come out of LDS with transposing reads.
+//
+// Two ways to cut the work, in one launch:
+//  * sequences with more than 32 rows: 128 rows to a workgroup, which its four waves share out, and 64 keys
+//    at a time in LDS for all of them; where such tiles are few, their keys are cut into pieces;
+//  * sequences with up to 32 rows (single tokens): the waves of a workgroup hold the same rows and
+//    share out the keys, 32 each at a time. All keys of all such sequences and heads make one list
+//    of tiles of 128, of which every workgroup takes an equal share, however the lengths differ.
+// What lies in pieces or crosses shares is joined by a second launch.
 #include "paged.h"
 
+#include <algorithm>
+#include <cfloat>
 #include <cmath>
 
 namespace {
+
+typedef float f32x16_v __attribute__((ext_vector_type(16)));
+typedef float f32x4_v __attribute__((ext_vector_type(4)));
+typedef short s16x4_v __attribute__((ext_vector_type(4)));
+typedef short s16x8_v __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8_v __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2_v __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8_v __attribute__((ext_vector_type(8)));
+typedef __attribute__((address_space(3))) void lds_void;
+typedef __attribute__((address_space(1))) const void global_void;
+
+constexpr int ROWS = 128;      // rows of a workgroup, many-rows form
+constexpr int FEW = 32;        // rows up to which a sequence takes the few-rows form
+constexpr int FEW_KEYS = 128;  // keys of a tile of that form
+constexpr int D_MAX = 256, GROUP_MAX = 64;
 
 struct AttentionArgs {
   const void *q, *k, *v;
@@ -16,65 +49,734 @@ struct AttentionArgs {
   long q_token, q_head;
   CacheSteps kc, vc;
   Batch batch;
-  int Hq, Hkv, group, D, window;
-  float scale;
+  int Hq, Hkv, D, window;
+  FastDiv group, heads;
+  float scale;      // |scale| * log2(e), above 0
+  int negate;       // of a scale below 0
+  int same_pages;   // a run of 8 keys lies on one page
+  int few;          // FEW, or 0: all sequences take the many-rows form
+  int few_blocks, few_rows, many_tiles, pieces;
+  FastDiv piece_div;
+  float *few_part, *many_part;  // partial sums: rows of D, then pairs (maximum, sum)
 };
 
-// One wave per row: its lanes hold the elements of a head, one key after the other.
 template <typename E>
-__global__ __launch_bounds__(256) void attention_rows_kernel(AttentionArgs a) {
-  using raw = typename E::raw;
-  const int lane = threadIdx.x & 63;
-  const long row = blockIdx.x * 4l + (threadIdx.x >> 6);
-  if (row >= (long)a.batch.T * a.Hq) return;
-  const int t = (int)(row / a.Hq), h = (int)(row - (long)t * a.Hq), kv = h / a.group;
-  float q[4] = {}, o[4] = {}, m = -INFINITY, l = 0.f;
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (lane + 64 * i < a.D) q[i] = E::load(static_cast<const raw*>(a.q)[t * a.q_token + h * a.q_head + lane + 64 * i]);
-  const int b = a.batch.sequence(t);
-  if (b < a.batch.B) {
-    const long p = (long)a.batch.lengths[b] - a.batch.new_rows(b) + t - a.batch.first_row(b);
-    const int end = (int)min(p + 1, (long)a.batch.length(b)), begin = a.window ? (int)max(p - a.window + 1, 0l) : 0;
-    for (int j = begin; j < end; ++j) {
-      const long page = a.batch.page_of(b, j);
-      if (page < 0) continue;
-      const int slot = j - (int)a.batch.page.div(j) * (int)a.batch.page.d;
-      const raw* k = static_cast<const raw*>(a.k) + page * a.kc.page + slot * a.kc.slot + kv * a.kc.head;
-      const raw* v = static_cast<const raw*>(a.v) + page * a.vc.page + slot * a.vc.slot + kv * a.vc.head;
-      float s = 0.f, x[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        x[i] = 0.f;
-        if (lane + 64 * i < a.D) s += q[i] * E::load(k[lane + 64 * i]), x[i] = E::load(v[lane + 64 * i]);
-      }
-      s = wave_sum_f32(s) * a.scale;
-      if (s == -INFINITY) continue;
-      if (s > m) {
-        const float c = expf(m - s);
-        l *= c, m = s;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) o[i] *= c;
-      }
-      const float e = expf(s - m);
-      l += e;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) o[i] += e * x[i];
-    }
+struct Mma;
+template <>
+struct Mma<ElemBF16> {
+  using frag = bf16x8_v;
+  QMOE_DEV static f32x16_v mma(s16x8_v a, s16x8_v b, f32x16_v c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(frag, a), __builtin_bit_cast(frag, b), c, 0, 0, 0);
   }
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (lane + 64 * i < a.D) static_cast<raw*>(a.out)[row * a.D + lane + 64 * i] = E::store(l == 0.f ? 0.f : o[i] / l);
+  QMOE_DEV static uint32_t pack(float lo, float hi) { return pk_bf16(lo, hi); }
+  static constexpr uint32_t EXPONENT = 0x7f807f80u, ONE = 0x00800080u;
+};
+template <>
+struct Mma<ElemF16> {
+  using frag = f16x8_v;
+  QMOE_DEV static f32x16_v mma(s16x8_v a, s16x8_v b, f32x16_v c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(frag, a), __builtin_bit_cast(frag, b), c, 0, 0, 0);
+  }
+  QMOE_DEV static uint32_t pack(float lo, float hi) {
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2_v){lo, hi}, f16x2_v));
+  }
+  static constexpr uint32_t EXPONENT = 0x7c007c00u, ONE = 0x04000400u;
+};
+
+// max or sum with lane ^ 32
+QMOE_DEV float other_half(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float((threadIdx.x & 32) ? r[0] : r[1]);
 }
 
+// Heads of up to 32 * NK elements. In LDS rows are DP elements apart; the 16-byte pieces of a row are XOR'd with
+// its number, so that what one instruction reads of many rows spreads over the banks: rows of K one piece
+// each, rows of V 64 bytes each.
+template <int NK>
+struct Layout {
+  static constexpr int DC = 32 * NK, DP = NK <= 2 ? 64 : NK <= 4 ? 128 : 256, STRIDE = 2 * DP;
+  static constexpr int PIECES = DP / 8, RPI = 64 / PIECES;  // rows of a wave's load instruction
+  static constexpr int TILE = 64 * STRIDE, LDS = 4 * TILE;
+  QMOE_DEV static int k_swizzle(int row) { return DP == 64 ? (row >> 1) & 7 : DP == 128 ? row & 15 : row & 7; }
+  QMOE_DEV static int v_swizzle(int row) { return DP == 64 ? 4 * ((row >> 1) & 1) : 4 * (row & 3); }
+};
+
+// The keys that a lane's row sees: [low, high], those present in the tile.
+struct Seen {
+  int low, high;
+};
+
+// 32 rows of a wave against NJ blocks of 32 keys.
+template <typename E, int NK, int NJ>
+struct Rows {
+  using L = Layout<NK>;
+  f32x16_v o[NK];  // o[dt][r]: element 32 dt + 8 (r >> 2) + 4 half + (r & 3) of row lane & 31
+  float m, l;      // maximum in units of log2, sum of this half's keys
+
+  QMOE_DEV void clear() {
+    m = -INFINITY, l = 0.f;
+#pragma unroll
+    for (int dt = 0; dt < NK; ++dt)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) o[dt][r] = 0.f;
+  }
+
+  // Number in the tile of the key in register r of block j, in lanes of the first half; 4 more in the others.
+  QMOE_DEV static constexpr int key_of(int j, int r) { return 32 * j + 8 * (r >> 2) + (r & 3); }
+
+  // Scores s become weights relative to the running maximum, which moves only where a score exceeds
+  // it by 2^8: weights stay below 2^8, where fp32 and the 16-bit types hold them as well as below 1, and
+  // most tiles leave the output's registers alone.
+  QMOE_DEV void weigh(f32x16_v (&s)[NJ], float scale, s16x8_v (&p)[2 * NJ]) {
+    float t = s[0][0];
+#pragma unroll
+    for (int j = 0; j < NJ; ++j)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) t = fmaxf(t, s[j][r]);
+    t = fmaxf(t, other_half(t)) * scale;
+    if (__any(t > m + 8.f)) {
+      const float top = fmaxf(m, t), f = m == top ? 1.f : __builtin_amdgcn_exp2f(m - top);
+      m = top, l *= f;
+#pragma unroll
+      for (int dt = 0; dt < NK; ++dt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[dt][r] *= f;
+    }
+    const float base = m == -INFINITY ? 0.f : m;
+    float sum[4] = {};
+#pragma unroll
+    for (int j = 0; j < NJ; ++j)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        s[j][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j][r], scale, -base));
+        sum[r & 3] += s[j][r];
+      }
+    l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+#pragma unroll
+    for (int i = 0; i < 2 * NJ; ++i) {
+      uint32_t w[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) w[r] = Mma<E>::pack(s[i / 2][8 * (i & 1) + 2 * r], s[i / 2][8 * (i & 1) + 2 * r + 1]);
+      p[i] = __builtin_bit_cast(s16x8_v, (u32x4_v){w[0], w[1], w[2], w[3]});
+    }
+  }
+
+  // o += V^T p, V's rows in LDS. A lane of a transposing read names 4 elements of a row: in groups of 16 lanes,
+  // lane i row i >> 2 and elements 4 (i & 3) of 16; it gets element i of the four rows.
+  QMOE_DEV void add(const unsigned char* v, const s16x8_v (&p)[2 * NJ]) {
+    const int lane = threadIdx.x & 63, half = lane >> 5, row = 4 * half + ((lane >> 2) & 3);
+    const int piece = 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1), swizzle = L::v_swizzle(row);
+    const unsigned char* base = v + row * L::STRIDE + 8 * (lane & 1);
+#pragma unroll
+    for (int i = 0; i < 2 * NJ; ++i)
+#pragma unroll
+      for (int dt = 0; dt < NK; ++dt) {
+        const unsigned char* at = base + 16 * i * L::STRIDE + 16 * ((4 * dt + piece) ^ swizzle);
+        typedef __attribute__((address_space(3))) s16x4_v lds_frag;
+        const s16x4_v a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_frag*)at);
+        const s16x4_v b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_frag*)(at + 8 * L::STRIDE));
+        o[dt] = Mma<E>::mma(__builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7), p[i], o[dt]);
+      }
+  }
+
+  // Whether a value of V's rows in LDS is infinite or NaN.
+  QMOE_DEV static bool unusual(const unsigned char* v) {
+    const int lane = threadIdx.x & 63;
+    uint32_t any = 0;
+#pragma unroll 4
+    for (int i = lane; i < 32 * NJ * L::PIECES; i += 64) {
+      const u32x4_v w = *reinterpret_cast<const u32x4_v*>(v + 16 * i);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) any |= (w[q] & Mma<E>::EXPONENT) + Mma<E>::ONE;
+    }
+    return __any((any & 0x80008000u) != 0);
+  }
+
+  // The same sum key by key: a weight of 0 times a value that is infinite or NaN would be NaN, so values that
+  // a row does not see are taken out. Rare (an unusual value beside a tile's border), so short code.
+  QMOE_DEV void add_careful(const unsigned char* v, const f32x16_v (&s)[NJ], Seen seen, uint64_t present, int first) {
+    const int half = (threadIdx.x >> 5) & 1;
+#pragma unroll 1
+    for (int i = 0; i < 32 * NJ; ++i) {
+      const int of = i / 2;  // register of the key, in lanes of half i & 1
+      float w = 0.f;
+#pragma unroll
+      for (int j = 0; j < NJ; ++j)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) w = of == 16 * j + r ? s[j][r] : w;
+      const float other = other_half(w);
+      w = (i & 1) == half ? w : other;
+      const int key = key_of(of >> 4, of & 15) + 4 * (i & 1), swizzle = L::v_swizzle(key);
+      const bool sees_it = ((present >> key) & 1) && first + key >= seen.low && first + key <= seen.high;
+      const unsigned char* row = v + key * L::STRIDE + 8 * half;
+#pragma unroll
+      for (int dt = 0; dt < NK; ++dt)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const s16x4_v x = *reinterpret_cast<const s16x4_v*>(row + 16 * ((4 * dt + c) ^ swizzle));
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[dt][4 * c + e] += w * (sees_it ? E::load((uint16_t)x[e]) : 0.f);
+        }
+    }
+  }
+
+  // One tile: scores s, whose keys start at `first`; `whole`: every row sees all of them.
+  QMOE_DEV void take(f32x16_v (&s)[NJ], const unsigned char* v, float scale, bool whole, Seen seen, uint64_t present, int first) {
+    const int half = (threadIdx.x >> 5) & 1;
+    int careful = 0;
+    if (!whole) {
+      const int from = first + 4 * half, low = seen.low - from, high = seen.high - from;
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) {
+        const uint32_t there = (uint32_t)(present >> (32 * j)) >> (4 * half);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int key = key_of(j, r);
+          if (!((there >> (key & 31)) & 1) || key < low || key > high) s[j][r] = -INFINITY;
+        }
+      }
+      careful = __builtin_amdgcn_readfirstlane(unusual(v));
+    }
+    s16x8_v p[2 * NJ];
+    weigh(s, scale, p);
+    if (careful) add_careful(v, s, seen, present, first);
+    else add(v, p);
+  }
+};
+
+// Rows of q as the second operand of K Q^T: elements 16 ks + 8 half of row lane & 31.
+template <int NK>
+QMOE_DEV void load_q(s16x8_v (&q)[2 * NK], const uint16_t* row, int D, bool valid, int negate) {
+  const int half = (threadIdx.x >> 5) & 1;
+#pragma unroll
+  for (int ks = 0; ks < 2 * NK; ++ks) {
+    u32x4_v w = {0, 0, 0, 0};
+    if (valid && 16 * ks + 8 * half < D) {
+      w = *reinterpret_cast<const u32x4_any*>(row + 16 * ks + 8 * half);
+      if (negate) w ^= 0x80008000u;
+    }
+    q[ks] = __builtin_bit_cast(s16x8_v, w);
+  }
+}
+
+// Positions of a sequence's rows, as ints: what precedes its first new token, clamped.
+QMOE_DEV int tokens_before(const Batch& batch, int b, int n) {
+  return (int)max((long)batch.lengths[b] - n, -0x40000000l);
+}
+
+// A byte offset of lane `src` (wave-uniform) as a scalar.
+QMOE_DEV long read_lane(long v, int src) {
+  const uint32_t lo = __builtin_amdgcn_readlane((int)v, src), hi = __builtin_amdgcn_readlane((int)(v >> 32), src);
+  return (long)(((uint64_t)hi << 32) | lo);
+}
+
+// COUNT runs of rows, one 16-byte piece per lane, straight to LDS: run g is rows `src` + g * every of the
+// tile, whose offsets the lanes hold, to `to` + g * 1024 * every / RPI. Lanes past the head's elements load
+// nothing. A row that is not there is skipped, or zeroed. `run`: the rows of a run lie one step apart.
+template <int NK, int COUNT, bool KEYS>
+QMOE_DEV void load_rows(unsigned char* to, const unsigned char* base, long offset, uint64_t present, bool whole, bool run,
+                        int src, int every, uint32_t step, int D) {
+  using L = Layout<NK>;
+  const int lane = threadIdx.x & 63, row = lane / L::PIECES;
+  auto piece_of = [&](int mine) { return (lane % L::PIECES) ^ (KEYS ? L::k_swizzle(mine) : L::v_swizzle(mine)); };
+  if (whole && run) {
+#pragma unroll
+    for (int g = 0; g < COUNT; ++g) {
+      // (opaque, so that no sums of the base and a lane's offset are kept over the loop)
+      uint64_t p = reinterpret_cast<uint64_t>(base) + read_lane(offset, src + g * every);
+      asm volatile("" : "+s"(p));
+      const int piece = piece_of(src + g * every + row);
+      if (8 * piece < D)
+        __builtin_amdgcn_global_load_lds((global_void*)(p + (row * step + 16u * piece)),
+                                         (lds_void*)(to + g * (1024 * every / L::RPI)), 16, 0, 0);
+    }
+  } else {
+#pragma unroll 1
+    for (int g = 0; g < COUNT; ++g) {
+      const int mine = src + g * every + row, piece = piece_of(mine);
+      unsigned char* at = to + g * (1024 * every / L::RPI);
+      const long from = __shfl(offset, mine);
+      if (8 * piece < D) {
+        if ((present >> mine) & 1)
+          __builtin_amdgcn_global_load_lds((global_void*)(base + from + 16 * piece), (lds_void*)at, 16, 0, 0);
+        else if (!KEYS)
+          *reinterpret_cast<u32x4_v*>(at + 16 * lane) = (u32x4_v){0, 0, 0, 0};
+      }
+    }
+  }
+}
+
+// Bytes of a cache's row of position `key` on page `entry` (0 for none).
+QMOE_DEV long row_offset(const CacheSteps& c, const FastDiv& page, int entry, int key) {
+  const int slot = key - (int)page.div(key) * (int)page.d;
+  return entry < 0 ? 0 : 2 * (entry * c.page + slot * c.slot);
+}
+
+// ---------------------------------------------------------------- sequences of many rows
+
+template <typename E, int NK>
+QMOE_DEV void many_rows(const AttentionArgs& a, int block, unsigned char* lds) {
+  using L = Layout<NK>;
+  const int lane = threadIdx.x & 63, half = lane >> 5, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const Batch& batch = a.batch;
+  // heads next to each other (on XCDs of their own, whose L2 then holds few heads' keys), the last
+  // tiles, which see the most keys, first
+  const int rest = a.heads.div(block), h = block - rest * a.Hkv, back = a.piece_div.div(rest);
+  const int piece = rest - back * a.pieces, tile_of = a.many_tiles - 1 - back;
+  const int G = a.group.d;
+
+  // Sequence b's tiles start at start(b) G / ROWS + b: no two sequences' overlap, a few numbers are
+  // no tile at all. The rows behind the last sequence are one without keys.
+  int b = 0;
+  for (int i = 1; i <= batch.B; i += 64)
+    b += __popcll(__ballot(i + lane <= batch.B && batch.start(min(i + lane, batch.B)) * G / ROWS + i + lane <= tile_of));
+  const int row0 = batch.start(b), n = b < batch.B ? max(batch.start(b + 1) - row0, 0) : batch.T - row0, rows = n * G;
+  const int r0 = (tile_of - row0 * G / ROWS - b) * ROWS;
+  if (r0 < 0 || r0 >= rows || (b < batch.B && rows <= a.few)) return;
+  const int before = b < batch.B ? tokens_before(batch, b, n) : -0x40000000, length = b < batch.B ? batch.length(b) : 0;
+
+  // the workgroup's keys [begin, end), this piece's tiles of them
+  const int first_pos = before + (int)a.group.div(r0), last_pos = before + (int)a.group.div(min(r0 + ROWS, rows) - 1);
+  const int end = min(last_pos + 1, length), begin = a.window ? max(first_pos - a.window + 1, 0) & ~63 : 0;
+  const int tiles = end > begin ? (end - begin + 63) / 64 : 0;
+  const int used = max(1, min(a.pieces, (tiles + 3) / 4));
+  const int t0 = (int)((long)tiles * piece / used), t1 = piece < used ? (int)((long)tiles * (piece + 1) / used) : t0;
+
+  const int r = r0 + 32 * wave + (lane & 31), token = a.group.div(r), of = r - token * G;
+  const bool valid = r < rows;
+  const long row = (long)(row0 + token) * a.Hq + h * G + of;  // of the output
+  const int pos = before + token;
+  const Seen seen = {a.window ? pos - a.window + 1 : 0, valid ? pos : -1};
+  // the wave's first and last position
+  const bool live = r0 + 32 * wave < rows;
+  const int wave_first = before + (int)a.group.div(r0 + 32 * wave);
+  const int wave_last = live ? before + (int)a.group.div(min(r0 + 32 * wave + 32, rows) - 1) : -1;
+
+  s16x8_v q[2 * NK];
+  load_q<NK>(q, static_cast<const uint16_t*>(a.q) + (row0 + token) * a.q_token + (h * G + of) * a.q_head, a.D, valid, a.negate);
+  Rows<E, NK, 2> acc;
+  acc.clear();
+
+  const unsigned char* kb = static_cast<const unsigned char*>(a.k) + 2 * h * a.kc.head;
+  const unsigned char* vb = static_cast<const unsigned char*>(a.v) + 2 * h * a.vc.head;
+  const int* table = batch.table + b * batch.table_ld;
+  auto entry_of = [&](int tile) {
+    const int key = begin + 64 * tile + lane;
+    return key < end ? table[batch.page.div(key)] : -1;
+  };
+  // loads a tile, 1 KB at a time; returns which keys are there
+  constexpr int GROUPS = 64 / L::RPI / 4;
+  auto load = [&](int tile, int entry, unsigned char* to) {
+    const int key = begin + 64 * tile + lane;
+    if (entry >= batch.n_pages) entry = -1;
+    const uint64_t present = __ballot(entry >= 0);
+    const bool whole = present == ~0ull;
+    const long ko = row_offset(a.kc, batch.page, entry, key), vo = row_offset(a.vc, batch.page, entry, key);
+    to += 1024 * wave;
+    load_rows<NK, GROUPS, true>(to, kb, ko, present, whole, a.same_pages, wave * L::RPI, 4 * L::RPI, (uint32_t)(2 * a.kc.slot), a.D);
+    load_rows<NK, GROUPS, false>(to + L::TILE, vb, vo, present, whole, a.same_pages, wave * L::RPI, 4 * L::RPI,
+                                 (uint32_t)(2 * a.vc.slot), a.D);
+    return present;
+  };
+
+  if (a.D < L::DC) {  // the elements behind a head's
+    for (int i = threadIdx.x; i < L::LDS / 16; i += 256) reinterpret_cast<u32x4_v*>(lds)[i] = (u32x4_v){0, 0, 0, 0};
+    __syncthreads();
+  }
+  uint64_t present_next = 0;
+  int entry = -1;
+  if (t0 < t1) {
+    present_next = load(t0, entry_of(t0), lds + (t0 & 1) * 2 * L::TILE);
+    if (t0 + 1 < t1) entry = entry_of(t0 + 1);
+  }
+  const int k_row = lane & 31, k_base = k_row * L::STRIDE, k_swizzle = L::k_swizzle(k_row);
+  // One tile from LDS at `k`, while the next is loaded to `next`. (As a function of two pointers that
+  // share nothing, which spares a wait for the load before every transposing read.)
+  auto step = [&](int tile, const unsigned char* __restrict__ k, unsigned char* __restrict__ next) {
+    // the tile has landed, and every wave is past the one before it, whose half of LDS takes the next
+    asm volatile("" ::: "memory");
+    wait_vm_lgkm0<0>();
+    barrier_no_fence();
+    const uint64_t present = present_next;
+    if (tile + 1 < t1) {
+      present_next = load(tile + 1, entry, next);
+      if (tile + 2 < t1) entry = entry_of(tile + 2);
+    }
+    const int first = begin + 64 * tile;
+    if (first > wave_last || (a.window && first + 63 <= wave_first - a.window)) return;
+    f32x16_v s[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[j][i] = 0.f;
+#pragma unroll
+    for (int ks = 0; ks < 2 * NK; ++ks)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const s16x8_v f = *reinterpret_cast<const s16x8_v*>(k + k_base + 32 * j * L::STRIDE + 16 * ((2 * ks + half) ^ k_swizzle));
+        s[j] = Mma<E>::mma(f, q[ks], s[j]);
+      }
+    const bool whole = present == ~0ull && first + 63 <= wave_first && (!a.window || first > wave_last - a.window);
+    acc.take(s, k + L::TILE, a.scale, whole, seen, present, first);
+  };
+  for (int tile = t0; tile < t1; ++tile) step(tile, lds + (tile & 1) * 2 * L::TILE, lds + (~tile & 1) * 2 * L::TILE);
+
+  const float l = acc.l + other_half(acc.l);
+  if (!valid) return;
+  if (a.pieces > 1) {
+    const long all = (long)batch.T * a.Hq, at = piece * all + row;
+    if (half == 0) reinterpret_cast<float2*>(a.many_part + a.pieces * all * a.D)[at] = make_float2(acc.m, l);
+    if (l == 0.f) return;
+    float* to = a.many_part + at * a.D;
+#pragma unroll
+    for (int dt = 0; dt < NK; ++dt)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const int d = 32 * dt + 8 * c + 4 * half;
+        if (d < a.D) *reinterpret_cast<f32x4_v*>(to + d) = (f32x4_v){acc.o[dt][4 * c], acc.o[dt][4 * c + 1], acc.o[dt][4 * c + 2], acc.o[dt][4 * c + 3]};
+      }
+    return;
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  uint16_t* to = static_cast<uint16_t*>(a.out) + row * a.D;
+#pragma unroll
+  for (int dt = 0; dt < NK; ++dt)
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const int d = 32 * dt + 8 * c + 4 * half;
+      if (d < a.D)
+        *reinterpret_cast<uint2*>(to + d) = make_uint2(Mma<E>::pack(acc.o[dt][4 * c] * inv, acc.o[dt][4 * c + 1] * inv),
+                                                       Mma<E>::pack(acc.o[dt][4 * c + 2] * inv, acc.o[dt][4 * c + 3] * inv));
+    }
+}
+
+// ---------------------------------------------------------------- sequences of few rows
+
+// A sequence of few rows: its keys [begin, end) and tiles of 128 of them, 0 for one that is not.
+struct FewKeys {
+  int n, before, begin, end, tiles;
+};
+QMOE_DEV FewKeys few_keys(const AttentionArgs& a, int b) {
+  FewKeys s;
+  s.n = a.batch.new_rows(b);
+  s.before = tokens_before(a.batch, b, s.n);
+  s.end = min(s.before + s.n, a.batch.length(b));
+  s.begin = a.window ? max(s.before - a.window + 1, 0) & ~31 : 0;
+  const bool is = s.n > 0 && s.n * (int)a.group.d <= a.few;
+  s.tiles = is ? max(1, (max(s.end - s.begin, 0) + FEW_KEYS - 1) / FEW_KEYS) : 0;
+  return s;
+}
+
+// Tiles of all heads of the sequences before one's own and in all, by a wave's lanes.
+QMOE_DEV long prefix_sum(long v) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int o = 1; o < 64; o *= 2) {
+    const long w = __shfl_up(v, o);
+    if (lane >= o) v += w;
+  }
+  return v;
+}
+
+// The list of tiles: sequence, then head, then tile. Where tile f of it lies.
+struct Place {
+  int b;       // B: behind the end
+  long start;  // first tile of the sequence
+};
+QMOE_DEV Place locate(const AttentionArgs& a, long f) {
+  const int lane = threadIdx.x & 63;
+  long sum = 0;
+  for (int i = 0; i < a.batch.B; i += 64) {
+    const long mine = i + lane < a.batch.B ? (long)few_keys(a, i + lane).tiles * a.Hkv : 0;
+    const long upto = sum + prefix_sum(mine);
+    const uint64_t past = __ballot(upto > f);
+    if (past) {
+      const int at = __ffsll((unsigned long long)past) - 1;
+      return {i + at, read_lane(upto - mine, at)};
+    }
+    sum = read_lane(upto, 63);
+  }
+  return {a.batch.B, sum};
+}
+// Tiles that each of the workgroups takes.
+QMOE_DEV long share_of(const AttentionArgs& a) {
+  const int lane = threadIdx.x & 63;
+  long sum = 0;
+  for (int i = lane; i < a.batch.B; i += 64) sum += few_keys(a, i).tiles;
+  const long total = read_lane(prefix_sum(sum), 63) * a.Hkv;
+  return max((total + a.few_blocks - 1) / a.few_blocks, 1l);
+}
+// Where a workgroup's part of a head's keys is kept: it has at most two that others share, one that
+// it ends with and one that it goes on with.
+QMOE_DEV long part_of(long block, bool begins) { return 2 * block + (begins ? 1 : 0); }
+
+template <typename E, int NK>
+QMOE_DEV void few_rows(const AttentionArgs& a, int block, unsigned char* lds) {
+  using L = Layout<NK>;
+  __shared__ float m_of[4][32], l_of[4][32];
+  const int lane = threadIdx.x & 63, half = lane >> 5, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const Batch& batch = a.batch;
+  const int G = a.group.d;
+
+  if (!a.many_tiles) {  // rows behind the last sequence
+    const long from = (long)batch.start(batch.B) * a.Hq * a.D / 8, to = (long)batch.T * a.Hq * a.D / 8;
+    for (long i = from + block * 256l + threadIdx.x; i < to; i += a.few_blocks * 256l)
+      static_cast<u32x4_v*>(a.out)[i] = (u32x4_v){0, 0, 0, 0};
+  }
+
+  // (all that locates the work is the same in every lane: kept in scalars)
+  const long share = share_of(a), stop = share * (block + 1);
+  long f = share * block;
+  Place place = locate(a, f);
+  while (f < stop && place.b < batch.B) {
+    const int b = place.b;
+    const FewKeys keys = few_keys(a, b);
+    const int h = __builtin_amdgcn_readfirstlane((int)((f - place.start) / keys.tiles));
+    const long head_start = place.start + (long)h * keys.tiles;
+    const int x0 = (int)(f - head_start), x1 = (int)min((long)keys.tiles, stop - head_start);
+    f = head_start + x1;
+    const int row0 = batch.first_row(b), rows = keys.n * G;
+
+    const int r = lane & 31, token = a.group.div(r), of = r - token * G;
+    const bool valid = r < rows;
+    const int pos = keys.before + token;
+    const Seen seen = {a.window ? pos - a.window + 1 : 0, valid ? pos : -1};
+    s16x8_v q[2 * NK];
+    load_q<NK>(q, static_cast<const uint16_t*>(a.q) + (row0 + token) * a.q_token + (h * G + of) * a.q_head, a.D, valid, a.negate);
+    Rows<E, NK, 1> acc;
+    acc.clear();
+
+    const unsigned char* kb = static_cast<const unsigned char*>(a.k) + 2 * h * a.kc.head + 16 * half;
+    const unsigned char* vb = static_cast<const unsigned char*>(a.v) + 2 * h * a.vc.head;
+    const int* table = batch.table + b * batch.table_ld;
+    auto first_of = [&](int x) { return keys.begin + FEW_KEYS * x + 32 * wave; };
+    auto entry_of = [&](int x) {
+      const int key = first_of(x) + (lane & 31);
+      return key < keys.end ? table[batch.page.div(key)] : -1;
+    };
+    unsigned char* mine = lds + wave * 64 * L::STRIDE;  // two times 32 rows of V
+    // K's rows go straight to registers: lane & 31 is the row of the first operand
+    auto load = [&](int x, int entry, s16x8_v (&k)[2 * NK], unsigned char* to) {
+      const int key = first_of(x) + (lane & 31);
+      if (entry >= batch.n_pages) entry = -1;
+      const uint64_t present = __ballot(entry >= 0);
+      const bool whole = present == ~0ull;
+      const long ko = row_offset(a.kc, batch.page, entry, key), vo = row_offset(a.vc, batch.page, entry, key);
+#pragma unroll
+      for (int ks = 0; ks < 2 * NK; ++ks) {
+        u32x4_v w = {0, 0, 0, 0};
+        if (entry >= 0 && 16 * ks + 8 * half < a.D) w = *reinterpret_cast<const u32x4_v*>(kb + ko + 32 * ks);
+        k[ks] = __builtin_bit_cast(s16x8_v, w);
+      }
+      load_rows<NK, 32 / L::RPI, false>(to, vb, vo, present, whole, a.same_pages, 0, L::RPI,
+                                        (uint32_t)(2 * a.vc.slot), a.D);
+      return present;
+    };
+    s16x8_v k[2 * NK], k_next[2 * NK];
+    uint64_t present_next = 0;
+    int entry = -1;
+    if (x0 < x1) {
+      present_next = load(x0, entry_of(x0), k_next, mine + (x0 & 1) * 32 * L::STRIDE);
+      if (x0 + 1 < x1) entry = entry_of(x0 + 1);
+    }
+    auto step = [&](int x, const unsigned char* __restrict__ v, unsigned char* __restrict__ next) {
+      asm volatile("" ::: "memory");
+      wait_vm_lgkm0<0>();
+      asm volatile("" ::: "memory");
+#pragma unroll
+      for (int ks = 0; ks < 2 * NK; ++ks) k[ks] = k_next[ks];
+      const uint64_t present = present_next;
+      if (x + 1 < x1) {
+        present_next = load(x + 1, entry, k_next, next);
+        if (x + 2 < x1) entry = entry_of(x + 2);
+      }
+      const int first = first_of(x);
+      f32x16_v s[1];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[0][i] = 0.f;
+#pragma unroll
+      for (int ks = 0; ks < 2 * NK; ++ks) s[0] = Mma<E>::mma(k[ks], q[ks], s[0]);
+      const bool whole = present == ~0ull && first + 31 <= keys.before && (!a.window || first > keys.before + keys.n - 1 - a.window);
+      acc.take(s, v, a.scale, whole, seen, present, first);
+    };
+    for (int x = x0; x < x1; ++x) step(x, mine + (x & 1) * 32 * L::STRIDE, mine + (~x & 1) * 32 * L::STRIDE);
+
+    // the four waves' sums: each brought to the common maximum, then added through LDS
+    const float l = acc.l + other_half(acc.l);
+    if (half == 0) m_of[wave][r] = acc.m, l_of[wave][r] = l;
+    __syncthreads();  // (and V's rows in LDS are done with)
+    float top = m_of[0][r];
+#pragma unroll
+    for (int w = 1; w < 4; ++w) top = fmaxf(top, m_of[w][r]);
+    const float scale = acc.m == top ? 1.f : __builtin_amdgcn_exp2f(acc.m - top);
+    f32x4_v* sums = reinterpret_cast<f32x4_v*>(lds) + (wave * 32 + r) * (L::DC / 4);
+#pragma unroll
+    for (int dt = 0; dt < NK; ++dt)
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+        sums[(8 * dt + 2 * c + half) ^ (r & 7)] = (f32x4_v){acc.o[dt][4 * c] * scale, acc.o[dt][4 * c + 1] * scale,
+                                                            acc.o[dt][4 * c + 2] * scale, acc.o[dt][4 * c + 3] * scale};
+    __syncthreads();
+    const bool alone = x0 == 0 && x1 == keys.tiles;
+    const long part = part_of(block, x0 == 0);
+    const int quads = a.D / 4;
+    for (int i = threadIdx.x; i < rows * quads; i += 256) {
+      const int at = i / quads, d = i - at * quads;
+      float best = m_of[0][at], total = 0.f;
+#pragma unroll
+      for (int w = 1; w < 4; ++w) best = fmaxf(best, m_of[w][at]);
+      f32x4_v sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        sum += reinterpret_cast<const f32x4_v*>(lds)[(w * 32 + at) * (L::DC / 4) + (d ^ (at & 7))];
+        total += l_of[w][at] * (m_of[w][at] == best ? 1.f : __builtin_amdgcn_exp2f(m_of[w][at] - best));
+      }
+      if (alone) {
+        const float inv = total == 0.f ? 0.f : 1.f / total;
+        const int tok = a.group.div(at);
+        const long row = (long)(row0 + tok) * a.Hq + h * G + at - tok * G;
+        reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + row * a.D)[d] =
+            make_uint2(Mma<E>::pack(sum[0] * inv, sum[1] * inv), Mma<E>::pack(sum[2] * inv, sum[3] * inv));
+      } else {
+        reinterpret_cast<f32x4_v*>(a.few_part + (part * a.few_rows + at) * a.D)[d] = sum;
+        if (d == 0)
+          reinterpret_cast<float2*>(a.few_part + 2l * a.few_blocks * a.few_rows * a.D)[part * a.few_rows + at] = make_float2(best, total);
+      }
+    }
+    __syncthreads();
+    if (f >= place.start + (long)keys.tiles * a.Hkv && f < stop) place = locate(a, f);
+  }
+}
+
+template <typename E, int NK>
+__global__ __launch_bounds__(256, (NK <= 4 ? 2 : 1)) void attention_kernel(AttentionArgs a) {
+  __shared__ __align__(16) unsigned char lds[Layout<NK>::LDS];
+  if ((int)blockIdx.x < a.few_blocks) few_rows<E, NK>(a, blockIdx.x, lds);
+  else many_rows<E, NK>(a, blockIdx.x - a.few_blocks, lds);
+}
+
+// ---------------------------------------------------------------- joining
+
+// One row's parts: sums of D and (maximum, sum), `count` of them; a workgroup per row, its waves take every
+// fourth part, then their sums are joined through LDS.
+template <typename E, typename At>
+QMOE_DEV void join_row(const float* sums, const float2* tops, At at, int count, uint16_t* out, int D) {
+  __shared__ float part[4][D_MAX], m_of[4], l_of[4];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  float m = -INFINITY, l = 0.f;
+  f32x4_v o = {0.f, 0.f, 0.f, 0.f};
+  const bool mine = 4 * lane < D;
+  for (int c = wave; c < count; c += 4) {
+    const long p = at(c);
+    const float2 t = tops[p];
+    if (t.y == 0.f) continue;
+    f32x4_v x = {0.f, 0.f, 0.f, 0.f};
+    if (mine) x = *reinterpret_cast<const f32x4_v*>(sums + p * D + 4 * lane);
+    const float top = fmaxf(m, t.x), f = m == top ? 1.f : __builtin_amdgcn_exp2f(m - top);
+    const float g = t.x == top ? 1.f : __builtin_amdgcn_exp2f(t.x - top);
+    m = top, l = l * f + t.y * g;
+    o = o * f + x * g;
+  }
+  if (mine) *reinterpret_cast<f32x4_v*>(&part[wave][4 * lane]) = o;
+  if (lane == 0) m_of[wave] = m, l_of[wave] = l;
+  __syncthreads();
+  float top = m_of[0], total = 0.f, sum = 0.f;
+#pragma unroll
+  for (int w = 1; w < 4; ++w) top = fmaxf(top, m_of[w]);
+  const int d = threadIdx.x;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    const float f = m_of[w] == top ? 1.f : __builtin_amdgcn_exp2f(m_of[w] - top);
+    total += l_of[w] * f;
+    if (d < D) sum += part[w][d] * f;
+  }
+  if (d < D) out[d] = E::store(total == 0.f ? 0.f : sum / total);
+}
+
+// Blocks [0, few_blocks) x few_rows: the head whose tiles the first boundary inside lies between shares
+// block - 1 and block, one row each. Behind them one for every row, where the many-rows form cut keys
+// into pieces.
 template <typename E>
+__global__ __launch_bounds__(256) void join_kernel(AttentionArgs a) {
+  const Batch& batch = a.batch;
+  const int few = a.few_blocks * a.few_rows, G = a.group.d;
+  if ((int)blockIdx.x < few) {
+    const int block = blockIdx.x / a.few_rows, at = blockIdx.x - block * a.few_rows;
+    if (block == 0) return;
+    const long share = share_of(a), f = share * block;
+    const Place place = locate(a, f);
+    if (place.b >= batch.B) return;
+    const FewKeys keys = few_keys(a, place.b);
+    const int h = (int)((f - place.start) / keys.tiles);
+    const long start = place.start + (long)h * keys.tiles;
+    if (start == f || start < f - share || at >= keys.n * G) return;
+    const long last = (start + keys.tiles - 1) / share;
+    const int token = a.group.div(at);
+    const long row = (long)(batch.first_row(place.b) + token) * a.Hq + h * G + at - token * G;
+    join_row<E>(a.few_part, reinterpret_cast<const float2*>(a.few_part + 2l * a.few_blocks * a.few_rows * a.D),
+                [&](int c) { return part_of(block - 1 + c, c == 0) * a.few_rows + at; }, (int)(last - block + 2),
+                static_cast<uint16_t*>(a.out) + row * a.D, a.D);
+  } else {
+    const int row = blockIdx.x - few, t = row / a.Hq;
+    const int b = batch.sequence(t);
+    if (b < batch.B && batch.new_rows(b) * G <= a.few) return;
+    const long all = (long)batch.T * a.Hq;
+    join_row<E>(a.many_part, reinterpret_cast<const float2*>(a.many_part + a.pieces * all * a.D),
+                [&](int c) { return c * all + row; }, a.pieces, static_cast<uint16_t*>(a.out) + (long)row * a.D, a.D);
+  }
+}
+
+// ---------------------------------------------------------------- host
+
+// How a call is cut, from what the host knows of it.
+struct Plan {
+  int few, few_blocks, few_rows, many_tiles, pieces;
+  size_t few_floats, many_floats;
+};
+Plan plan_for(int T, int B, int Hq, int Hkv, int D, int page, int width, bool one_each) {
+  const int G = Hq / Hkv;
+  Plan p = {};
+  const bool many = one_each ? G > FEW : (long)T * G > FEW;  // may there be sequences of many rows
+  const bool few = !many || (!one_each && B > 1);            // and of few
+  p.few = few ? FEW : 0;
+  p.few_rows = one_each ? G : FEW;
+  p.pieces = 1;
+  const int slots = D > 128 ? 256 : 512;  // workgroups that run at once
+  const long most = (long)width * page;   // keys
+  if (few) {
+    const long tiles = (long)B * Hkv * std::max<long>(1, (most + FEW_KEYS - 1) / FEW_KEYS);
+    p.few_blocks = (int)std::min<long>(slots, tiles);
+    p.few_floats = 2l * p.few_blocks * p.few_rows * (D + 2);
+  }
+  if (many) {
+    p.many_tiles = (int)((long)T * G / ROWS) + B + 1;
+    const long items = (((long)T * G + ROWS - 1) / ROWS) * Hkv;
+    p.pieces = (int)std::max<long>(1, std::min({16l, slots / items, (most + 255) / 256}));
+    if (p.pieces > 1) p.many_floats = (size_t)p.pieces * T * Hq * (D + 2);
+  }
+  return p;
+}
+
+template <typename E, int NK>
 int launch(const AttentionArgs& a, hipStream_t st) {
-  const long rows = (long)a.batch.T * a.Hq;
-  hipLaunchKernelGGL((attention_rows_kernel<E>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, a);
+  const long blocks = a.few_blocks + (long)a.many_tiles * a.Hkv * a.pieces;
+  if (blocks > 0x7fffffffl) return QMOE_EINVAL;
+  hipLaunchKernelGGL((attention_kernel<E, NK>), dim3((unsigned)blocks), dim3(256), 0, st, a);
+  const int rc = (int)hipGetLastError();
+  const long joins = (long)a.few_blocks * a.few_rows + (a.pieces > 1 ? (long)a.batch.T * a.Hq : 0);
+  if (rc || joins == 0) return rc;
+  hipLaunchKernelGGL((join_kernel<E>), dim3((unsigned)joins), dim3(256), 0, st, a);
   return (int)hipGetLastError();
 }
 
-constexpr int D_MAX = 256, GROUP_MAX = 64;
+template <typename E>
+int dispatch(const AttentionArgs& a, hipStream_t st) {
+  if (a.D <= 64) return launch<E, 2>(a, st);
+  if (a.D <= 96) return launch<E, 3>(a, st);
+  if (a.D <= 128) return launch<E, 4>(a, st);
+  if (a.D <= 192) return launch<E, 6>(a, st);
+  return launch<E, 8>(a, st);
+}
 
 bool bad_shape(int T, int B, int Hq, int Hkv, int D) {
   return T < 0 || B < 0 || Hq < 1 || Hkv < 1 || Hq > 4096 || Hq % Hkv || Hq / Hkv > GROUP_MAX || D < 8 || D > D_MAX || D % 8 ||
@@ -86,7 +788,9 @@ bool bad_shape(int T, int B, int Hq, int Hkv, int D) {
 extern "C" {
 
 size_t qmoe_paged_attention_workspace(int T, int B, int Hq, int Hkv, int D, int page, int table_width, int one_each) {
-  return 0;
+  if (bad_shape(T, B, Hq, Hkv, D) || page < 1 || table_width < 0) return 0;
+  const Plan p = plan_for(T, B, Hq, Hkv, D, page, table_width, one_each);
+  return 4 * (p.few_floats + p.many_floats);
 }
 
 int qmoe_paged_attention(const void* q, long q_token, long q_head, const void* k_cache, long k_page, long k_slot,
@@ -95,13 +799,18 @@ int qmoe_paged_attention(const void* q, long q_token, long q_head, const void* k
                          void* out, int T, int B, int Hq, int Hkv, int D, int page, long n_pages, float scale,
                          int window, void* workspace, size_t workspace_bytes, void* stream) {
   if (bad_shape(T, B, Hq, Hkv, D) || (type != QMOE_BF16 && type != QMOE_F16)) return QMOE_EINVAL;
+  constexpr float LOG2E = 1.44269504088896341f;
   if (page < 1 || page > 1 << 30 || n_pages < 0 || table_width < 0 || table_ld < 0 || (!starts && T != B) ||
-      window < 0 || !std::isfinite(scale))
+      window < 0 || !std::isfinite(scale * LOG2E))
     return QMOE_EINVAL;
   if ((k_page | k_slot | k_head | v_page | v_slot | v_head) & 7) return QMOE_EINVAL;
   if ((reinterpret_cast<uintptr_t>(k_cache) | reinterpret_cast<uintptr_t>(v_cache)) & 15) return QMOE_EINVAL;
   if (T == 0) return QMOE_OK;
   if (!q || !out || missing(k_cache, v_cache, n_pages, table, table_width, lengths, B)) return QMOE_EINVAL;
+  const Plan p = plan_for(T, B, Hq, Hkv, D, page, table_width, !starts);
+  if (p.few_floats + p.many_floats &&
+      (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15) || workspace_bytes < 4 * (p.few_floats + p.many_floats)))
+    return QMOE_EWORKSPACE;
   AttentionArgs a = {};
   a.q = q, a.k = k_cache, a.v = v_cache, a.out = out, a.q_token = q_token, a.q_head = q_head;
   a.kc = {k_page, k_slot, k_head}, a.vc = {v_page, v_slot, v_head};
@@ -109,8 +818,14 @@ int qmoe_paged_attention(const void* q, long q_token, long q_head, const void* k
   a.batch.starts = static_cast<const int*>(starts);
   a.batch.table_ld = table_ld, a.batch.n_pages = n_pages, a.batch.T = T, a.batch.B = B, a.batch.width = table_width;
   a.batch.page = FastDiv(page);
-  a.Hq = Hq, a.Hkv = Hkv, a.group = Hq / Hkv, a.D = D, a.window = window, a.scale = scale;
-  return type == QMOE_BF16 ? launch<ElemBF16>(a, (hipStream_t)stream) : launch<ElemF16>(a, (hipStream_t)stream);
+  a.Hq = Hq, a.Hkv = Hkv, a.D = D, a.window = window;
+  a.group = FastDiv(Hq / Hkv), a.heads = FastDiv(Hkv), a.piece_div = FastDiv(p.pieces);
+  a.scale = std::max(std::fabs(scale) * LOG2E, FLT_MIN), a.negate = scale < 0;
+  a.same_pages = page % 8 == 0 && std::max(k_slot, v_slot) < 1 << 26;
+  a.few = p.few, a.few_blocks = p.few_blocks, a.few_rows = p.few_rows, a.many_tiles = p.many_tiles, a.pieces = p.pieces;
+  a.few_part = static_cast<float*>(workspace);
+  a.many_part = a.few_part + p.few_floats;
+  return type == QMOE_BF16 ? dispatch<ElemBF16>(a, (hipStream_t)stream) : dispatch<ElemF16>(a, (hipStream_t)stream);
 }
 
 }  // extern "C"

@@ -38,10 +38,9 @@ struct Batch {
     return b;
   }
   // First new row and number of new rows of sequence b; both within [0, T] whatever `starts` holds.
-  QMOE_DEV int first_row(int b) const { return starts ? min(max(starts[b], 0), T) : b; }
-  QMOE_DEV int new_rows(int b) const {
-    return starts ? max(min(max(starts[b + 1], 0), T) - first_row(b), 0) : 1;
-  }
+  QMOE_DEV int start(int b) const { return starts ? min(max(starts[b], 0), T) : b; }
+  QMOE_DEV int first_row(int b) const { return start(b); }
+  QMOE_DEV int new_rows(int b) const { return starts ? max(start(b + 1) - start(b), 0) : 1; }
   // Cached tokens of sequence b, as many as its row of the table can hold.
   QMOE_DEV int length(int b) const {
     const long most = min((long)width * page.d, 0x7fffffffl);
