@@ -53,12 +53,32 @@ struct AttentionArgs {
   FastDiv group, heads;
   float scale;      // |scale| * log2(e), above 0
   int negate;       // of a scale below 0
-  int same_pages;   // a run of 8 keys lies on one page
+  int same_pages;   // 16 keys on 16 lie on one page
   int few;          // FEW, or 0: all sequences take the many-rows form
-  int few_blocks, few_rows, many_tiles, pieces;
+  int few_blocks, few_rows, many_tiles, pieces, slots;
   FastDiv piece_div;
   float *few_part, *many_part;  // partial sums: rows of D, then pairs (maximum, sum)
 };
+
+// Maxima and sums behind the partial sums' rows.
+QMOE_DEV float2* few_tops(const AttentionArgs& a) {
+  return reinterpret_cast<float2*>(a.few_part + 2l * a.few_blocks * a.few_rows * a.D);
+}
+QMOE_DEV float2* many_tops(const AttentionArgs& a) {
+  return reinterpret_cast<float2*>(a.many_part + 2l * (a.slots + 1) * ROWS * a.D);
+}
+
+// Inclusive sums over a wave's lanes.
+QMOE_DEV int prefix_sum(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);  // row_shr 1, 2, 4, 8
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // row_bcast 15: to rows 1 and 3
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // row_bcast 31: to rows 2 and 3
+  return v;
+}
+QMOE_DEV int lane_of(int v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
 
 template <typename E>
 struct Mma;
@@ -270,12 +290,13 @@ QMOE_DEV long read_lane(long v, int src) {
   return (long)(((uint64_t)hi << 32) | lo);
 }
 
-// COUNT runs of rows, one 16-byte piece per lane, straight to LDS: run g is rows `src` + g * every of the
-// tile, whose offsets the lanes hold, to `to` + g * 1024 * every / RPI. Lanes past the head's elements load
-// nothing. A row that is not there is skipped, or zeroed. `run`: the rows of a run lie one step apart.
-template <int NK, int COUNT, bool KEYS>
+// COUNT runs of rows, one 16-byte piece per lane, straight to LDS: run g is rows src + g * EVERY of the
+// tile, whose offsets the lanes hold, to `to` + 1 KB * g * EVERY / RPI. Lanes past the head's elements load nothing
+// (FULL: there are none). A row that is not there is skipped, or zeroed. `run`: 16 rows on 16 lie one step
+// apart, so that an offset of each 16, as a scalar, does for all of them.
+template <int NK, bool FULL, int COUNT, int EVERY, bool KEYS>
 QMOE_DEV void load_rows(unsigned char* to, const unsigned char* base, long offset, uint64_t present, bool whole, bool run,
-                        int src, int every, uint32_t step, int D) {
+                        int src, uint32_t step, int D) {
   using L = Layout<NK>;
   const int lane = threadIdx.x & 63, row = lane / L::PIECES;
   auto piece_of = [&](int mine) { return (lane % L::PIECES) ^ (KEYS ? L::k_swizzle(mine) : L::v_swizzle(mine)); };
@@ -283,20 +304,21 @@ QMOE_DEV void load_rows(unsigned char* to, const unsigned char* base, long offse
 #pragma unroll
     for (int g = 0; g < COUNT; ++g) {
       // (opaque, so that no sums of the base and a lane's offset are kept over the loop)
-      uint64_t p = reinterpret_cast<uint64_t>(base) + read_lane(offset, src + g * every);
+      const int from = src + g * EVERY;
+      uint64_t p = reinterpret_cast<uint64_t>(base) + read_lane(offset, from & ~15) + (from & 15) * step;
       asm volatile("" : "+s"(p));
-      const int piece = piece_of(src + g * every + row);
-      if (8 * piece < D)
+      const int piece = piece_of(from + row);
+      if (FULL || 8 * piece < D)
         __builtin_amdgcn_global_load_lds((global_void*)(p + (row * step + 16u * piece)),
-                                         (lds_void*)(to + g * (1024 * every / L::RPI)), 16, 0, 0);
+                                         (lds_void*)(to + g * (1024 * EVERY / L::RPI)), 16, 0, 0);
     }
   } else {
 #pragma unroll 1
     for (int g = 0; g < COUNT; ++g) {
-      const int mine = src + g * every + row, piece = piece_of(mine);
-      unsigned char* at = to + g * (1024 * every / L::RPI);
+      const int mine = src + g * EVERY + row, piece = piece_of(mine);
+      unsigned char* at = to + g * (1024 * EVERY / L::RPI);
       const long from = __shfl(offset, mine);
-      if (8 * piece < D) {
+      if (FULL || 8 * piece < D) {
         if ((present >> mine) & 1)
           __builtin_amdgcn_global_load_lds((global_void*)(base + from + 16 * piece), (lds_void*)at, 16, 0, 0);
         else if (!KEYS)
@@ -308,13 +330,70 @@ QMOE_DEV void load_rows(unsigned char* to, const unsigned char* base, long offse
 
 // Bytes of a cache's row of position `key` on page `entry` (0 for none).
 QMOE_DEV long row_offset(const CacheSteps& c, const FastDiv& page, int entry, int key) {
-  const int slot = key - (int)page.div(key) * (int)page.d;
-  return entry < 0 ? 0 : 2 * (entry * c.page + slot * c.slot);
+  const uint32_t slot = key - page.div(key) * page.d;
+  return entry < 0 ? 0 : (long)((uint64_t)(uint32_t)entry * (uint32_t)(2 * c.page) + slot * (uint32_t)(2 * c.slot));
 }
 
 // ---------------------------------------------------------------- sequences of many rows
 
-template <typename E, int NK>
+// A tile of 128 rows of a sequence of many, or of the rows behind the last one (b = B, no keys).
+struct ManyTile {
+  int b, row0, rows, r0, before, begin, tiles;  // r0 < 0: none
+};
+QMOE_DEV ManyTile many_tile(const AttentionArgs& a, int number) {
+  const int lane = threadIdx.x & 63, G = a.group.d;
+  const Batch& batch = a.batch;
+  ManyTile t = {};
+  // Sequence b's tiles start at start(b) G / ROWS + b: no two sequences' overlap, a few numbers are
+  // no tile at all.
+  for (int i = 1; i <= batch.B; i += 64)
+    t.b += __popcll(__ballot(i + lane <= batch.B && batch.start(min(i + lane, batch.B)) * G / ROWS + i + lane <= number));
+  t.row0 = batch.start(t.b);
+  const bool is = t.b < batch.B;
+  const int n = is ? max(batch.start(t.b + 1) - t.row0, 0) : batch.T - t.row0;
+  t.rows = n * G;
+  t.r0 = (number - t.row0 * G / ROWS - t.b) * ROWS;
+  if (t.r0 >= t.rows || (is && t.rows <= a.few)) t.r0 = -1;
+  t.before = is ? tokens_before(batch, t.b, n) : -0x40000000;
+  const int first_pos = t.before + (int)a.group.div(max(t.r0, 0)), last_pos = t.before + (int)a.group.div(min(t.r0 + ROWS, t.rows) - 1);
+  const int end = min(last_pos + 1, is ? batch.length(t.b) : 0);
+  t.begin = a.window ? max(first_pos - a.window + 1, 0) & ~63 : 0;
+  t.tiles = end > t.begin ? (end - t.begin + 63) / 64 : 0;
+  return t;
+}
+
+// Where tiles are few, each is cut into pieces of so many 64 keys that all pieces of the call make up about
+// as many as run at once. Tiles of a sequence count alike, with the most keys that one of them may see; in
+// the list of all tiles' keys (sequence, tile, head), a piece that starts in stretch u of that size is kept at
+// 2 u, or 2 u + 1 if it is the first of its tile: a tile in pieces is longer than a stretch, so these differ.
+struct Pieces {
+  int size, start;  // in units of 64 keys: a piece; this tile's start in the list
+};
+QMOE_DEV Pieces pieces_of(const AttentionArgs& a, const ManyTile& t, int h) {
+  const int lane = threadIdx.x & 63, G = a.group.d;
+  const Batch& batch = a.batch;
+  int total = 0, before = 0, of = 0;
+  for (int i = 0; i < batch.B; i += 64) {
+    int tiles = 0, keys = 0;
+    if (i + lane < batch.B) {
+      const int n = batch.new_rows(i + lane), rows = n * G;
+      if (rows > a.few) {
+        tiles = (rows + ROWS - 1) / ROWS;
+        keys = min(tokens_before(batch, i + lane, n) + n, batch.length(i + lane));
+        keys = (max(keys, 0) + 63) / 64;
+        if (a.window) keys = min(keys, (a.window + ROWS / G + 64) / 64 + 1);
+        keys = max(keys, 1);
+      }
+    }
+    const int mine = tiles * keys * a.Hkv, upto = prefix_sum(mine);
+    if (t.b >= i && t.b < i + 64) before = total + lane_of(upto - mine, t.b - i), of = lane_of(keys, t.b - i);
+    total += lane_of(upto, 63);
+  }
+  return {max(8, (total + a.slots - 1) / a.slots), before + (t.r0 / ROWS * a.Hkv + h) * of};
+}
+QMOE_DEV long piece_at(const Pieces& p, int piece) { return 2l * ((p.start + piece * p.size) / p.size) + (piece == 0); }
+
+template <typename E, int NK, bool FULL>
 QMOE_DEV void many_rows(const AttentionArgs& a, int block, unsigned char* lds) {
   using L = Layout<NK>;
   const int lane = threadIdx.x & 63, half = lane >> 5, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -322,25 +401,23 @@ QMOE_DEV void many_rows(const AttentionArgs& a, int block, unsigned char* lds) {
   // heads next to each other (on XCDs of their own, whose L2 then holds few heads' keys), the last
   // tiles, which see the most keys, first
   const int rest = a.heads.div(block), h = block - rest * a.Hkv, back = a.piece_div.div(rest);
-  const int piece = rest - back * a.pieces, tile_of = a.many_tiles - 1 - back;
-  const int G = a.group.d;
-
-  // Sequence b's tiles start at start(b) G / ROWS + b: no two sequences' overlap, a few numbers are
-  // no tile at all. The rows behind the last sequence are one without keys.
-  int b = 0;
-  for (int i = 1; i <= batch.B; i += 64)
-    b += __popcll(__ballot(i + lane <= batch.B && batch.start(min(i + lane, batch.B)) * G / ROWS + i + lane <= tile_of));
-  const int row0 = batch.start(b), n = b < batch.B ? max(batch.start(b + 1) - row0, 0) : batch.T - row0, rows = n * G;
-  const int r0 = (tile_of - row0 * G / ROWS - b) * ROWS;
-  if (r0 < 0 || r0 >= rows || (b < batch.B && rows <= a.few)) return;
-  const int before = b < batch.B ? tokens_before(batch, b, n) : -0x40000000, length = b < batch.B ? batch.length(b) : 0;
-
-  // the workgroup's keys [begin, end), this piece's tiles of them
-  const int first_pos = before + (int)a.group.div(r0), last_pos = before + (int)a.group.div(min(r0 + ROWS, rows) - 1);
-  const int end = min(last_pos + 1, length), begin = a.window ? max(first_pos - a.window + 1, 0) & ~63 : 0;
-  const int tiles = end > begin ? (end - begin + 63) / 64 : 0;
-  const int used = max(1, min(a.pieces, (tiles + 3) / 4));
-  const int t0 = (int)((long)tiles * piece / used), t1 = piece < used ? (int)((long)tiles * (piece + 1) / used) : t0;
+  const int piece = rest - back * a.pieces;
+  const ManyTile mt = many_tile(a, a.many_tiles - 1 - back);
+  if (mt.r0 < 0) return;
+  int t0 = 0, t1 = mt.tiles;
+  bool cut = false;
+  Pieces pieces = {};
+  if (a.pieces > 1) {
+    if (piece * 8 >= max(mt.tiles, 1)) return;  // no piece is shorter
+    pieces = pieces_of(a, mt, h);
+    const int count = min((mt.tiles + pieces.size - 1) / pieces.size, a.pieces);
+    if (piece >= max(count, 1)) return;
+    cut = count > 1;
+    t0 = piece * pieces.size;
+    if (piece + 1 < count) t1 = t0 + pieces.size;
+  }
+  const int G = a.group.d, b = mt.b, row0 = mt.row0, rows = mt.rows, r0 = mt.r0, before = mt.before, begin = mt.begin;
+  const int end = min(before + (int)a.group.div(min(r0 + ROWS, rows) - 1) + 1, b < batch.B ? batch.length(b) : 0);
 
   const int r = r0 + 32 * wave + (lane & 31), token = a.group.div(r), of = r - token * G;
   const bool valid = r < rows;
@@ -373,13 +450,13 @@ QMOE_DEV void many_rows(const AttentionArgs& a, int block, unsigned char* lds) {
     const bool whole = present == ~0ull;
     const long ko = row_offset(a.kc, batch.page, entry, key), vo = row_offset(a.vc, batch.page, entry, key);
     to += 1024 * wave;
-    load_rows<NK, GROUPS, true>(to, kb, ko, present, whole, a.same_pages, wave * L::RPI, 4 * L::RPI, (uint32_t)(2 * a.kc.slot), a.D);
-    load_rows<NK, GROUPS, false>(to + L::TILE, vb, vo, present, whole, a.same_pages, wave * L::RPI, 4 * L::RPI,
-                                 (uint32_t)(2 * a.vc.slot), a.D);
+    load_rows<NK, FULL, GROUPS, 4 * L::RPI, true>(to, kb, ko, present, whole, a.same_pages, wave * L::RPI, (uint32_t)(2 * a.kc.slot), a.D);
+    load_rows<NK, FULL, GROUPS, 4 * L::RPI, false>(to + L::TILE, vb, vo, present, whole, a.same_pages, wave * L::RPI,
+                                                   (uint32_t)(2 * a.vc.slot), a.D);
     return present;
   };
 
-  if (a.D < L::DC) {  // the elements behind a head's
+  if (!FULL) {  // the elements behind a head's
     for (int i = threadIdx.x; i < L::LDS / 16; i += 256) reinterpret_cast<u32x4_v*>(lds)[i] = (u32x4_v){0, 0, 0, 0};
     __syncthreads();
   }
@@ -423,10 +500,9 @@ QMOE_DEV void many_rows(const AttentionArgs& a, int block, unsigned char* lds) {
 
   const float l = acc.l + other_half(acc.l);
   if (!valid) return;
-  if (a.pieces > 1) {
-    const long all = (long)batch.T * a.Hq, at = piece * all + row;
-    if (half == 0) reinterpret_cast<float2*>(a.many_part + a.pieces * all * a.D)[at] = make_float2(acc.m, l);
-    if (l == 0.f) return;
+  if (cut) {
+    const long at = piece_at(pieces, piece) * ROWS + 32 * wave + (lane & 31);
+    if (half == 0) many_tops(a)[at] = make_float2(acc.m, l);
     float* to = a.many_part + at * a.D;
 #pragma unroll
     for (int dt = 0; dt < NK; ++dt)
@@ -467,50 +543,44 @@ QMOE_DEV FewKeys few_keys(const AttentionArgs& a, int b) {
   return s;
 }
 
-// Tiles of all heads of the sequences before one's own and in all, by a wave's lanes.
-QMOE_DEV long prefix_sum(long v) {
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int o = 1; o < 64; o *= 2) {
-    const long w = __shfl_up(v, o);
-    if (lane >= o) v += w;
+// The list of tiles: sequence, then head, then tile. Every workgroup takes `share` of them.
+struct FewList {
+  FewKeys mine;  // of sequence `lane`
+  int share;
+  QMOE_DEV FewList(const AttentionArgs& a) {
+    const int lane = threadIdx.x & 63;
+    mine = FewKeys{};
+    if (lane < a.batch.B) mine = few_keys(a, lane);
+    int sum = mine.tiles;
+    for (int i = 64 + lane; i < a.batch.B; i += 64) sum += few_keys(a, i).tiles;
+    const int total = lane_of(prefix_sum(sum), 63) * a.Hkv;
+    share = max((total + a.few_blocks - 1) / a.few_blocks, 1);
   }
-  return v;
-}
-
-// The list of tiles: sequence, then head, then tile. Where tile f of it lies.
-struct Place {
-  int b;       // B: behind the end
-  long start;  // first tile of the sequence
-};
-QMOE_DEV Place locate(const AttentionArgs& a, long f) {
-  const int lane = threadIdx.x & 63;
-  long sum = 0;
-  for (int i = 0; i < a.batch.B; i += 64) {
-    const long mine = i + lane < a.batch.B ? (long)few_keys(a, i + lane).tiles * a.Hkv : 0;
-    const long upto = sum + prefix_sum(mine);
-    const uint64_t past = __ballot(upto > f);
-    if (past) {
-      const int at = __ffsll((unsigned long long)past) - 1;
-      return {i + at, read_lane(upto - mine, at)};
+  // The sequence (B behind the end) that tile f of the list belongs to, its keys and its first tile.
+  QMOE_DEV int locate(const AttentionArgs& a, int f, FewKeys& keys, int& start) const {
+    const int lane = threadIdx.x & 63;
+    start = 0;
+    for (int i = 0; i < a.batch.B; i += 64) {
+      FewKeys k = mine;
+      if (i) k = i + lane < a.batch.B ? few_keys(a, i + lane) : FewKeys{};
+      const int tiles = k.tiles * a.Hkv, upto = start + prefix_sum(tiles);
+      const uint64_t past = __ballot(upto > f);
+      if (past) {
+        const int at = __ffsll((unsigned long long)past) - 1;
+        start = lane_of(upto - tiles, at);
+        keys = {lane_of(k.n, at), lane_of(k.before, at), lane_of(k.begin, at), lane_of(k.end, at), lane_of(k.tiles, at)};
+        return i + at;
+      }
+      start = lane_of(upto, 63);
     }
-    sum = read_lane(upto, 63);
+    return a.batch.B;
   }
-  return {a.batch.B, sum};
-}
-// Tiles that each of the workgroups takes.
-QMOE_DEV long share_of(const AttentionArgs& a) {
-  const int lane = threadIdx.x & 63;
-  long sum = 0;
-  for (int i = lane; i < a.batch.B; i += 64) sum += few_keys(a, i).tiles;
-  const long total = read_lane(prefix_sum(sum), 63) * a.Hkv;
-  return max((total + a.few_blocks - 1) / a.few_blocks, 1l);
-}
+};
 // Where a workgroup's part of a head's keys is kept: it has at most two that others share, one that
 // it ends with and one that it goes on with.
-QMOE_DEV long part_of(long block, bool begins) { return 2 * block + (begins ? 1 : 0); }
+QMOE_DEV long part_of(int block, bool begins) { return 2l * block + (begins ? 1 : 0); }
 
-template <typename E, int NK>
+template <typename E, int NK, bool FULL>
 QMOE_DEV void few_rows(const AttentionArgs& a, int block, unsigned char* lds) {
   using L = Layout<NK>;
   __shared__ float m_of[4][32], l_of[4][32];
@@ -524,16 +594,14 @@ QMOE_DEV void few_rows(const AttentionArgs& a, int block, unsigned char* lds) {
       static_cast<u32x4_v*>(a.out)[i] = (u32x4_v){0, 0, 0, 0};
   }
 
-  // (all that locates the work is the same in every lane: kept in scalars)
-  const long share = share_of(a), stop = share * (block + 1);
-  long f = share * block;
-  Place place = locate(a, f);
-  while (f < stop && place.b < batch.B) {
-    const int b = place.b;
-    const FewKeys keys = few_keys(a, b);
-    const int h = __builtin_amdgcn_readfirstlane((int)((f - place.start) / keys.tiles));
-    const long head_start = place.start + (long)h * keys.tiles;
-    const int x0 = (int)(f - head_start), x1 = (int)min((long)keys.tiles, stop - head_start);
+  const FewList list(a);
+  const int stop = list.share * (block + 1);
+  int f = list.share * block, start;
+  FewKeys keys;
+  int b = list.locate(a, f, keys, start);
+  while (f < stop && b < batch.B) {
+    const int h = (f - start) / keys.tiles, head_start = start + h * keys.tiles;
+    const int x0 = f - head_start, x1 = min(keys.tiles, stop - head_start);
     f = head_start + x1;
     const int row0 = batch.first_row(b), rows = keys.n * G;
 
@@ -552,54 +620,65 @@ QMOE_DEV void few_rows(const AttentionArgs& a, int block, unsigned char* lds) {
     auto first_of = [&](int x) { return keys.begin + FEW_KEYS * x + 32 * wave; };
     auto entry_of = [&](int x) {
       const int key = first_of(x) + (lane & 31);
-      return key < keys.end ? table[batch.page.div(key)] : -1;
+      return x < x1 && key < keys.end ? table[batch.page.div(key)] : -1;
     };
     unsigned char* mine = lds + wave * 64 * L::STRIDE;  // two times 32 rows of V
-    // K's rows go straight to registers: lane & 31 is the row of the first operand
-    auto load = [&](int x, int entry, s16x8_v (&k)[2 * NK], unsigned char* to) {
-      const int key = first_of(x) + (lane & 31);
-      if (entry >= batch.n_pages) entry = -1;
-      const uint64_t present = __ballot(entry >= 0);
-      const bool whole = present == ~0ull;
-      const long ko = row_offset(a.kc, batch.page, entry, key), vo = row_offset(a.vc, batch.page, entry, key);
+    // K's rows go straight to registers (lane & 31 is the row of the first operand), V's to LDS
+    s16x8_v k[2 * NK];
+    auto load_k = [&](int x, int entry) {
+      // (a key without a page: the cache's first, left out by its score)
+      const unsigned char* row = kb + row_offset(a.kc, batch.page, entry, first_of(x) + (lane & 31));
+      if (FULL) {
 #pragma unroll
-      for (int ks = 0; ks < 2 * NK; ++ks) {
-        u32x4_v w = {0, 0, 0, 0};
-        if (entry >= 0 && 16 * ks + 8 * half < a.D) w = *reinterpret_cast<const u32x4_v*>(kb + ko + 32 * ks);
-        k[ks] = __builtin_bit_cast(s16x8_v, w);
+        for (int ks = 0; ks < 2 * NK; ++ks) k[ks] = *reinterpret_cast<const s16x8_v*>(row + 32 * ks);
+      } else {
+#pragma unroll
+        for (int ks = 0; ks < 2 * NK; ++ks) {
+          const bool in = 16 * ks + 8 * half < a.D;
+          u32x4_v w = *reinterpret_cast<const u32x4_v*>(in ? row + 32 * ks : row);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) w[i] = in ? w[i] : 0;
+          k[ks] = __builtin_bit_cast(s16x8_v, w);
+        }
       }
-      load_rows<NK, 32 / L::RPI, false>(to, vb, vo, present, whole, a.same_pages, 0, L::RPI,
-                                        (uint32_t)(2 * a.vc.slot), a.D);
-      return present;
     };
-    s16x8_v k[2 * NK], k_next[2 * NK];
-    uint64_t present_next = 0;
-    int entry = -1;
-    if (x0 < x1) {
-      present_next = load(x0, entry_of(x0), k_next, mine + (x0 & 1) * 32 * L::STRIDE);
-      if (x0 + 1 < x1) entry = entry_of(x0 + 1);
+    auto load_v = [&](int x, int entry, uint64_t present, unsigned char* to) {
+      const long vo = row_offset(a.vc, batch.page, entry, first_of(x) + (lane & 31));
+      load_rows<NK, FULL, 32 / L::RPI, L::RPI, false>(to, vb, vo, present, present == ~0ull, a.same_pages, 0, (uint32_t)(2 * a.vc.slot), a.D);
+    };
+    uint64_t present = 0;
+    int entry = entry_of(x0), entry_next = entry_of(x0 + 1);
+    auto known = [&](int e) { return e < batch.n_pages ? e : -1; };
+    entry = known(entry);
+    present = __ballot(entry >= 0);
+    const bool any = keys.end > keys.begin;  // (there is a page, then)
+    if (any) {
+      load_v(x0, entry, present, mine);
+      load_k(x0, entry);
     }
     auto step = [&](int x, const unsigned char* __restrict__ v, unsigned char* __restrict__ next) {
       asm volatile("" ::: "memory");
       wait_vm_lgkm0<0>();
       asm volatile("" ::: "memory");
-#pragma unroll
-      for (int ks = 0; ks < 2 * NK; ++ks) k[ks] = k_next[ks];
-      const uint64_t present = present_next;
-      if (x + 1 < x1) {
-        present_next = load(x + 1, entry, k_next, next);
-        if (x + 2 < x1) entry = entry_of(x + 2);
-      }
+      const uint64_t here = present;
+      entry = known(entry_next);
+      present = __ballot(entry >= 0);
+      if (x + 1 < x1) load_v(x + 1, entry, present, next);
+      entry_next = entry_of(x + 2);
       const int first = first_of(x);
       f32x16_v s[1];
 #pragma unroll
       for (int i = 0; i < 16; ++i) s[0][i] = 0.f;
 #pragma unroll
       for (int ks = 0; ks < 2 * NK; ++ks) s[0] = Mma<E>::mma(k[ks], q[ks], s[0]);
-      const bool whole = present == ~0ull && first + 31 <= keys.before && (!a.window || first > keys.before + keys.n - 1 - a.window);
-      acc.take(s, v, a.scale, whole, seen, present, first);
+      // The next keys take these registers (behind the last tile: the first row of the cache; a branch around
+      // the loads would cost a wait for them where it ends).
+      asm volatile("" ::: "memory");
+      load_k(x + 1, entry);
+      const bool whole = here == ~0ull && first + 31 <= keys.before && (!a.window || first > keys.before + keys.n - 1 - a.window);
+      acc.take(s, v, a.scale, whole, seen, here, first);
     };
-    for (int x = x0; x < x1; ++x) step(x, mine + (x & 1) * 32 * L::STRIDE, mine + (~x & 1) * 32 * L::STRIDE);
+    for (int x = x0; any && x < x1; ++x) step(x, mine + ((x - x0) & 1) * 32 * L::STRIDE, mine + ((x - x0 + 1) & 1) * 32 * L::STRIDE);
 
     // the four waves' sums: each brought to the common maximum, then added through LDS
     const float l = acc.l + other_half(acc.l);
@@ -639,90 +718,120 @@ QMOE_DEV void few_rows(const AttentionArgs& a, int block, unsigned char* lds) {
             make_uint2(Mma<E>::pack(sum[0] * inv, sum[1] * inv), Mma<E>::pack(sum[2] * inv, sum[3] * inv));
       } else {
         reinterpret_cast<f32x4_v*>(a.few_part + (part * a.few_rows + at) * a.D)[d] = sum;
-        if (d == 0)
-          reinterpret_cast<float2*>(a.few_part + 2l * a.few_blocks * a.few_rows * a.D)[part * a.few_rows + at] = make_float2(best, total);
+        if (d == 0) few_tops(a)[part * a.few_rows + at] = make_float2(best, total);
       }
     }
     __syncthreads();
-    if (f >= place.start + (long)keys.tiles * a.Hkv && f < stop) place = locate(a, f);
+    if (f >= start + keys.tiles * a.Hkv && f < stop) b = list.locate(a, f, keys, start);
   }
 }
 
-template <typename E, int NK>
-__global__ __launch_bounds__(256, (NK <= 4 ? 2 : 1)) void attention_kernel(AttentionArgs a) {
+template <typename E, int NK, bool FULL>
+__global__ __launch_bounds__(256, (NK <= 4 ? 2 : 1)) void attention_many_kernel(AttentionArgs a) {
   __shared__ __align__(16) unsigned char lds[Layout<NK>::LDS];
-  if ((int)blockIdx.x < a.few_blocks) few_rows<E, NK>(a, blockIdx.x, lds);
-  else many_rows<E, NK>(a, blockIdx.x - a.few_blocks, lds);
+  many_rows<E, NK, FULL>(a, blockIdx.x, lds);
+}
+template <typename E, int NK, bool FULL>
+__global__ __launch_bounds__(256, (NK <= 4 ? 2 : 1)) void attention_few_kernel(AttentionArgs a) {
+  __shared__ __align__(16) unsigned char lds[Layout<NK>::LDS];
+  few_rows<E, NK, FULL>(a, blockIdx.x, lds);
 }
 
 // ---------------------------------------------------------------- joining
 
-// One row's parts: sums of D and (maximum, sum), `count` of them; a workgroup per row, its waves take every
-// fourth part, then their sums are joined through LDS.
+// One row's parts: sums of D and (maximum, sum), `count` of them at at(c). The parts' scales first, then as
+// many parts at once as the threads make rows of D, eight of them in flight each.
+constexpr int JOIN_ROWS = 8;  // workgroups that share out the rows of a tile
+constexpr int PARTS_MAX = 520;
 template <typename E, typename At>
 QMOE_DEV void join_row(const float* sums, const float2* tops, At at, int count, uint16_t* out, int D) {
-  __shared__ float part[4][D_MAX], m_of[4], l_of[4];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  __shared__ float scale[PARTS_MAX], sum_of[4];
+  __shared__ __align__(16) f32x4_v part[256];
+  const int tid = threadIdx.x;
+  float2 t[3];
   float m = -INFINITY, l = 0.f;
-  f32x4_v o = {0.f, 0.f, 0.f, 0.f};
-  const bool mine = 4 * lane < D;
-  for (int c = wave; c < count; c += 4) {
-    const long p = at(c);
-    const float2 t = tops[p];
-    if (t.y == 0.f) continue;
-    f32x4_v x = {0.f, 0.f, 0.f, 0.f};
-    if (mine) x = *reinterpret_cast<const f32x4_v*>(sums + p * D + 4 * lane);
-    const float top = fmaxf(m, t.x), f = m == top ? 1.f : __builtin_amdgcn_exp2f(m - top);
-    const float g = t.x == top ? 1.f : __builtin_amdgcn_exp2f(t.x - top);
-    m = top, l = l * f + t.y * g;
-    o = o * f + x * g;
+#pragma unroll
+  for (int i = 0; i < 3; ++i) {
+    t[i] = make_float2(-INFINITY, 0.f);
+    if (tid + 256 * i < count) t[i] = tops[at(tid + 256 * i)];
+    m = fmaxf(m, t[i].x);
   }
-  if (mine) *reinterpret_cast<f32x4_v*>(&part[wave][4 * lane]) = o;
-  if (lane == 0) m_of[wave] = m, l_of[wave] = l;
+#pragma unroll
+  for (int o = 32; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+  if ((tid & 63) == 0) sum_of[tid >> 6] = m;
   __syncthreads();
-  float top = m_of[0], total = 0.f, sum = 0.f;
+  m = fmaxf(fmaxf(sum_of[0], sum_of[1]), fmaxf(sum_of[2], sum_of[3]));
 #pragma unroll
-  for (int w = 1; w < 4; ++w) top = fmaxf(top, m_of[w]);
-  const int d = threadIdx.x;
+  for (int i = 0; i < 3; ++i)
+    if (tid + 256 * i < count) {
+      const float f = t[i].y == 0.f ? 0.f : t[i].x == m ? 1.f : __builtin_amdgcn_exp2f(t[i].x - m);
+      scale[tid + 256 * i] = f;
+      l += t[i].y == 0.f ? 0.f : t[i].y * f;
+    }
+  l = wave_sum_f32(l);
+  __syncthreads();
+  if ((tid & 63) == 0) sum_of[tid >> 6] = l;
+  const int quads = D / 4, streams = 256 / quads, stream = tid / quads, quad = tid - stream * quads;
+  f32x4_v o = {0.f, 0.f, 0.f, 0.f};
+  if (stream < streams)
+    for (int c = stream; c < count; c += 8 * streams) {
+      f32x4_v x[8];
 #pragma unroll
-  for (int w = 0; w < 4; ++w) {
-    const float f = m_of[w] == top ? 1.f : __builtin_amdgcn_exp2f(m_of[w] - top);
-    total += l_of[w] * f;
-    if (d < D) sum += part[w][d] * f;
+      for (int i = 0; i < 8; ++i) x[i] = reinterpret_cast<const f32x4_v*>(sums + at(min(c + i * streams, count - 1)) * D)[quad];
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (c + i * streams < count) o += x[i] * scale[c + i * streams];
+    }
+  part[tid] = o;
+  __syncthreads();
+  l = (sum_of[0] + sum_of[1]) + (sum_of[2] + sum_of[3]);
+  if (tid < quads) {
+    for (int c = 1; c < streams; ++c) o += part[c * quads + tid];
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    reinterpret_cast<uint2*>(out)[tid] = make_uint2(Mma<E>::pack(o[0] * inv, o[1] * inv), Mma<E>::pack(o[2] * inv, o[3] * inv));
   }
-  if (d < D) out[d] = E::store(total == 0.f ? 0.f : sum / total);
+  __syncthreads();
 }
 
-// Blocks [0, few_blocks) x few_rows: the head whose tiles the first boundary inside lies between shares
-// block - 1 and block, one row each. Behind them one for every row, where the many-rows form cut keys
-// into pieces.
+// Blocks [0, few_blocks) x join_rows: the head inside whose tiles the first boundary is the one between the
+// shares of block - 1 and block, every join_rows-th row. Behind them, where the many-rows form cuts
+// keys into pieces, so many for each tile and head.
 template <typename E>
-__global__ __launch_bounds__(256) void join_kernel(AttentionArgs a) {
+__global__ __launch_bounds__(256) void join_kernel(AttentionArgs a, int join_rows) {
   const Batch& batch = a.batch;
-  const int few = a.few_blocks * a.few_rows, G = a.group.d;
+  const int few = a.few_blocks * join_rows, G = a.group.d;
   if ((int)blockIdx.x < few) {
-    const int block = blockIdx.x / a.few_rows, at = blockIdx.x - block * a.few_rows;
+    const int block = blockIdx.x / join_rows;
     if (block == 0) return;
-    const long share = share_of(a), f = share * block;
-    const Place place = locate(a, f);
-    if (place.b >= batch.B) return;
-    const FewKeys keys = few_keys(a, place.b);
-    const int h = (int)((f - place.start) / keys.tiles);
-    const long start = place.start + (long)h * keys.tiles;
-    if (start == f || start < f - share || at >= keys.n * G) return;
-    const long last = (start + keys.tiles - 1) / share;
-    const int token = a.group.div(at);
-    const long row = (long)(batch.first_row(place.b) + token) * a.Hq + h * G + at - token * G;
-    join_row<E>(a.few_part, reinterpret_cast<const float2*>(a.few_part + 2l * a.few_blocks * a.few_rows * a.D),
-                [&](int c) { return part_of(block - 1 + c, c == 0) * a.few_rows + at; }, (int)(last - block + 2),
-                static_cast<uint16_t*>(a.out) + row * a.D, a.D);
+    const FewList list(a);
+    const int f = list.share * block;
+    FewKeys keys;
+    int start;
+    const int b = list.locate(a, f, keys, start);
+    if (b >= batch.B) return;
+    const int h = (f - start) / keys.tiles;
+    start += h * keys.tiles;
+    if (start == f || start < f - list.share) return;
+    const int last = (start + keys.tiles - 1) / list.share, row0 = batch.first_row(b);
+    for (int r = blockIdx.x - block * join_rows; r < keys.n * G; r += join_rows) {
+      const int token = a.group.div(r);
+      const long row = (long)(row0 + token) * a.Hq + h * G + r - token * G;
+      join_row<E>(a.few_part, few_tops(a), [&](int c) { return part_of(block - 1 + c, c == 0) * a.few_rows + r; },
+                  last - block + 2, static_cast<uint16_t*>(a.out) + row * a.D, a.D);
+    }
   } else {
-    const int row = blockIdx.x - few, t = row / a.Hq;
-    const int b = batch.sequence(t);
-    if (b < batch.B && batch.new_rows(b) * G <= a.few) return;
-    const long all = (long)batch.T * a.Hq;
-    join_row<E>(a.many_part, reinterpret_cast<const float2*>(a.many_part + a.pieces * all * a.D),
-                [&](int c) { return c * all + row; }, a.pieces, static_cast<uint16_t*>(a.out) + (long)row * a.D, a.D);
+    const int block = blockIdx.x - few, rest = block / JOIN_ROWS, number = a.heads.div(rest), h = rest - number * a.Hkv;
+    const ManyTile t = many_tile(a, number);
+    if (t.r0 < 0 || t.tiles <= 8) return;
+    const Pieces pieces = pieces_of(a, t, h);
+    const int count = min((t.tiles + pieces.size - 1) / pieces.size, a.pieces);
+    if (count <= 1) return;
+    for (int r = block - rest * JOIN_ROWS; r < min(ROWS, t.rows - t.r0); r += JOIN_ROWS) {
+      const int token = a.group.div(t.r0 + r);
+      const long row = (long)(t.row0 + token) * a.Hq + h * G + t.r0 + r - token * G;
+      join_row<E>(a.many_part, many_tops(a), [&](int c) { return piece_at(pieces, c) * ROWS + r; }, count,
+                  static_cast<uint16_t*>(a.out) + row * a.D, a.D);
+    }
   }
 }
 
@@ -730,9 +839,10 @@ __global__ __launch_bounds__(256) void join_kernel(AttentionArgs a) {
 
 // How a call is cut, from what the host knows of it.
 struct Plan {
-  int few, few_blocks, few_rows, many_tiles, pieces;
+  int few, few_blocks, few_rows, many_tiles, pieces, slots;
   size_t few_floats, many_floats;
 };
+constexpr int PIECES_MAX = 64;
 Plan plan_for(int T, int B, int Hq, int Hkv, int D, int page, int width, bool one_each) {
   const int G = Hq / Hkv;
   Plan p = {};
@@ -741,41 +851,54 @@ Plan plan_for(int T, int B, int Hq, int Hkv, int D, int page, int width, bool on
   p.few = few ? FEW : 0;
   p.few_rows = one_each ? G : FEW;
   p.pieces = 1;
-  const int slots = D > 128 ? 256 : 512;  // workgroups that run at once
-  const long most = (long)width * page;   // keys
+  p.slots = D > 128 ? 256 : 512;  // workgroups that run at once
+  const long most = std::min((long)width * page, 0x7fffffffl);  // keys
   if (few) {
     const long tiles = (long)B * Hkv * std::max<long>(1, (most + FEW_KEYS - 1) / FEW_KEYS);
-    p.few_blocks = (int)std::min<long>(slots, tiles);
+    p.few_blocks = (int)std::max(1l, std::min<long>(p.slots, tiles));
     p.few_floats = 2l * p.few_blocks * p.few_rows * (D + 2);
   }
   if (many) {
     p.many_tiles = (int)((long)T * G / ROWS) + B + 1;
-    const long items = (((long)T * G + ROWS - 1) / ROWS) * Hkv;
-    p.pieces = (int)std::max<long>(1, std::min({16l, slots / items, (most + 255) / 256}));
-    if (p.pieces > 1) p.many_floats = (size_t)p.pieces * T * Hq * (D + 2);
+    const long items = (((long)T * G + ROWS - 1) / ROWS) * Hkv, units = (most + 63) / 64;
+    if (items < 4 * p.slots && ((long)p.many_tiles * Hkv + p.slots) * (units + 8) < 1l << 31)
+      p.pieces = (int)std::max<long>(1, std::min({units / 8, (long)PIECES_MAX, std::max(8l, 16l * p.slots / items)}));
+    if (p.pieces > 1) p.many_floats = 2l * (p.slots + 1) * ROWS * (D + 2);
   }
   return p;
 }
 
-template <typename E, int NK>
+template <typename E, int NK, bool FULL>
 int launch(const AttentionArgs& a, hipStream_t st) {
-  const long blocks = a.few_blocks + (long)a.many_tiles * a.Hkv * a.pieces;
-  if (blocks > 0x7fffffffl) return QMOE_EINVAL;
-  hipLaunchKernelGGL((attention_kernel<E, NK>), dim3((unsigned)blocks), dim3(256), 0, st, a);
-  const int rc = (int)hipGetLastError();
-  const long joins = (long)a.few_blocks * a.few_rows + (a.pieces > 1 ? (long)a.batch.T * a.Hq : 0);
-  if (rc || joins == 0) return rc;
-  hipLaunchKernelGGL((join_kernel<E>), dim3((unsigned)joins), dim3(256), 0, st, a);
+  const long tiles = (long)a.many_tiles * a.Hkv, blocks = tiles * a.pieces;
+  if (blocks > 0x7fffffffl || tiles * JOIN_ROWS > 0x7ffffffl) return QMOE_EINVAL;
+  if (a.few_blocks) {
+    hipLaunchKernelGGL((attention_few_kernel<E, NK, FULL>), dim3(a.few_blocks), dim3(256), 0, st, a);
+    if (const int rc = (int)hipGetLastError()) return rc;
+  }
+  if (blocks) {
+    hipLaunchKernelGGL((attention_many_kernel<E, NK, FULL>), dim3((unsigned)blocks), dim3(256), 0, st, a);
+    if (const int rc = (int)hipGetLastError()) return rc;
+  }
+  const int join_rows = std::min(a.few_rows, JOIN_ROWS);
+  const long joins = (long)a.few_blocks * join_rows + (a.pieces > 1 ? tiles * JOIN_ROWS : 0);
+  if (joins == 0) return QMOE_OK;
+  hipLaunchKernelGGL((join_kernel<E>), dim3((unsigned)joins), dim3(256), 0, st, a, join_rows);
   return (int)hipGetLastError();
+}
+
+template <typename E, int NK>
+int launch_heads(const AttentionArgs& a, hipStream_t st) {
+  return a.D == 32 * NK ? launch<E, NK, true>(a, st) : launch<E, NK, false>(a, st);
 }
 
 template <typename E>
 int dispatch(const AttentionArgs& a, hipStream_t st) {
-  if (a.D <= 64) return launch<E, 2>(a, st);
-  if (a.D <= 96) return launch<E, 3>(a, st);
-  if (a.D <= 128) return launch<E, 4>(a, st);
-  if (a.D <= 192) return launch<E, 6>(a, st);
-  return launch<E, 8>(a, st);
+  if (a.D <= 64) return launch_heads<E, 2>(a, st);
+  if (a.D <= 96) return launch_heads<E, 3>(a, st);
+  if (a.D <= 128) return launch_heads<E, 4>(a, st);
+  if (a.D <= 192) return launch_heads<E, 6>(a, st);
+  return launch_heads<E, 8>(a, st);
 }
 
 bool bad_shape(int T, int B, int Hq, int Hkv, int D) {
@@ -807,6 +930,10 @@ int qmoe_paged_attention(const void* q, long q_token, long q_head, const void* k
   if ((reinterpret_cast<uintptr_t>(k_cache) | reinterpret_cast<uintptr_t>(v_cache)) & 15) return QMOE_EINVAL;
   if (T == 0) return QMOE_OK;
   if (!q || !out || missing(k_cache, v_cache, n_pages, table, table_width, lengths, B)) return QMOE_EINVAL;
+  // bytes within a page, from page to page, and the list of the few-rows form are counted in 32 bits
+  for (const long step : {k_page, v_page, k_slot * page, v_slot * page, k_head, v_head})
+    if (step < 0 || step >= 1l << 30) return QMOE_EINVAL;
+  if ((long)B * Hkv * (std::min((long)table_width * page, 0x7fffffffl) / FEW_KEYS + 1) > 0x7fffff00l) return QMOE_EINVAL;
   const Plan p = plan_for(T, B, Hq, Hkv, D, page, table_width, !starts);
   if (p.few_floats + p.many_floats &&
       (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15) || workspace_bytes < 4 * (p.few_floats + p.many_floats)))
@@ -821,8 +948,9 @@ int qmoe_paged_attention(const void* q, long q_token, long q_head, const void* k
   a.Hq = Hq, a.Hkv = Hkv, a.D = D, a.window = window;
   a.group = FastDiv(Hq / Hkv), a.heads = FastDiv(Hkv), a.piece_div = FastDiv(p.pieces);
   a.scale = std::max(std::fabs(scale) * LOG2E, FLT_MIN), a.negate = scale < 0;
-  a.same_pages = page % 8 == 0 && std::max(k_slot, v_slot) < 1 << 26;
-  a.few = p.few, a.few_blocks = p.few_blocks, a.few_rows = p.few_rows, a.many_tiles = p.many_tiles, a.pieces = p.pieces;
+  a.same_pages = page % 16 == 0;
+  a.few = p.few, a.few_blocks = p.few_blocks, a.few_rows = p.few_rows, a.many_tiles = p.many_tiles;
+  a.pieces = p.pieces, a.slots = p.slots;
   a.few_part = static_cast<float*>(workspace);
   a.many_part = a.few_part + p.few_floats;
   return type == QMOE_BF16 ? dispatch<ElemBF16>(a, (hipStream_t)stream) : dispatch<ElemF16>(a, (hipStream_t)stream);

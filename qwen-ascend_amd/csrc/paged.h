@@ -43,7 +43,7 @@ struct Batch {
   QMOE_DEV int new_rows(int b) const { return starts ? max(start(b + 1) - start(b), 0) : 1; }
   // Cached tokens of sequence b, as many as its row of the table can hold.
   QMOE_DEV int length(int b) const {
-    const long most = min((long)width * page.d, 0x7fffffffl);
+    const long most = n_pages ? min((long)width * page.d, 0x7fffffffl) : 0;
     return (int)min(max((long)lengths[b], 0l), most);
   }
   // The page of position p in [0, length(b)), or -1 where the table names none of the cache's.
