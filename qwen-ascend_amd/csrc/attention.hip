@@ -199,53 +199,10 @@ struct Rows {
       }
   }
 
-  // Whether a value of V's rows in LDS is infinite or NaN.
-  QMOE_DEV static bool unusual(const unsigned char* v) {
-    const int lane = threadIdx.x & 63;
-    uint32_t any = 0;
-#pragma unroll 4
-    for (int i = lane; i < 32 * NJ * L::PIECES; i += 64) {
-      const u32x4_v w = *reinterpret_cast<const u32x4_v*>(v + 16 * i);
-#pragma unroll
-      for (int q = 0; q < 4; ++q) any |= (w[q] & Mma<E>::EXPONENT) + Mma<E>::ONE;
-    }
-    return __any((any & 0x80008000u) != 0);
-  }
-
-  // The same sum key by key: a weight of 0 times a value that is infinite or NaN would be NaN, so values that
-  // a row does not see are taken out. Rare (an unusual value beside a tile's border), so short code.
-  QMOE_DEV void add_careful(const unsigned char* v, const f32x16_v (&s)[NJ], Seen seen, uint64_t present, int first) {
-    const int half = (threadIdx.x >> 5) & 1;
-#pragma unroll 1
-    for (int i = 0; i < 32 * NJ; ++i) {
-      const int of = i / 2;  // register of the key, in lanes of half i & 1
-      float w = 0.f;
-#pragma unroll
-      for (int j = 0; j < NJ; ++j)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) w = of == 16 * j + r ? s[j][r] : w;
-      const float other = other_half(w);
-      w = (i & 1) == half ? w : other;
-      const int key = key_of(of >> 4, of & 15) + 4 * (i & 1), swizzle = L::v_swizzle(key);
-      const bool sees_it = ((present >> key) & 1) && first + key >= seen.low && first + key <= seen.high;
-      const unsigned char* row = v + key * L::STRIDE + 8 * half;
-#pragma unroll
-      for (int dt = 0; dt < NK; ++dt)
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const s16x4_v x = *reinterpret_cast<const s16x4_v*>(row + 16 * ((4 * dt + c) ^ swizzle));
-#pragma unroll
-          for (int e = 0; e < 4; ++e) o[dt][4 * c + e] += w * (sees_it ? E::load((uint16_t)x[e]) : 0.f);
-        }
-    }
-  }
-
   // One tile: scores s, whose keys start at `first`; `whole`: every row sees all of them.
   QMOE_DEV void take(f32x16_v (&s)[NJ], const unsigned char* v, float scale, bool whole, Seen seen, uint64_t present, int first) {
-    const int half = (threadIdx.x >> 5) & 1;
-    int careful = 0;
     if (!whole) {
-      const int from = first + 4 * half, low = seen.low - from, high = seen.high - from;
+      const int half = (threadIdx.x >> 5) & 1, from = first + 4 * half, low = seen.low - from, high = seen.high - from;
 #pragma unroll
       for (int j = 0; j < NJ; ++j) {
         const uint32_t there = (uint32_t)(present >> (32 * j)) >> (4 * half);
@@ -255,28 +212,63 @@ struct Rows {
           if (!((there >> (key & 31)) & 1) || key < low || key > high) s[j][r] = -INFINITY;
         }
       }
-      careful = __builtin_amdgcn_readfirstlane(unusual(v));
     }
     s16x8_v p[2 * NJ];
     weigh(s, scale, p);
-    if (careful) add_careful(v, s, seen, present, first);
-    else add(v, p);
+    add(v, p);
+  }
+
+  // The infinite and NaN values of one key, which were left out of its tile: o += v where the row sees it.
+  // v: its value row.
+  QMOE_DEV void add_unusual(const unsigned char* v, bool sees, int D) {
+    const int half = (threadIdx.x >> 5) & 1;
+#pragma unroll
+    for (int dt = 0; dt < NK; ++dt)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const s16x4_v x = *reinterpret_cast<const s16x4_v*>(v + 2 * min(32 * dt + 8 * c + 4 * half, D - 4));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float f = E::load((uint16_t)x[e]);
+          if (sees && !(f - f == 0.f)) o[dt][4 * c + e] += f;
+        }
+      }
   }
 };
 
-// Rows of q as the second operand of K Q^T: elements 16 ks + 8 half of row lane & 31.
-template <int NK>
-QMOE_DEV void load_q(s16x8_v (&q)[2 * NK], const uint16_t* row, int D, bool valid, int negate) {
-  const int half = (threadIdx.x >> 5) & 1;
+// Values of V that some rows of a tile see and others do not: a weight of 0 times an infinity or NaN would
+// be NaN. So in tiles that not every row sees whole, such values become 0 (COUNT KB at v + `every` KB each,
+// as this wave loaded them); the rows that see them get them after the loop. Returns whether there were any.
+template <typename E, int COUNT>
+QMOE_DEV bool clean(unsigned char* v, int every) {
+  const int lane = threadIdx.x & 63;
+  bool any = false;
+#pragma unroll 1
+  for (int g = 0; g < COUNT; ++g) {
+    u32x4_v* at = reinterpret_cast<u32x4_v*>(v + g * every * 1024) + lane;
+    u32x4_v w = *at;
+    uint32_t odd = 0;
 #pragma unroll
-  for (int ks = 0; ks < 2 * NK; ++ks) {
-    u32x4_v w = {0, 0, 0, 0};
-    if (valid && 16 * ks + 8 * half < D) {
-      w = *reinterpret_cast<const u32x4_any*>(row + 16 * ks + 8 * half);
-      if (negate) w ^= 0x80008000u;
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t u = ((w[i] & Mma<E>::EXPONENT) + Mma<E>::ONE) & 0x80008000u;
+      odd |= u;
+      if (u & 0x8000u) w[i] &= 0xffff0000u;
+      if (u & 0x80000000u) w[i] &= 0xffffu;
     }
-    q[ks] = __builtin_bit_cast(s16x8_v, w);
+    if (odd) *at = w;
+    any |= odd != 0;
   }
+  return __any(any);
+}
+
+// Elements at, at + 1, .. at + 7 of a row of q.
+QMOE_DEV s16x8_v q_piece(const uint16_t* row, int at, int D, bool valid, int negate) {
+  u32x4_v w = {0, 0, 0, 0};
+  if (valid && at < D) {
+    w = *reinterpret_cast<const u32x4_any*>(row + at);
+    if (negate) w ^= 0x80008000u;
+  }
+  return __builtin_bit_cast(s16x8_v, w);
 }
 
 // Positions of a sequence's rows, as ints: what precedes its first new token, clamped.
@@ -429,8 +421,10 @@ QMOE_DEV void many_rows(const AttentionArgs& a, int block, unsigned char* lds) {
   const int wave_first = before + (int)a.group.div(r0 + 32 * wave);
   const int wave_last = live ? before + (int)a.group.div(min(r0 + 32 * wave + 32, rows) - 1) : -1;
 
-  s16x8_v q[2 * NK];
-  load_q<NK>(q, static_cast<const uint16_t*>(a.q) + (row0 + token) * a.q_token + (h * G + of) * a.q_head, a.D, valid, a.negate);
+  s16x8_v q[2 * NK];  // the second operand of K Q^T: elements 16 ks + 8 half of row lane & 31
+  const uint16_t* q_row = static_cast<const uint16_t*>(a.q) + (row0 + token) * a.q_token + (h * G + of) * a.q_head;
+#pragma unroll
+  for (int ks = 0; ks < 2 * NK; ++ks) q[ks] = q_piece(q_row, 16 * ks + 8 * half, a.D, valid, a.negate);
   Rows<E, NK, 2> acc;
   acc.clear();
 
@@ -460,6 +454,9 @@ QMOE_DEV void many_rows(const AttentionArgs& a, int block, unsigned char* lds) {
     for (int i = threadIdx.x; i < L::LDS / 16; i += 256) reinterpret_cast<u32x4_v*>(lds)[i] = (u32x4_v){0, 0, 0, 0};
     __syncthreads();
   }
+  __shared__ int unusual;
+  if (threadIdx.x == 0) unusual = 0;  // (before the first barrier of the loop, after which it may be set)
+  __syncthreads();
   uint64_t present_next = 0;
   int entry = -1;
   if (t0 < t1) {
@@ -469,10 +466,20 @@ QMOE_DEV void many_rows(const AttentionArgs& a, int block, unsigned char* lds) {
   const int k_row = lane & 31, k_base = k_row * L::STRIDE, k_swizzle = L::k_swizzle(k_row);
   // One tile from LDS at `k`, while the next is loaded to `next`. (As a function of two pointers that
   // share nothing, which spares a wait for the load before every transposing read.)
-  auto step = [&](int tile, const unsigned char* __restrict__ k, unsigned char* __restrict__ next) {
+  const int last_pos = before + (int)a.group.div(min(r0 + ROWS, rows) - 1), first_pos = before + (int)a.group.div(r0);
+  auto partial = [&](int tile, uint64_t present) {  // not seen whole by every row of the workgroup
+    const int first = begin + 64 * tile;
+    return present != ~0ull || first + 63 > first_pos || (a.window && first <= last_pos - a.window);
+  };
+  auto step = [&](int tile, unsigned char* __restrict__ now, unsigned char* __restrict__ next) {
     // the tile has landed, and every wave is past the one before it, whose half of LDS takes the next
     asm volatile("" ::: "memory");
     wait_vm_lgkm0<0>();
+    if (partial(tile, present_next) && clean<E, GROUPS>(now + L::TILE + 1024 * wave, 4)) {
+      unusual = 1;
+      asm volatile("" ::: "memory");
+      wait_vm_lgkm0<0>();
+    }
     barrier_no_fence();
     const uint64_t present = present_next;
     if (tile + 1 < t1) {
@@ -490,13 +497,29 @@ QMOE_DEV void many_rows(const AttentionArgs& a, int block, unsigned char* lds) {
     for (int ks = 0; ks < 2 * NK; ++ks)
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        const s16x8_v f = *reinterpret_cast<const s16x8_v*>(k + k_base + 32 * j * L::STRIDE + 16 * ((2 * ks + half) ^ k_swizzle));
+        const s16x8_v f = *reinterpret_cast<const s16x8_v*>(now + k_base + 32 * j * L::STRIDE + 16 * ((2 * ks + half) ^ k_swizzle));
         s[j] = Mma<E>::mma(f, q[ks], s[j]);
       }
     const bool whole = present == ~0ull && first + 63 <= wave_first && (!a.window || first > wave_last - a.window);
-    acc.take(s, k + L::TILE, a.scale, whole, seen, present, first);
+    acc.take(s, now + L::TILE, a.scale, whole, seen, present, first);
   };
   for (int tile = t0; tile < t1; ++tile) step(tile, lds + (tile & 1) * 2 * L::TILE, lds + (~tile & 1) * 2 * L::TILE);
+  __syncthreads();
+  if (unusual) {
+    for (int tile = t0; tile < t1; ++tile) {
+      int e = entry_of(tile);
+      if (e >= batch.n_pages) e = -1;
+      const uint64_t present = __ballot(e >= 0);
+      if (!partial(tile, present)) continue;
+      const long vo = row_offset(a.vc, batch.page, e, begin + 64 * tile + lane);
+#pragma unroll 1
+      for (int i = 0; i < 64; ++i) {
+        const int key = begin + 64 * tile + i;
+        const bool sees = ((present >> i) & 1) && key >= seen.low && key <= seen.high;
+        acc.add_unusual(vb + ((present >> i) & 1 ? read_lane(vo, i) : 0), sees, FULL ? L::DC : a.D);
+      }
+    }
+  }
 
   const float l = acc.l + other_half(acc.l);
   if (!valid) return;
@@ -543,31 +566,35 @@ QMOE_DEV FewKeys few_keys(const AttentionArgs& a, int b) {
   return s;
 }
 
-// The list of tiles: sequence, then head, then tile. Every workgroup takes `share` of them.
+// The list of tiles: sequence, then head, then tile, with LEAD places before each head's tiles that stand for
+// what a head costs beside them (its first loads and its sums through LDS, about as long as two tiles).
+// Every workgroup takes `share` places.
+constexpr int LEAD = 2;
 struct FewList {
   FewKeys mine;  // of sequence `lane`
   int share;
+  QMOE_DEV static int places(const FewKeys& k) { return k.tiles ? k.tiles + LEAD : 0; }
   QMOE_DEV FewList(const AttentionArgs& a) {
     const int lane = threadIdx.x & 63;
     mine = FewKeys{};
     if (lane < a.batch.B) mine = few_keys(a, lane);
-    int sum = mine.tiles;
-    for (int i = 64 + lane; i < a.batch.B; i += 64) sum += few_keys(a, i).tiles;
+    int sum = places(mine);
+    for (int i = 64 + lane; i < a.batch.B; i += 64) sum += places(few_keys(a, i));
     const int total = lane_of(prefix_sum(sum), 63) * a.Hkv;
     share = max((total + a.few_blocks - 1) / a.few_blocks, 1);
   }
-  // The sequence (B behind the end) that tile f of the list belongs to, its keys and its first tile.
+  // The sequence (B behind the end) that place f of the list belongs to, its keys and its first place.
   QMOE_DEV int locate(const AttentionArgs& a, int f, FewKeys& keys, int& start) const {
     const int lane = threadIdx.x & 63;
     start = 0;
     for (int i = 0; i < a.batch.B; i += 64) {
       FewKeys k = mine;
       if (i) k = i + lane < a.batch.B ? few_keys(a, i + lane) : FewKeys{};
-      const int tiles = k.tiles * a.Hkv, upto = start + prefix_sum(tiles);
+      const int mine_all = places(k) * a.Hkv, upto = start + prefix_sum(mine_all);
       const uint64_t past = __ballot(upto > f);
       if (past) {
         const int at = __ffsll((unsigned long long)past) - 1;
-        start = lane_of(upto - tiles, at);
+        start = lane_of(upto - mine_all, at);
         keys = {lane_of(k.n, at), lane_of(k.before, at), lane_of(k.begin, at), lane_of(k.end, at), lane_of(k.tiles, at)};
         return i + at;
       }
@@ -584,6 +611,7 @@ template <typename E, int NK, bool FULL>
 QMOE_DEV void few_rows(const AttentionArgs& a, int block, unsigned char* lds) {
   using L = Layout<NK>;
   __shared__ float m_of[4][32], l_of[4][32];
+  __shared__ s16x8_v q_lds[NK > 4 ? 2 * NK * 64 : 1];
   const int lane = threadIdx.x & 63, half = lane >> 5, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const Batch& batch = a.batch;
   const int G = a.group.d;
@@ -600,17 +628,27 @@ QMOE_DEV void few_rows(const AttentionArgs& a, int block, unsigned char* lds) {
   FewKeys keys;
   int b = list.locate(a, f, keys, start);
   while (f < stop && b < batch.B) {
-    const int h = (f - start) / keys.tiles, head_start = start + h * keys.tiles;
-    const int x0 = f - head_start, x1 = min(keys.tiles, stop - head_start);
-    f = head_start + x1;
+    const int each = FewList::places(keys), h = (f - start) / each, tiles_start = start + h * each + LEAD;
+    const int x0 = max(f - tiles_start, 0), x1 = min(keys.tiles, stop - tiles_start);
+    f = tiles_start + max(x1, 0);
+    if (x1 <= 0) break;  // its places before the tiles only
     const int row0 = batch.first_row(b), rows = keys.n * G;
 
     const int r = lane & 31, token = a.group.div(r), of = r - token * G;
     const bool valid = r < rows;
     const int pos = keys.before + token;
     const Seen seen = {a.window ? pos - a.window + 1 : 0, valid ? pos : -1};
-    s16x8_v q[2 * NK];
-    load_q<NK>(q, static_cast<const uint16_t*>(a.q) + (row0 + token) * a.q_token + (h * G + of) * a.q_head, a.D, valid, a.negate);
+    // q in registers, or, where the sums of wide heads need these, in LDS
+    s16x8_v q[NK > 4 ? 1 : 2 * NK];
+    const uint16_t* q_row = static_cast<const uint16_t*>(a.q) + (row0 + token) * a.q_token + (h * G + of) * a.q_head;
+    if constexpr (NK > 4) {
+#pragma unroll
+      for (int ks = wave; ks < 2 * NK; ks += 4) q_lds[ks * 64 + lane] = q_piece(q_row, 16 * ks + 8 * half, a.D, valid, a.negate);
+      __syncthreads();
+    } else {
+#pragma unroll
+      for (int ks = 0; ks < 2 * NK; ++ks) q[ks] = q_piece(q_row, 16 * ks + 8 * half, a.D, valid, a.negate);
+    }
     Rows<E, NK, 1> acc;
     acc.clear();
 
@@ -656,11 +694,17 @@ QMOE_DEV void few_rows(const AttentionArgs& a, int block, unsigned char* lds) {
       load_v(x0, entry, present, mine);
       load_k(x0, entry);
     }
-    auto step = [&](int x, const unsigned char* __restrict__ v, unsigned char* __restrict__ next) {
+    bool unusual = false;
+    auto whole = [&](int x, uint64_t there) {  // seen by every row
+      const int first = first_of(x);
+      return there == ~0ull && first + 31 <= keys.before && (!a.window || first > keys.before + keys.n - 1 - a.window);
+    };
+    auto step = [&](int x, unsigned char* __restrict__ v, unsigned char* __restrict__ next) {
       asm volatile("" ::: "memory");
       wait_vm_lgkm0<0>();
       asm volatile("" ::: "memory");
       const uint64_t here = present;
+      if (!whole(x, here) && clean<E, 32 / L::RPI>(v, 1)) unusual = true;
       entry = known(entry_next);
       present = __ballot(entry >= 0);
       if (x + 1 < x1) load_v(x + 1, entry, present, next);
@@ -670,15 +714,31 @@ QMOE_DEV void few_rows(const AttentionArgs& a, int block, unsigned char* lds) {
 #pragma unroll
       for (int i = 0; i < 16; ++i) s[0][i] = 0.f;
 #pragma unroll
-      for (int ks = 0; ks < 2 * NK; ++ks) s[0] = Mma<E>::mma(k[ks], q[ks], s[0]);
+      for (int ks = 0; ks < 2 * NK; ++ks) {
+        if constexpr (NK > 4) s[0] = Mma<E>::mma(k[ks], q_lds[ks * 64 + lane], s[0]);
+        else s[0] = Mma<E>::mma(k[ks], q[ks], s[0]);
+      }
       // The next keys take these registers (behind the last tile: the first row of the cache; a branch around
       // the loads would cost a wait for them where it ends).
       asm volatile("" ::: "memory");
       load_k(x + 1, entry);
-      const bool whole = here == ~0ull && first + 31 <= keys.before && (!a.window || first > keys.before + keys.n - 1 - a.window);
-      acc.take(s, v, a.scale, whole, seen, here, first);
+      acc.take(s, v, a.scale, whole(x, here), seen, here, first);
     };
     for (int x = x0; any && x < x1; ++x) step(x, mine + ((x - x0) & 1) * 32 * L::STRIDE, mine + ((x - x0 + 1) & 1) * 32 * L::STRIDE);
+    if (unusual) {
+      for (int x = x0; x < x1; ++x) {
+        const int e = known(entry_of(x));
+        const uint64_t there = __ballot(e >= 0);
+        if (whole(x, there)) continue;
+        const long vo = row_offset(a.vc, batch.page, e, first_of(x) + (lane & 31));
+#pragma unroll 1
+        for (int i = 0; i < 32; ++i) {
+          const int key = first_of(x) + i;
+          const bool sees = ((there >> i) & 1) && key >= seen.low && key <= seen.high;
+          acc.add_unusual(vb + ((there >> i) & 1 ? read_lane(vo, i) : 0), sees, FULL ? L::DC : a.D);
+        }
+      }
+    }
 
     // the four waves' sums: each brought to the common maximum, then added through LDS
     const float l = acc.l + other_half(acc.l);
@@ -722,7 +782,7 @@ QMOE_DEV void few_rows(const AttentionArgs& a, int block, unsigned char* lds) {
       }
     }
     __syncthreads();
-    if (f >= start + keys.tiles * a.Hkv && f < stop) b = list.locate(a, f, keys, start);
+    if (f >= start + each * a.Hkv && f < stop) b = list.locate(a, f, keys, start);
   }
 }
 
@@ -809,9 +869,9 @@ __global__ __launch_bounds__(256) void join_kernel(AttentionArgs a, int join_row
     int start;
     const int b = list.locate(a, f, keys, start);
     if (b >= batch.B) return;
-    const int h = (f - start) / keys.tiles;
-    start += h * keys.tiles;
-    if (start == f || start < f - list.share) return;
+    const int each = FewList::places(keys), h = (f - start) / each;
+    start += h * each + LEAD;
+    if (start >= f || start < f - list.share) return;
     const int last = (start + keys.tiles - 1) / list.share, row0 = batch.first_row(b);
     for (int r = blockIdx.x - block * join_rows; r < keys.n * G; r += join_rows) {
       const int token = a.group.div(r);
@@ -854,7 +914,7 @@ Plan plan_for(int T, int B, int Hq, int Hkv, int D, int page, int width, bool on
   p.slots = D > 128 ? 256 : 512;  // workgroups that run at once
   const long most = std::min((long)width * page, 0x7fffffffl);  // keys
   if (few) {
-    const long tiles = (long)B * Hkv * std::max<long>(1, (most + FEW_KEYS - 1) / FEW_KEYS);
+    const long tiles = (long)B * Hkv * (std::max<long>(1, (most + FEW_KEYS - 1) / FEW_KEYS));
     p.few_blocks = (int)std::max(1l, std::min<long>(p.slots, tiles));
     p.few_floats = 2l * p.few_blocks * p.few_rows * (D + 2);
   }
@@ -933,7 +993,7 @@ int qmoe_paged_attention(const void* q, long q_token, long q_head, const void* k
   // bytes within a page, from page to page, and the list of the few-rows form are counted in 32 bits
   for (const long step : {k_page, v_page, k_slot * page, v_slot * page, k_head, v_head})
     if (step < 0 || step >= 1l << 30) return QMOE_EINVAL;
-  if ((long)B * Hkv * (std::min((long)table_width * page, 0x7fffffffl) / FEW_KEYS + 1) > 0x7fffff00l) return QMOE_EINVAL;
+  if ((long)B * Hkv * (std::min((long)table_width * page, 0x7fffffffl) / FEW_KEYS + 1 + LEAD) > 0x7fffff00l) return QMOE_EINVAL;
   const Plan p = plan_for(T, B, Hq, Hkv, D, page, table_width, !starts);
   if (p.few_floats + p.many_floats &&
       (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15) || workspace_bytes < 4 * (p.few_floats + p.many_floats)))
