@@ -786,82 +786,104 @@ QMOE_DEV void few_rows(const AttentionArgs& a, int block, unsigned char* lds) {
   }
 }
 
-template <typename E, int NK, bool FULL>
-__global__ __launch_bounds__(256, (NK <= 4 ? 2 : 1)) void attention_many_kernel(AttentionArgs a) {
+// Each form by itself, and both in one launch (the few-rows form in the first blocks).
+enum { MANY = 1, FEW_ROWS = 2 };
+template <typename E, int NK, bool FULL, int FORMS>
+__global__ __launch_bounds__(256, (NK <= 4 ? 2 : 1)) void attention_kernel(AttentionArgs a) {
   __shared__ __align__(16) unsigned char lds[Layout<NK>::LDS];
-  many_rows<E, NK, FULL>(a, blockIdx.x, lds);
-}
-template <typename E, int NK, bool FULL>
-__global__ __launch_bounds__(256, (NK <= 4 ? 2 : 1)) void attention_few_kernel(AttentionArgs a) {
-  __shared__ __align__(16) unsigned char lds[Layout<NK>::LDS];
-  few_rows<E, NK, FULL>(a, blockIdx.x, lds);
+  if constexpr (FORMS == MANY) many_rows<E, NK, FULL>(a, blockIdx.x, lds);
+  else if constexpr (FORMS == FEW_ROWS) few_rows<E, NK, FULL>(a, blockIdx.x, lds);
+  else if ((int)blockIdx.x < a.few_blocks) few_rows<E, NK, FULL>(a, blockIdx.x, lds);
+  else many_rows<E, NK, FULL>(a, blockIdx.x - a.few_blocks, lds);
 }
 
 // ---------------------------------------------------------------- joining
 
-// One row's parts: sums of D and (maximum, sum), `count` of them at at(c). The parts' scales first, then as
-// many parts at once as the threads make rows of D, eight of them in flight each.
-constexpr int JOIN_ROWS = 8;  // workgroups that share out the rows of a tile
+// Rows' parts: sums of D and (maximum, sum), `count` of them for a row, part c of row r at at(r, c); rows
+// `from` and so on below `rows`. Up to 64 parts: a wave to a row, 4 JOIN of them at once; more: a
+// workgroup to a row. The parts' scales first, then as many parts at once as threads make rows of D, eight of
+// them in flight each.
+constexpr int JOIN = 8;  // workgroups that share out the rows of a tile
 constexpr int PARTS_MAX = 520;
-template <typename E, typename At>
-QMOE_DEV void join_row(const float* sums, const float2* tops, At at, int count, uint16_t* out, int D) {
+template <typename E, typename At, typename Out>
+QMOE_DEV void join_rows(const float* sums, const float2* tops, At at, int count, int slot, int rows, Out out, int D) {
   __shared__ float scale[PARTS_MAX], sum_of[4];
   __shared__ __align__(16) f32x4_v part[256];
-  const int tid = threadIdx.x;
-  float2 t[3];
-  float m = -INFINITY, l = 0.f;
-#pragma unroll
-  for (int i = 0; i < 3; ++i) {
-    t[i] = make_float2(-INFINITY, 0.f);
-    if (tid + 256 * i < count) t[i] = tops[at(tid + 256 * i)];
-    m = fmaxf(m, t[i].x);
-  }
-#pragma unroll
-  for (int o = 32; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
-  if ((tid & 63) == 0) sum_of[tid >> 6] = m;
-  __syncthreads();
-  m = fmaxf(fmaxf(sum_of[0], sum_of[1]), fmaxf(sum_of[2], sum_of[3]));
-#pragma unroll
-  for (int i = 0; i < 3; ++i)
-    if (tid + 256 * i < count) {
-      const float f = t[i].y == 0.f ? 0.f : t[i].x == m ? 1.f : __builtin_amdgcn_exp2f(t[i].x - m);
-      scale[tid + 256 * i] = f;
-      l += t[i].y == 0.f ? 0.f : t[i].y * f;
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const bool alone = count <= 64;  // a wave by itself
+  const int tid = alone ? lane : threadIdx.x, threads = alone ? 64 : 256;
+  const int quads = D / 4, streams = threads / quads, stream = tid / quads, quad = tid - stream * quads;
+  float* scales = alone ? scale + 64 * wave : scale;
+  f32x4_v* parts = alone ? part + 64 * wave : part;
+  auto meet = [&] {
+    if (alone) {
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+    } else {
+      __syncthreads();
     }
-  l = wave_sum_f32(l);
-  __syncthreads();
-  if ((tid & 63) == 0) sum_of[tid >> 6] = l;
-  const int quads = D / 4, streams = 256 / quads, stream = tid / quads, quad = tid - stream * quads;
-  f32x4_v o = {0.f, 0.f, 0.f, 0.f};
-  if (stream < streams)
-    for (int c = stream; c < count; c += 8 * streams) {
-      f32x4_v x[8];
+  };
+  for (int r = alone ? slot * 4 + wave : slot; r < rows; r += alone ? 4 * JOIN : JOIN) {
+    float2 t[3];
+    float m = -INFINITY, l = 0.f;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = reinterpret_cast<const f32x4_v*>(sums + at(min(c + i * streams, count - 1)) * D)[quad];
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (c + i * streams < count) o += x[i] * scale[c + i * streams];
+    for (int i = 0; i < 3; ++i) {
+      t[i] = make_float2(-INFINITY, 0.f);
+      if ((i == 0 || !alone) && tid + 256 * i < count) t[i] = tops[at(r, tid + 256 * i)];
+      m = fmaxf(m, t[i].x);
     }
-  part[tid] = o;
-  __syncthreads();
-  l = (sum_of[0] + sum_of[1]) + (sum_of[2] + sum_of[3]);
-  if (tid < quads) {
-    for (int c = 1; c < streams; ++c) o += part[c * quads + tid];
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    reinterpret_cast<uint2*>(out)[tid] = make_uint2(Mma<E>::pack(o[0] * inv, o[1] * inv), Mma<E>::pack(o[2] * inv, o[3] * inv));
+#pragma unroll
+    for (int o = 32; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+    if (!alone) {
+      if (lane == 0) sum_of[wave] = m;
+      meet();
+      m = fmaxf(fmaxf(sum_of[0], sum_of[1]), fmaxf(sum_of[2], sum_of[3]));
+      meet();
+    }
+#pragma unroll
+    for (int i = 0; i < 3; ++i)
+      if ((i == 0 || !alone) && tid + 256 * i < count) {
+        const float f = t[i].y == 0.f ? 0.f : t[i].x == m ? 1.f : __builtin_amdgcn_exp2f(t[i].x - m);
+        scales[tid + 256 * i] = f;
+        l += t[i].y == 0.f ? 0.f : t[i].y * f;
+      }
+    l = wave_sum_f32(l);
+    if (!alone && lane == 0) sum_of[wave] = l;
+    meet();
+    if (!alone) l = (sum_of[0] + sum_of[1]) + (sum_of[2] + sum_of[3]);
+    f32x4_v o = {0.f, 0.f, 0.f, 0.f};
+    if (stream < streams)
+      for (int c = stream; c < count; c += 8 * streams) {
+        f32x4_v x[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = reinterpret_cast<const f32x4_v*>(sums + at(r, min(c + i * streams, count - 1)) * D)[quad];
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (c + i * streams < count && scales[c + i * streams] != 0.f) o += x[i] * scales[c + i * streams];
+      }
+    parts[tid] = o;
+    meet();
+    if (tid < quads) {
+      for (int c = 1; c < streams; ++c) o += parts[c * quads + tid];
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      reinterpret_cast<uint2*>(out(r))[tid] = make_uint2(Mma<E>::pack(o[0] * inv, o[1] * inv), Mma<E>::pack(o[2] * inv, o[3] * inv));
+    }
+    meet();
   }
-  __syncthreads();
 }
 
-// Blocks [0, few_blocks) x join_rows: the head inside whose tiles the first boundary is the one between the
-// shares of block - 1 and block, every join_rows-th row. Behind them, where the many-rows form cuts
-// keys into pieces, so many for each tile and head.
+// Blocks [0, few_blocks) x JOIN: the head inside whose tiles the first boundary is the one between the
+// shares of block - 1 and block. Behind them, where the many-rows form cuts keys into pieces, JOIN for
+// each tile and head.
 template <typename E>
-__global__ __launch_bounds__(256) void join_kernel(AttentionArgs a, int join_rows) {
+__global__ __launch_bounds__(256) void join_kernel(AttentionArgs a) {
   const Batch& batch = a.batch;
-  const int few = a.few_blocks * join_rows, G = a.group.d;
+  const int few = a.few_blocks * JOIN, G = a.group.d, block = blockIdx.x < few ? blockIdx.x / JOIN : (blockIdx.x - few) / JOIN;
+  const int slot = (blockIdx.x < few ? blockIdx.x : blockIdx.x - few) % JOIN;
+  const float *sums, *tops;
+  int count, rows, row0, h, first;  // rows of the tile; its first token's row and its own first row
+  Pieces pieces = {};
   if ((int)blockIdx.x < few) {
-    const int block = blockIdx.x / join_rows;
     if (block == 0) return;
     const FewList list(a);
     const int f = list.share * block;
@@ -869,30 +891,34 @@ __global__ __launch_bounds__(256) void join_kernel(AttentionArgs a, int join_row
     int start;
     const int b = list.locate(a, f, keys, start);
     if (b >= batch.B) return;
-    const int each = FewList::places(keys), h = (f - start) / each;
+    const int each = FewList::places(keys);
+    h = (f - start) / each;
     start += h * each + LEAD;
     if (start >= f || start < f - list.share) return;
-    const int last = (start + keys.tiles - 1) / list.share, row0 = batch.first_row(b);
-    for (int r = blockIdx.x - block * join_rows; r < keys.n * G; r += join_rows) {
-      const int token = a.group.div(r);
-      const long row = (long)(row0 + token) * a.Hq + h * G + r - token * G;
-      join_row<E>(a.few_part, few_tops(a), [&](int c) { return part_of(block - 1 + c, c == 0) * a.few_rows + r; },
-                  last - block + 2, static_cast<uint16_t*>(a.out) + row * a.D, a.D);
-    }
+    count = (start + keys.tiles - 1) / list.share - block + 2;
+    rows = keys.n * G, row0 = batch.first_row(b), first = 0;
   } else {
-    const int block = blockIdx.x - few, rest = block / JOIN_ROWS, number = a.heads.div(rest), h = rest - number * a.Hkv;
+    const int number = a.heads.div(block);
+    h = block - number * a.Hkv;
     const ManyTile t = many_tile(a, number);
     if (t.r0 < 0 || t.tiles <= 8) return;
-    const Pieces pieces = pieces_of(a, t, h);
-    const int count = min((t.tiles + pieces.size - 1) / pieces.size, a.pieces);
+    pieces = pieces_of(a, t, h);
+    count = min((t.tiles + pieces.size - 1) / pieces.size, a.pieces);
     if (count <= 1) return;
-    for (int r = block - rest * JOIN_ROWS; r < min(ROWS, t.rows - t.r0); r += JOIN_ROWS) {
-      const int token = a.group.div(t.r0 + r);
-      const long row = (long)(t.row0 + token) * a.Hq + h * G + t.r0 + r - token * G;
-      join_row<E>(a.many_part, many_tops(a), [&](int c) { return piece_at(pieces, c) * ROWS + r; }, count,
-                  static_cast<uint16_t*>(a.out) + row * a.D, a.D);
-    }
+    rows = min(ROWS, t.rows - t.r0), row0 = t.row0, first = t.r0;
   }
+  const bool is_few = (int)blockIdx.x < few;
+  sums = is_few ? a.few_part : a.many_part;
+  tops = reinterpret_cast<const float*>(is_few ? few_tops(a) : many_tops(a));
+  join_rows<E>(sums, reinterpret_cast<const float2*>(tops),
+               [&](int r, int c) { return is_few ? part_of(block - 1 + c, c == 0) * a.few_rows + r : piece_at(pieces, c) * ROWS + r; },
+               count, slot, rows,
+               [&](int r) {
+                 const int token = a.group.div(first + r);
+                 const long row = (long)(row0 + token) * a.Hq + h * G + first + r - token * G;
+                 return static_cast<uint16_t*>(a.out) + row * a.D;
+               },
+               a.D);
 }
 
 // ---------------------------------------------------------------- host
@@ -930,20 +956,16 @@ Plan plan_for(int T, int B, int Hq, int Hkv, int D, int page, int width, bool on
 
 template <typename E, int NK, bool FULL>
 int launch(const AttentionArgs& a, hipStream_t st) {
-  const long tiles = (long)a.many_tiles * a.Hkv, blocks = tiles * a.pieces;
-  if (blocks > 0x7fffffffl || tiles * JOIN_ROWS > 0x7ffffffl) return QMOE_EINVAL;
-  if (a.few_blocks) {
-    hipLaunchKernelGGL((attention_few_kernel<E, NK, FULL>), dim3(a.few_blocks), dim3(256), 0, st, a);
-    if (const int rc = (int)hipGetLastError()) return rc;
-  }
-  if (blocks) {
-    hipLaunchKernelGGL((attention_many_kernel<E, NK, FULL>), dim3((unsigned)blocks), dim3(256), 0, st, a);
-    if (const int rc = (int)hipGetLastError()) return rc;
-  }
-  const int join_rows = std::min(a.few_rows, JOIN_ROWS);
-  const long joins = (long)a.few_blocks * join_rows + (a.pieces > 1 ? tiles * JOIN_ROWS : 0);
-  if (joins == 0) return QMOE_OK;
-  hipLaunchKernelGGL((join_kernel<E>), dim3((unsigned)joins), dim3(256), 0, st, a, join_rows);
+  const long tiles = (long)a.many_tiles * a.Hkv, blocks = tiles * a.pieces + a.few_blocks;
+  if (blocks > 0x7fffffffl || tiles * JOIN > 0x7ffffffl) return QMOE_EINVAL;
+  const dim3 grid((unsigned)blocks), threads(256);
+  if (!a.few_blocks) hipLaunchKernelGGL((attention_kernel<E, NK, FULL, MANY>), grid, threads, 0, st, a);
+  else if (!tiles) hipLaunchKernelGGL((attention_kernel<E, NK, FULL, FEW_ROWS>), grid, threads, 0, st, a);
+  else hipLaunchKernelGGL((attention_kernel<E, NK, FULL, MANY | FEW_ROWS>), grid, threads, 0, st, a);
+  const int rc = (int)hipGetLastError();
+  const long joins = JOIN * (a.few_blocks + (a.pieces > 1 ? tiles : 0));
+  if (rc || joins == 0) return rc;
+  hipLaunchKernelGGL((join_kernel<E>), dim3((unsigned)joins), threads, 0, st, a);
   return (int)hipGetLastError();
 }
 
