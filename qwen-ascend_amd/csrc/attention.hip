@@ -89,6 +89,10 @@ struct Mma<ElemBF16> {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(frag, a), __builtin_bit_cast(frag, b), c, 0, 0, 0);
   }
   QMOE_DEV static uint32_t pack(float lo, float hi) { return pk_bf16(lo, hi); }
+  // sum + both elements, in fp32
+  QMOE_DEV static float add_pair(uint32_t v, float sum) {
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_v, v), __builtin_bit_cast(bf16x2_v, 0x3f803f80u), sum, false);
+  }
   static constexpr uint32_t EXPONENT = 0x7f807f80u, ONE = 0x00800080u;
 };
 template <>
@@ -100,13 +104,20 @@ struct Mma<ElemF16> {
   QMOE_DEV static uint32_t pack(float lo, float hi) {
     return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2_v){lo, hi}, f16x2_v));
   }
+  QMOE_DEV static float add_pair(uint32_t v, float sum) {
+    return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2_v, v), __builtin_bit_cast(f16x2_v, 0x3c003c00u), sum, false);
+  }
   static constexpr uint32_t EXPONENT = 0x7c007c00u, ONE = 0x04000400u;
 };
 
-// max or sum with lane ^ 32
-QMOE_DEV float other_half(float v) {
+// Maximum and sum with lane ^ 32.
+QMOE_DEV float half_max(float v) {
   const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return __uint_as_float((threadIdx.x & 32) ? r[0] : r[1]);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+QMOE_DEV float half_sum(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
 // Heads of up to 32 * NK elements. In LDS rows are DP elements apart; the 16-byte pieces of a row are XOR'd with
@@ -147,38 +158,41 @@ struct Rows {
   // Scores s become weights relative to the running maximum, which moves only where a score exceeds
   // it by 2^8: weights stay below 2^8, where fp32 and the 16-bit types hold them as well as below 1, and
   // most tiles leave the output's registers alone.
-  QMOE_DEV void weigh(f32x16_v (&s)[NJ], float scale, s16x8_v (&p)[2 * NJ]) {
+  QMOE_DEV static float top_of(const f32x16_v (&s)[NJ], float scale) {
     float t = s[0][0];
 #pragma unroll
     for (int j = 0; j < NJ; ++j)
 #pragma unroll
       for (int r = 0; r < 16; ++r) t = fmaxf(t, s[j][r]);
-    t = fmaxf(t, other_half(t)) * scale;
-    if (__any(t > m + 8.f)) {
-      const float top = fmaxf(m, t), f = m == top ? 1.f : __builtin_amdgcn_exp2f(m - top);
-      m = top, l *= f;
+    return half_max(t) * scale;
+  }
+  QMOE_DEV bool above(float t) const { return __any(t > m + 8.f); }
+  // All weights taken so far must be in o and l.
+  QMOE_DEV void raise(float t) {
+    const float top = fmaxf(m, t), f = m == top ? 1.f : __builtin_amdgcn_exp2f(m - top);
+    m = top, l *= f;
 #pragma unroll
-      for (int dt = 0; dt < NK; ++dt)
+    for (int dt = 0; dt < NK; ++dt)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) o[dt][r] *= f;
-    }
+      for (int r = 0; r < 16; ++r) o[dt][r] *= f;
+  }
+  QMOE_DEV void weigh(const f32x16_v (&s)[NJ], float scale, s16x8_v (&p)[2 * NJ]) {
     const float base = m == -INFINITY ? 0.f : m;
-    float sum[4] = {};
-#pragma unroll
-    for (int j = 0; j < NJ; ++j)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        s[j][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j][r], scale, -base));
-        sum[r & 3] += s[j][r];
-      }
-    l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+    float sum[2] = {};
 #pragma unroll
     for (int i = 0; i < 2 * NJ; ++i) {
       uint32_t w[4];
 #pragma unroll
-      for (int r = 0; r < 4; ++r) w[r] = Mma<E>::pack(s[i / 2][8 * (i & 1) + 2 * r], s[i / 2][8 * (i & 1) + 2 * r + 1]);
+      for (int r = 0; r < 4; ++r) {
+        const int at = 8 * (i & 1) + 2 * r;
+        const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i / 2][at], scale, -base));
+        const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i / 2][at + 1], scale, -base));
+        w[r] = Mma<E>::pack(x, y);
+        sum[r & 1] = Mma<E>::add_pair(w[r], sum[r & 1]);
+      }
       p[i] = __builtin_bit_cast(s16x8_v, (u32x4_v){w[0], w[1], w[2], w[3]});
     }
+    l += sum[0] + sum[1];
   }
 
   // o += V^T p, V's rows in LDS. A lane of a transposing read names 4 elements of a row: in groups of 16 lanes,
@@ -199,23 +213,18 @@ struct Rows {
       }
   }
 
-  // One tile: scores s, whose keys start at `first`; `whole`: every row sees all of them.
-  QMOE_DEV void take(f32x16_v (&s)[NJ], const unsigned char* v, float scale, bool whole, Seen seen, uint64_t present, int first) {
-    if (!whole) {
-      const int half = (threadIdx.x >> 5) & 1, from = first + 4 * half, low = seen.low - from, high = seen.high - from;
+  // Scores of keys `first` and so on: those that the row does not see become -inf.
+  QMOE_DEV static void mask(f32x16_v (&s)[NJ], Seen seen, uint64_t present, int first) {
+    const int half = (threadIdx.x >> 5) & 1, from = first + 4 * half, low = seen.low - from, high = seen.high - from;
 #pragma unroll
-      for (int j = 0; j < NJ; ++j) {
-        const uint32_t there = (uint32_t)(present >> (32 * j)) >> (4 * half);
+    for (int j = 0; j < NJ; ++j) {
+      const uint32_t there = (uint32_t)(present >> (32 * j)) >> (4 * half);
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int key = key_of(j, r);
-          if (!((there >> (key & 31)) & 1) || key < low || key > high) s[j][r] = -INFINITY;
-        }
+      for (int r = 0; r < 16; ++r) {
+        const int key = key_of(j, r);
+        if (!((there >> (key & 31)) & 1) || key < low || key > high) s[j][r] = -INFINITY;
       }
     }
-    s16x8_v p[2 * NJ];
-    weigh(s, scale, p);
-    add(v, p);
   }
 
   // The infinite and NaN values of one key, which were left out of its tile: o += v where the row sees it.
@@ -425,7 +434,7 @@ QMOE_DEV void many_rows(const AttentionArgs& a, int block, unsigned char* lds) {
   const uint16_t* q_row = static_cast<const uint16_t*>(a.q) + (row0 + token) * a.q_token + (h * G + of) * a.q_head;
 #pragma unroll
   for (int ks = 0; ks < 2 * NK; ++ks) q[ks] = q_piece(q_row, 16 * ks + 8 * half, a.D, valid, a.negate);
-  Rows<E, NK, 2> acc;
+  Rows<E, NK, 1> acc;
   acc.clear();
 
   const unsigned char* kb = static_cast<const unsigned char*>(a.k) + 2 * h * a.kc.head;
@@ -464,14 +473,52 @@ QMOE_DEV void many_rows(const AttentionArgs& a, int block, unsigned char* lds) {
     if (t0 + 1 < t1) entry = entry_of(t0 + 1);
   }
   const int k_row = lane & 31, k_base = k_row * L::STRIDE, k_swizzle = L::k_swizzle(k_row);
-  // One tile from LDS at `k`, while the next is loaded to `next`. (As a function of two pointers that
-  // share nothing, which spares a wait for the load before every transposing read.)
   const int last_pos = before + (int)a.group.div(min(r0 + ROWS, rows) - 1), first_pos = before + (int)a.group.div(r0);
   auto partial = [&](int tile, uint64_t present) {  // not seen whole by every row of the workgroup
     const int first = begin + 64 * tile;
     return present != ~0ull || first + 63 > first_pos || (a.window && first <= last_pos - a.window);
   };
-  auto step = [&](int tile, unsigned char* __restrict__ now, unsigned char* __restrict__ next) {
+  // One tile from LDS at `now`, while the next is loaded to `next`. As a function of two pointers that share
+  // nothing, which spares a wait for the load before every transposing read; no wait and no barrier may stand
+  // in it, which such pointers would let the reads pass.
+  auto step = [&](int tile, const unsigned char* __restrict__ now, unsigned char* __restrict__ next) {
+    const uint64_t present = present_next;
+    if (tile + 1 < t1) {
+      present_next = load(tile + 1, entry, next);
+      if (tile + 2 < t1) entry = entry_of(tile + 2);
+    }
+    const int first = begin + 64 * tile;
+    if (first > wave_last || (a.window && first + 63 <= wave_first - a.window)) return;
+    // two halves of 32 keys: the matrix pipe takes the scores of the second while the vector pipe takes the
+    // weights of the first, then the sums of the first while it takes the weights of the second
+    f32x16_v s[2][1];
+    auto score = [&](int j) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[j][0][i] = 0.f;
+#pragma unroll
+      for (int ks = 0; ks < 2 * NK; ++ks) {
+        const s16x8_v f = *reinterpret_cast<const s16x8_v*>(now + k_base + 32 * j * L::STRIDE + 16 * ((2 * ks + half) ^ k_swizzle));
+        s[j][0] = Mma<E>::mma(f, q[ks], s[j][0]);
+      }
+    };
+    const bool whole = present == ~0ull && first + 63 <= wave_first && (!a.window || first > wave_last - a.window);
+    const unsigned char* v = now + L::TILE;
+    s16x8_v p0[2], p1[2];
+    score(0);
+    if (!whole) acc.mask(s[0], seen, present, first);
+    const float t0 = acc.top_of(s[0], a.scale);
+    if (acc.above(t0)) acc.raise(t0);
+    score(1);
+    acc.weigh(s[0], a.scale, p0);
+    if (!whole) acc.mask(s[1], seen, present >> 32, first + 32);
+    const float t1 = acc.top_of(s[1], a.scale);
+    acc.add(v, p0);
+    if (acc.above(t1)) acc.raise(t1);
+    acc.weigh(s[1], a.scale, p1);
+    acc.add(v + 32 * L::STRIDE, p1);
+  };
+  for (int tile = t0; tile < t1; ++tile) {
+    unsigned char *now = lds + (tile & 1) * 2 * L::TILE, *next = lds + (~tile & 1) * 2 * L::TILE;
     // the tile has landed, and every wave is past the one before it, whose half of LDS takes the next
     asm volatile("" ::: "memory");
     wait_vm_lgkm0<0>();
@@ -481,29 +528,8 @@ QMOE_DEV void many_rows(const AttentionArgs& a, int block, unsigned char* lds) {
       wait_vm_lgkm0<0>();
     }
     barrier_no_fence();
-    const uint64_t present = present_next;
-    if (tile + 1 < t1) {
-      present_next = load(tile + 1, entry, next);
-      if (tile + 2 < t1) entry = entry_of(tile + 2);
-    }
-    const int first = begin + 64 * tile;
-    if (first > wave_last || (a.window && first + 63 <= wave_first - a.window)) return;
-    f32x16_v s[2];
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) s[j][i] = 0.f;
-#pragma unroll
-    for (int ks = 0; ks < 2 * NK; ++ks)
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const s16x8_v f = *reinterpret_cast<const s16x8_v*>(now + k_base + 32 * j * L::STRIDE + 16 * ((2 * ks + half) ^ k_swizzle));
-        s[j] = Mma<E>::mma(f, q[ks], s[j]);
-      }
-    const bool whole = present == ~0ull && first + 63 <= wave_first && (!a.window || first > wave_last - a.window);
-    acc.take(s, now + L::TILE, a.scale, whole, seen, present, first);
-  };
-  for (int tile = t0; tile < t1; ++tile) step(tile, lds + (tile & 1) * 2 * L::TILE, lds + (~tile & 1) * 2 * L::TILE);
+    step(tile, now, next);
+  }
   __syncthreads();
   if (unusual) {
     for (int tile = t0; tile < t1; ++tile) {
@@ -521,7 +547,7 @@ QMOE_DEV void many_rows(const AttentionArgs& a, int block, unsigned char* lds) {
     }
   }
 
-  const float l = acc.l + other_half(acc.l);
+  const float l = half_sum(acc.l);
   if (!valid) return;
   if (cut) {
     const long at = piece_at(pieces, piece) * ROWS + 32 * wave + (lane & 31);
@@ -699,12 +725,9 @@ QMOE_DEV void few_rows(const AttentionArgs& a, int block, unsigned char* lds) {
       const int first = first_of(x);
       return there == ~0ull && first + 31 <= keys.before && (!a.window || first > keys.before + keys.n - 1 - a.window);
     };
-    auto step = [&](int x, unsigned char* __restrict__ v, unsigned char* __restrict__ next) {
-      asm volatile("" ::: "memory");
-      wait_vm_lgkm0<0>();
-      asm volatile("" ::: "memory");
+    // One tile's V in LDS at `v`, while the next is loaded to `next` (no wait in it, as in the other form).
+    auto step = [&](int x, const unsigned char* __restrict__ v, unsigned char* __restrict__ next) {
       const uint64_t here = present;
-      if (!whole(x, here) && clean<E, 32 / L::RPI>(v, 1)) unusual = true;
       entry = known(entry_next);
       present = __ballot(entry >= 0);
       if (x + 1 < x1) load_v(x + 1, entry, present, next);
@@ -722,9 +745,21 @@ QMOE_DEV void few_rows(const AttentionArgs& a, int block, unsigned char* lds) {
       // the loads would cost a wait for them where it ends).
       asm volatile("" ::: "memory");
       load_k(x + 1, entry);
-      acc.take(s, v, a.scale, whole(x, here), seen, here, first);
+      if (!whole(x, here)) acc.mask(s, seen, here, first);
+      s16x8_v p[2];
+      const float t = acc.top_of(s, a.scale);
+      if (acc.above(t)) acc.raise(t);
+      acc.weigh(s, a.scale, p);
+      acc.add(v, p);
     };
-    for (int x = x0; any && x < x1; ++x) step(x, mine + ((x - x0) & 1) * 32 * L::STRIDE, mine + ((x - x0 + 1) & 1) * 32 * L::STRIDE);
+    for (int x = x0; any && x < x1; ++x) {
+      unsigned char *v = mine + ((x - x0) & 1) * 32 * L::STRIDE, *next = mine + ((x - x0 + 1) & 1) * 32 * L::STRIDE;
+      asm volatile("" ::: "memory");
+      wait_vm_lgkm0<0>();
+      asm volatile("" ::: "memory");
+      if (!whole(x, present) && clean<E, 32 / L::RPI>(v, 1)) unusual = true;
+      step(x, v, next);
+    }
     if (unusual) {
       for (int x = x0; x < x1; ++x) {
         const int e = known(entry_of(x));
@@ -741,7 +776,7 @@ QMOE_DEV void few_rows(const AttentionArgs& a, int block, unsigned char* lds) {
     }
 
     // the four waves' sums: each brought to the common maximum, then added through LDS
-    const float l = acc.l + other_half(acc.l);
+    const float l = half_sum(acc.l);
     if (half == 0) m_of[wave][r] = acc.m, l_of[wave][r] = l;
     __syncthreads();  // (and V's rows in LDS are done with)
     float top = m_of[0][r];

@@ -30,9 +30,12 @@ HIPCC_FLAGS = [
 # rewrite reads the result back at once, which stalls the wave on the
 # atomic's round trip).
 # w8_gemm.hip: MFMA accumulators stay in VGPRs (the AGPR form moved the group
-# sums to VGPRs and back for every scale-group fma).
+# sums to VGPRs and back for every scale-group fma). attention.hip: the same
+# for the output's sums, which a new maximum rescales (heads of 256: moved and
+# spilled).
 FILE_FLAGS = {"w4_gemv.hip": ["-mllvm", "-amdgpu-atomic-optimizer-strategy=None"],
-              "w8_gemm.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
+              "w8_gemm.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
+              "attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
 
 
 def flags_for(src: Path) -> list:
