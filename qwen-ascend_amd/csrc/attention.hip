@@ -142,7 +142,7 @@ template <typename E, int NK, int NJ>
 struct Rows {
   using L = Layout<NK>;
   f32x16_v o[NK];  // o[dt][r]: element 32 dt + 8 (r >> 2) + 4 half + (r & 3) of row lane & 31
-  float m, l;      // maximum in units of log2, sum of this half's keys
+  float m, l;      // a score that weights are relative to, in units of log2; sum of this half's weights
 
   QMOE_DEV void clear() {
     m = -INFINITY, l = 0.f;
@@ -155,28 +155,10 @@ struct Rows {
   // Number in the tile of the key in register r of block j, in lanes of the first half; 4 more in the others.
   QMOE_DEV static constexpr int key_of(int j, int r) { return 32 * j + 8 * (r >> 2) + (r & 3); }
 
-  // Scores s become weights relative to the running maximum, which moves only where a score exceeds
-  // it by 2^8: weights stay below 2^8, where fp32 and the 16-bit types hold them as well as below 1, and
-  // most tiles leave the output's registers alone.
-  QMOE_DEV static float top_of(const f32x16_v (&s)[NJ], float scale) {
-    float t = s[0][0];
-#pragma unroll
-    for (int j = 0; j < NJ; ++j)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) t = fmaxf(t, s[j][r]);
-    return half_max(t) * scale;
-  }
-  QMOE_DEV bool above(float t) const { return __any(t > m + 8.f); }
-  // All weights taken so far must be in o and l.
-  QMOE_DEV void raise(float t) {
-    const float top = fmaxf(m, t), f = m == top ? 1.f : __builtin_amdgcn_exp2f(m - top);
-    m = top, l *= f;
-#pragma unroll
-    for (int dt = 0; dt < NK; ++dt)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) o[dt][r] *= f;
-  }
-  QMOE_DEV void weigh(const f32x16_v (&s)[NJ], float scale, s16x8_v (&p)[2 * NJ]) {
+  // Scores s become weights p = 2^(scale s - m); returns their sum over this lane's keys. m is the maximum of the
+  // keys of some tile and moves only where that sum exceeds 2^12: weights below that are held by fp32 and the 16-bit
+  // types as well as those below 1, so most tiles need no maximum and leave the output's sums alone.
+  QMOE_DEV float weigh(const f32x16_v (&s)[NJ], float scale, s16x8_v (&p)[2 * NJ]) const {
     const float base = m == -INFINITY ? 0.f : m;
     float sum[2] = {};
 #pragma unroll
@@ -192,7 +174,31 @@ struct Rows {
       }
       p[i] = __builtin_bit_cast(s16x8_v, (u32x4_v){w[0], w[1], w[2], w[3]});
     }
-    l += sum[0] + sum[1];
+    return sum[0] + sum[1];
+  }
+  // Whether a row needs another m for weights of that sum (any, if it has none yet).
+  QMOE_DEV bool moves(float sum) const { return __any(sum > (m == -INFINITY ? -1.f : 0x1p12f)); }
+  // m becomes the maximum of these scores, where it is below; all weights before must be in o and l.
+  QMOE_DEV void move(const f32x16_v (&s)[NJ], float scale) {
+    float t = s[0][0];
+#pragma unroll
+    for (int j = 0; j < NJ; ++j)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) t = fmaxf(t, s[j][r]);
+    const float top = fmaxf(m, half_max(t) * scale), f = m == top ? 1.f : __builtin_amdgcn_exp2f(m - top);
+    m = top, l *= f;
+#pragma unroll
+    for (int dt = 0; dt < NK; ++dt)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) o[dt][r] *= f;
+  }
+  // weigh() with the maximum moved if need be; what comes before must be in o.
+  QMOE_DEV void settle(const f32x16_v (&s)[NJ], float scale, s16x8_v (&p)[2 * NJ], float sum) {
+    if (moves(sum)) {
+      move(s, scale);
+      sum = weigh(s, scale, p);
+    }
+    l += sum;
   }
 
   // o += V^T p, V's rows in LDS. A lane of a transposing read names 4 elements of a row: in groups of 16 lanes,
@@ -506,15 +512,11 @@ QMOE_DEV void many_rows(const AttentionArgs& a, int block, unsigned char* lds) {
     s16x8_v p0[2], p1[2];
     score(0);
     if (!whole) acc.mask(s[0], seen, present, first);
-    const float t0 = acc.top_of(s[0], a.scale);
-    if (acc.above(t0)) acc.raise(t0);
     score(1);
-    acc.weigh(s[0], a.scale, p0);
+    acc.settle(s[0], a.scale, p0, acc.weigh(s[0], a.scale, p0));
     if (!whole) acc.mask(s[1], seen, present >> 32, first + 32);
-    const float t1 = acc.top_of(s[1], a.scale);
     acc.add(v, p0);
-    if (acc.above(t1)) acc.raise(t1);
-    acc.weigh(s[1], a.scale, p1);
+    acc.settle(s[1], a.scale, p1, acc.weigh(s[1], a.scale, p1));
     acc.add(v + 32 * L::STRIDE, p1);
   };
   for (int tile = t0; tile < t1; ++tile) {
@@ -747,9 +749,7 @@ QMOE_DEV void few_rows(const AttentionArgs& a, int block, unsigned char* lds) {
       load_k(x + 1, entry);
       if (!whole(x, here)) acc.mask(s, seen, here, first);
       s16x8_v p[2];
-      const float t = acc.top_of(s, a.scale);
-      if (acc.above(t)) acc.raise(t);
-      acc.weigh(s, a.scale, p);
+      acc.settle(s, a.scale, p, acc.weigh(s, a.scale, p));
       acc.add(v, p);
     };
     for (int x = x0; any && x < x1; ++x) {
