@@ -56,7 +56,6 @@ struct AttentionArgs {
   int same_pages;   // 16 keys on 16 lie on one page
   int few;          // FEW, or 0: all sequences take the many-rows form
   int few_blocks, few_rows, many_tiles, pieces, slots;
-  FastDiv piece_div;
   float *few_part, *many_part;  // partial sums: rows of D, then pairs (maximum, sum)
 };
 
@@ -345,29 +344,51 @@ QMOE_DEV long row_offset(const CacheSteps& c, const FastDiv& page, int entry, in
 
 // A tile of 128 rows of a sequence of many, or of the rows behind the last one (b = B, no keys).
 struct ManyTile {
-  int b, row0, rows, r0, before, begin, tiles;  // r0 < 0: none
+  int b, row0, rows, r0, before, begin, tiles;
 };
-QMOE_DEV ManyTile many_tile(const AttentionArgs& a, int number) {
-  const int lane = threadIdx.x & 63, G = a.group.d;
-  const Batch& batch = a.batch;
-  ManyTile t = {};
-  // Sequence b's tiles start at start(b) G / ROWS + b: no two sequences' overlap, a few numbers are
-  // no tile at all.
-  for (int i = 1; i <= batch.B; i += 64)
-    t.b += __popcll(__ballot(i + lane <= batch.B && batch.start(min(i + lane, batch.B)) * G / ROWS + i + lane <= number));
-  t.row0 = batch.start(t.b);
-  const bool is = t.b < batch.B;
-  const int n = is ? max(batch.start(t.b + 1) - t.row0, 0) : batch.T - t.row0;
-  t.rows = n * G;
-  t.r0 = (number - t.row0 * G / ROWS - t.b) * ROWS;
-  if (t.r0 >= t.rows || (is && t.rows <= a.few)) t.r0 = -1;
-  t.before = is ? tokens_before(batch, t.b, n) : -0x40000000;
-  const int first_pos = t.before + (int)a.group.div(max(t.r0, 0)), last_pos = t.before + (int)a.group.div(min(t.r0 + ROWS, t.rows) - 1);
-  const int end = min(last_pos + 1, is ? batch.length(t.b) : 0);
-  t.begin = a.window ? max(first_pos - a.window + 1, 0) & ~63 : 0;
-  t.tiles = end > t.begin ? (end - t.begin + 63) / 64 : 0;
-  return t;
-}
+// All such tiles, sequence after sequence.
+struct ManyList {
+  int rows, total;  // of sequence `lane`; tiles of all
+  QMOE_DEV static int tiles_of(const AttentionArgs& a, int s, int rows) {
+    return s < a.batch.B && rows <= a.few ? 0 : (rows + ROWS - 1) / ROWS;
+  }
+  QMOE_DEV static int rows_of(const AttentionArgs& a, int s) {
+    return (s < a.batch.B ? a.batch.new_rows(s) : s == a.batch.B ? a.batch.T - a.batch.start(s) : 0) * (int)a.group.d;
+  }
+  QMOE_DEV ManyList(const AttentionArgs& a) {
+    const int lane = threadIdx.x & 63;
+    rows = rows_of(a, lane);
+    int sum = tiles_of(a, lane, rows);
+    for (int s = 64 + lane; s <= a.batch.B; s += 64) sum += tiles_of(a, s, rows_of(a, s));
+    total = lane_of(prefix_sum(sum), 63);
+  }
+  // Tile `number` < total.
+  QMOE_DEV ManyTile find(const AttentionArgs& a, int number) const {
+    const int lane = threadIdx.x & 63;
+    const Batch& batch = a.batch;
+    ManyTile t = {};
+    int first = 0;
+    for (int i = 0; i <= batch.B; i += 64) {
+      const int r = i ? rows_of(a, i + lane) : rows, mine = tiles_of(a, i + lane, r), upto = first + prefix_sum(mine);
+      const uint64_t past = __ballot(upto > number);
+      if (past) {
+        const int at = __ffsll((unsigned long long)past) - 1;
+        t.b = i + at, t.rows = lane_of(r, at), first = lane_of(upto - mine, at);
+        break;
+      }
+      first = lane_of(upto, 63);
+    }
+    const bool is = t.b < batch.B;
+    const int G = a.group.d, n = a.group.div(t.rows);
+    t.row0 = batch.start(t.b), t.r0 = (number - first) * ROWS;
+    t.before = is ? tokens_before(batch, t.b, n) : -0x40000000;
+    const int first_pos = t.before + (int)a.group.div(t.r0), last_pos = t.before + (int)a.group.div(min(t.r0 + ROWS, t.rows) - 1);
+    const int end = min(last_pos + 1, is ? batch.length(t.b) : 0);
+    t.begin = a.window ? max(first_pos - a.window + 1, 0) & ~63 : 0;
+    t.tiles = end > t.begin ? (end - t.begin + 63) / 64 : 0;
+    return t;
+  }
+};
 
 // Where tiles are few, each is cut into pieces of so many 64 keys that all pieces of the call make up about
 // as many as run at once. Tiles of a sequence count alike, with the most keys that one of them may see; in
@@ -405,12 +426,17 @@ QMOE_DEV void many_rows(const AttentionArgs& a, int block, unsigned char* lds) {
   using L = Layout<NK>;
   const int lane = threadIdx.x & 63, half = lane >> 5, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const Batch& batch = a.batch;
-  // heads next to each other (on XCDs of their own, whose L2 then holds few heads' keys), the last
-  // tiles, which see the most keys, first
-  const int rest = a.heads.div(block), h = block - rest * a.Hkv, back = a.piece_div.div(rest);
-  const int piece = rest - back * a.pieces;
-  const ManyTile mt = many_tile(a, a.many_tiles - 1 - back);
-  if (mt.r0 < 0) return;
+  // Heads next to each other (on XCDs of their own, whose L2 then holds few heads' keys), the last
+  // tiles, which see the most keys, first; all first pieces before any second one, what there is not behind
+  // all. An XCD's shader engines take workgroups in turn: with the pieces of a tile next to each other, most
+  // of which there are not, all that there are went to one of the four (8000 new tokens 1978 us, now 620).
+  const ManyList list(a);
+  const int rest = a.heads.div(block), h = block - rest * a.Hkv;
+  if (list.total == 0) return;
+  const int piece = rest / list.total;
+  if (piece >= a.pieces) return;
+  const ManyTile mt = list.find(a, list.total - 1 - (rest - piece * list.total));
+  if (mt.r0 < 0 || mt.r0 >= mt.rows) return;
   int t0 = 0, t1 = mt.tiles;
   bool cut = false;
   Pieces pieces = {};
@@ -935,8 +961,10 @@ __global__ __launch_bounds__(256) void join_kernel(AttentionArgs a) {
   } else {
     const int number = a.heads.div(block);
     h = block - number * a.Hkv;
-    const ManyTile t = many_tile(a, number);
-    if (t.r0 < 0 || t.tiles <= 8) return;
+    const ManyList list(a);
+    if (number >= list.total) return;
+    const ManyTile t = list.find(a, number);
+    if (t.r0 < 0 || t.r0 >= t.rows || t.tiles <= 8) return;
     pieces = pieces_of(a, t, h);
     count = min((t.tiles + pieces.size - 1) / pieces.size, a.pieces);
     if (count <= 1) return;
@@ -1063,7 +1091,7 @@ int qmoe_paged_attention(const void* q, long q_token, long q_head, const void* k
   a.batch.table_ld = table_ld, a.batch.n_pages = n_pages, a.batch.T = T, a.batch.B = B, a.batch.width = table_width;
   a.batch.page = FastDiv(page);
   a.Hq = Hq, a.Hkv = Hkv, a.D = D, a.window = window;
-  a.group = FastDiv(Hq / Hkv), a.heads = FastDiv(Hkv), a.piece_div = FastDiv(p.pieces);
+  a.group = FastDiv(Hq / Hkv), a.heads = FastDiv(Hkv);
   a.scale = std::max(std::fabs(scale) * LOG2E, FLT_MIN), a.negate = scale < 0;
   a.same_pages = page % 16 == 0;
   a.few = p.few, a.few_blocks = p.few_blocks, a.few_rows = p.few_rows, a.many_tiles = p.many_tiles;
