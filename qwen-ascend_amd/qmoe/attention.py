@@ -22,6 +22,7 @@ from . import _lib
 from .rotary import _apart, _check_rotary, _heads, _positions
 
 _TYPES = _lib.TYPES
+_bump = torch.autograd.graph.increment_version
 
 
 def _check_batch(table, lengths, starts, T):
@@ -37,16 +38,24 @@ def _check_batch(table, lengths, starts, T):
         raise RuntimeError(f"starts must be int32 [{B + 1}]")
 
 
-def _check_cache(k_cache, v_cache, dtype, Hkv, D):
+def _cache_steps(k_cache, v_cache, dtype, Hkv, D):
+    """Element steps (page, place, head) of both caches, checked; whether both are contiguous."""
     if k_cache.dtype != dtype or v_cache.dtype != dtype:
         raise RuntimeError("the caches must have the new tokens' type")
-    if k_cache.dim() != 4 or k_cache.shape != v_cache.shape:
+    shape = k_cache.shape
+    if len(shape) != 4 or v_cache.shape != shape:
         raise RuntimeError("the caches must be [pages, page, Hkv, D], both alike")
-    if k_cache.shape[2:] != (Hkv, D) or k_cache.shape[1] < 1:
-        raise RuntimeError(f"caches {tuple(k_cache.shape)} do not match heads [{Hkv}, {D}]")
+    if shape[2] != Hkv or shape[3] != D or shape[1] < 1:
+        raise RuntimeError(f"caches {tuple(shape)} do not match heads [{Hkv}, {D}]")
+    if k_cache.is_neg() or v_cache.is_neg():
+        raise RuntimeError("the elements of a cached head must be contiguous, and no lazily negated view")
+    if k_cache.is_contiguous() and v_cache.is_contiguous():
+        steps = (shape[1] * Hkv * D, Hkv * D, D)
+        return steps, steps, True
     for c in (k_cache, v_cache):
-        if (c.stride(3) != 1 and D != 1) or c.is_neg():
+        if c.stride(3) != 1 and D != 1:
             raise RuntimeError("the elements of a cached head must be contiguous, and no lazily negated view")
+    return _steps(k_cache), _steps(v_cache), False
 
 
 def _steps(c):
@@ -73,10 +82,11 @@ def append_kv(k, v, k_cache, v_cache, table, lengths, *, starts=None, rotary=Non
     T, Hkv, D = k.shape
     if v.dtype != k.dtype or v.shape != k.shape or Hkv < 1:
         raise RuntimeError("v must have k's type and shape, and heads")
-    _check_cache(k_cache, v_cache, k.dtype, Hkv, D)
-    for c in (k_cache, v_cache):
-        if c.numel() and not _apart(c.shape[:3], c.stride()[:3], D):
-            raise RuntimeError("the places of a cache must not overlap")
+    k_steps, v_steps, contiguous = _cache_steps(k_cache, v_cache, k.dtype, Hkv, D)
+    if not contiguous:
+        for c in (k_cache, v_cache):
+            if c.numel() and not _apart(c.shape[:3], c.stride()[:3], D):
+                raise RuntimeError("the places of a cache must not overlap")
     _check_batch(table, lengths, starts, T)
     if q is not None and (q.dtype != k.dtype or q.dim() != 3 or q.shape[0] != T or q.shape[2] != D):
         raise RuntimeError(f"q must be [{T}, Hq, {D}] in k's type")
@@ -92,22 +102,23 @@ def append_kv(k, v, k_cache, v_cache, table, lengths, *, starts=None, rotary=Non
             return append_kv(k, v, k_cache, v_cache, table, lengths, starts=starts, rotary=rotary, positions=positions, q=q)
     for c in (k_cache, v_cache):
         if not c.is_inference():
-            torch.autograd.graph.increment_version(c)
-    k, v, table = _heads(k, "k"), _heads(v, "v"), _rows(table)
-    lengths = lengths.contiguous()
+            _bump(c)
+    k, v = _heads(k, "k"), _heads(v, "v")
+    (k_token, k_head, _), (v_token, v_head, _) = k.stride(), v.stride()
+    lengths, table = lengths.contiguous(), _rows(table)
     starts = None if starts is None else starts.contiguous()
     positions = None if positions is None else positions.contiguous()
     out, Hq, q_token, q_head = None, 0, 0, 0
     if q is not None:
-        out, q = _lib.contiguous_like(q, q.dtype), _heads(q, "q")
-        Hq, q_token, q_head = q.shape[1], q.stride(0), q.stride(1)
+        out, q, Hq = q.new_empty(q.shape), _heads(q, "q"), q.shape[1]
+        q_token, q_head, _ = q.stride()
     ptr = _lib.ptr
     some = q if Hq else None  # heads or none
     dim, interleaved, turn = (0, 0, 1.0) if rotary is None else (rotary.dim, int(rotary.layout == "interleaved"), rotary.turn)
     _lib.check(_lib.lib().qmoe_append_kv(
-        k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), ptr(some), q_token, q_head,
-        None if some is None else out.data_ptr(), _TYPES[k.dtype], k_cache.data_ptr(), *_steps(k_cache),
-        v_cache.data_ptr(), *_steps(v_cache), table.data_ptr(), table.stride(0), table.shape[1], lengths.data_ptr(),
+        k.data_ptr(), k_token, k_head, v.data_ptr(), v_token, v_head, ptr(some), q_token, q_head,
+        None if some is None else out.data_ptr(), _TYPES[k.dtype], k_cache.data_ptr(), *k_steps,
+        v_cache.data_ptr(), *v_steps, table.data_ptr(), table.stride(0), table.shape[1], lengths.data_ptr(),
         ptr(starts), ptr(positions), int(positions is not None and positions.dtype == torch.int64), ptr(frequencies), dim,
         interleaved, turn, T, table.shape[0], Hq, Hkv, D, k_cache.shape[1], k_cache.shape[0], _lib.stream_of(k)), "append_kv")
     return out
@@ -135,18 +146,19 @@ def paged_attention(q, k_cache, v_cache, table, lengths, *, starts=None, scale=N
         raise RuntimeError(f"{Hq} query heads cannot share {Hkv} key heads, at most 64 each and 4096 in all")
     if T * Hq >= 1 << 31:
         raise RuntimeError("q must have fewer than 2^31 rows of heads")
-    _check_cache(k_cache, v_cache, q.dtype, Hkv, D)
-    for c in (k_cache, v_cache):
-        if c.data_ptr() % 16 or any(s % 8 for s in _steps(c)):
-            raise RuntimeError("cached heads must be 16-byte aligned")
+    k_steps, v_steps, contiguous = _cache_steps(k_cache, v_cache, q.dtype, Hkv, D)
+    k_ptr, v_ptr = k_cache.data_ptr(), v_cache.data_ptr()
+    if (k_ptr | v_ptr) & 15 or not (contiguous or all(s % 8 == 0 for s in (*k_steps, *v_steps))):
+        raise RuntimeError("cached heads must be 16-byte aligned")
     _check_batch(table, lengths, starts, T)
     if window != int(window) or not 0 <= window < 1 << 31:
         raise RuntimeError("window must be 0 (none) or a number of tokens")
     if not _lib.operands(q, k_cache, v_cache, table, lengths, starts):
         with torch.cuda.device(q.device):
             return paged_attention(q, k_cache, v_cache, table, lengths, starts=starts, scale=scale, window=window)
-    out = _lib.contiguous_like(q, q.dtype)
+    out = torch.empty_like(q) if q.is_contiguous() else q.new_empty(q.shape)
     q, table, lengths = _heads(q, "q"), _rows(table), lengths.contiguous()
+    q_token, q_head, _ = q.stride()
     starts = None if starts is None else starts.contiguous()
     L, B, page, width = _lib.lib(), table.shape[0], k_cache.shape[1], table.shape[1]
     nbytes = L.qmoe_paged_attention_workspace(T, B, Hq, Hkv, D, page, width, int(starts is None))
@@ -154,8 +166,7 @@ def paged_attention(q, k_cache, v_cache, table, lengths, *, starts=None, scale=N
     ws = q.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
     ptr = _lib.ptr
     _lib.check(L.qmoe_paged_attention(
-        q.data_ptr(), q.stride(0), q.stride(1), k_cache.data_ptr(), *_steps(k_cache), v_cache.data_ptr(),
-        *_steps(v_cache), _TYPES[q.dtype], table.data_ptr(), table.stride(0), width, lengths.data_ptr(), ptr(starts),
+        q.data_ptr(), q_token, q_head, k_ptr, *k_steps, v_ptr, *v_steps, _TYPES[q.dtype], table.data_ptr(), table.stride(0), width, lengths.data_ptr(), ptr(starts),
         out.data_ptr(), T, B, Hq, Hkv, D, page, k_cache.shape[0], D ** -0.5 if scale is None else float(scale), int(window),
         ptr(ws), nbytes, _lib.stream_of(q)), "paged_attention")
     return out
