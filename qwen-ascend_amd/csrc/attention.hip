@@ -55,7 +55,7 @@ struct AttentionArgs {
   int negate;       // of a scale below 0
   int same_pages;   // 16 keys on 16 lie on one page
   int few;          // FEW, or 0: all sequences take the many-rows form
-  int few_blocks, few_rows, many_tiles, pieces, slots;
+  int few_blocks, few_rows, many_tiles, pieces, slots, join_few;
   float *few_part, *many_part;  // partial sums: rows of D, then pairs (maximum, sum)
 };
 
@@ -220,15 +220,15 @@ struct Rows {
 
   // Scores of keys `first` and so on: those that the row does not see become -inf.
   QMOE_DEV static void mask(f32x16_v (&s)[NJ], Seen seen, uint64_t present, int first) {
-    const int half = (threadIdx.x >> 5) & 1, from = first + 4 * half, low = seen.low - from, high = seen.high - from;
+    const int half = (threadIdx.x >> 5) & 1, from = first + 4 * half;
 #pragma unroll
     for (int j = 0; j < NJ; ++j) {
-      const uint32_t there = (uint32_t)(present >> (32 * j)) >> (4 * half);
+      const int low = seen.low - from - 32 * j, high = seen.high - from - 32 * j;
+      uint32_t bits = (uint32_t)(present >> (32 * j)) >> (4 * half);
+      bits = low > 31 || high < 0 ? 0 : bits & ~0u << max(low, 0) & ~0u >> (31 - min(high, 31));
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int key = key_of(j, r);
-        if (!((there >> (key & 31)) & 1) || key < low || key > high) s[j][r] = -INFINITY;
-      }
+      for (int r = 0; r < 16; ++r)
+        if (!((bits >> (key_of(j, r) & 31)) & 1)) s[j][r] = -INFINITY;
     }
   }
 
@@ -255,24 +255,28 @@ struct Rows {
 // as this wave loaded them); the rows that see them get them after the loop. Returns whether there were any.
 template <typename E, int COUNT>
 QMOE_DEV bool clean(unsigned char* v, int every) {
-  const int lane = threadIdx.x & 63;
-  bool any = false;
+  u32x4_v* at = reinterpret_cast<u32x4_v*>(v) + (threadIdx.x & 63);
+  u32x4_v w[COUNT];
+#pragma unroll
+  for (int g = 0; g < COUNT; ++g) w[g] = at[g * every * 64];
+  uint32_t any = 0;
+#pragma unroll
+  for (int g = 0; g < COUNT; ++g)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) any |= (w[g][i] & Mma<E>::EXPONENT) + Mma<E>::ONE;
+  if (!__any((any & 0x80008000u) != 0)) return false;
 #pragma unroll 1
   for (int g = 0; g < COUNT; ++g) {
-    u32x4_v* at = reinterpret_cast<u32x4_v*>(v + g * every * 1024) + lane;
-    u32x4_v w = *at;
-    uint32_t odd = 0;
+    u32x4_v x = at[g * every * 64];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const uint32_t u = ((w[i] & Mma<E>::EXPONENT) + Mma<E>::ONE) & 0x80008000u;
-      odd |= u;
-      if (u & 0x8000u) w[i] &= 0xffff0000u;
-      if (u & 0x80000000u) w[i] &= 0xffffu;
+      const uint32_t u = (x[i] & Mma<E>::EXPONENT) + Mma<E>::ONE;
+      if (u & 0x8000u) x[i] &= 0xffff0000u;
+      if (u & 0x80000000u) x[i] &= 0xffffu;
     }
-    if (odd) *at = w;
-    any |= odd != 0;
+    at[g * every * 64] = x;
   }
-  return __any(any);
+  return true;
 }
 
 // Elements at, at + 1, .. at + 7 of a row of q.
@@ -861,13 +865,13 @@ __global__ __launch_bounds__(256, (NK <= 4 ? 2 : 1)) void attention_kernel(Atten
 // ---------------------------------------------------------------- joining
 
 // Rows' parts: sums of D and (maximum, sum), `count` of them for a row, part c of row r at at(r, c); rows
-// `from` and so on below `rows`. Up to 64 parts: a wave to a row, 4 JOIN of them at once; more: a
-// workgroup to a row. The parts' scales first, then as many parts at once as threads make rows of D, eight of
+// `from` and so on below `rows`. Up to 64 parts: a wave to a row; more: a workgroup to a row; `slots`
+// workgroups share the rows. The parts' scales first, then as many parts at once as threads make rows of D, eight of
 // them in flight each.
-constexpr int JOIN = 8;  // workgroups that share out the rows of a tile
+constexpr int JOIN = 8, JOIN_FEW = 2;  // workgroups that share out the rows of a tile, of a head of few rows
 constexpr int PARTS_MAX = 520;
 template <typename E, typename At, typename Out>
-QMOE_DEV void join_rows(const float* sums, const float2* tops, At at, int count, int slot, int rows, Out out, int D) {
+QMOE_DEV void join_rows(const float* sums, const float2* tops, At at, int count, int slot, int slots, int rows, Out out, int D) {
   __shared__ float scale[PARTS_MAX], sum_of[4];
   __shared__ __align__(16) f32x4_v part[256];
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
@@ -884,7 +888,7 @@ QMOE_DEV void join_rows(const float* sums, const float2* tops, At at, int count,
       __syncthreads();
     }
   };
-  for (int r = alone ? slot * 4 + wave : slot; r < rows; r += alone ? 4 * JOIN : JOIN) {
+  for (int r = alone ? slot * 4 + wave : slot; r < rows; r += alone ? 4 * slots : slots) {
     float2 t[3];
     float m = -INFINITY, l = 0.f;
 #pragma unroll
@@ -933,18 +937,19 @@ QMOE_DEV void join_rows(const float* sums, const float2* tops, At at, int count,
   }
 }
 
-// Blocks [0, few_blocks) x JOIN: the head inside whose tiles the first boundary is the one between the
+// Blocks [0, few_blocks) x join_few: the head inside whose tiles the first boundary is the one between the
 // shares of block - 1 and block. Behind them, where the many-rows form cuts keys into pieces, JOIN for
 // each tile and head.
 template <typename E>
 __global__ __launch_bounds__(256) void join_kernel(AttentionArgs a) {
   const Batch& batch = a.batch;
-  const int few = a.few_blocks * JOIN, G = a.group.d, block = blockIdx.x < few ? blockIdx.x / JOIN : (blockIdx.x - few) / JOIN;
-  const int slot = (blockIdx.x < few ? blockIdx.x : blockIdx.x - few) % JOIN;
+  const int few = a.few_blocks * a.join_few, G = a.group.d;
+  const bool is_few = (int)blockIdx.x < few;
+  const int slots = is_few ? a.join_few : JOIN, at = is_few ? blockIdx.x : blockIdx.x - few, block = at / slots, slot = at - block * slots;
   const float *sums, *tops;
   int count, rows, row0, h, first;  // rows of the tile; its first token's row and its own first row
   Pieces pieces = {};
-  if ((int)blockIdx.x < few) {
+  if (is_few) {
     if (block == 0) return;
     const FewList list(a);
     const int f = list.share * block;
@@ -970,12 +975,11 @@ __global__ __launch_bounds__(256) void join_kernel(AttentionArgs a) {
     if (count <= 1) return;
     rows = min(ROWS, t.rows - t.r0), row0 = t.row0, first = t.r0;
   }
-  const bool is_few = (int)blockIdx.x < few;
   sums = is_few ? a.few_part : a.many_part;
   tops = reinterpret_cast<const float*>(is_few ? few_tops(a) : many_tops(a));
   join_rows<E>(sums, reinterpret_cast<const float2*>(tops),
                [&](int r, int c) { return is_few ? part_of(block - 1 + c, c == 0) * a.few_rows + r : piece_at(pieces, c) * ROWS + r; },
-               count, slot, rows,
+               count, slot, slots, rows,
                [&](int r) {
                  const int token = a.group.div(first + r);
                  const long row = (long)(row0 + token) * a.Hq + h * G + first + r - token * G;
@@ -1026,7 +1030,7 @@ int launch(const AttentionArgs& a, hipStream_t st) {
   else if (!tiles) hipLaunchKernelGGL((attention_kernel<E, NK, FULL, FEW_ROWS>), grid, threads, 0, st, a);
   else hipLaunchKernelGGL((attention_kernel<E, NK, FULL, MANY | FEW_ROWS>), grid, threads, 0, st, a);
   const int rc = (int)hipGetLastError();
-  const long joins = JOIN * (a.few_blocks + (a.pieces > 1 ? tiles : 0));
+  const long joins = (long)a.few_blocks * a.join_few + (a.pieces > 1 ? tiles * JOIN : 0);
   if (rc || joins == 0) return rc;
   hipLaunchKernelGGL((join_kernel<E>), dim3((unsigned)joins), threads, 0, st, a);
   return (int)hipGetLastError();
@@ -1096,6 +1100,8 @@ int qmoe_paged_attention(const void* q, long q_token, long q_head, const void* k
   a.same_pages = page % 16 == 0;
   a.few = p.few, a.few_blocks = p.few_blocks, a.few_rows = p.few_rows, a.many_tiles = p.many_tiles;
   a.pieces = p.pieces, a.slots = p.slots;
+  // (few heads: parts of a row beyond 64, a workgroup to each row)
+  a.join_few = p.few_blocks > 48l * B * Hkv ? JOIN : JOIN_FEW;
   a.few_part = static_cast<float*>(workspace);
   a.many_part = a.few_part + p.few_floats;
   return type == QMOE_BF16 ? dispatch<ElemBF16>(a, (hipStream_t)stream) : dispatch<ElemF16>(a, (hipStream_t)stream);
