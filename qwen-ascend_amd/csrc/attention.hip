@@ -1005,7 +1005,7 @@ Plan plan_for(int T, int B, int Hq, int Hkv, int D, int page, int width, bool on
   p.few_rows = one_each ? G : FEW;
   p.pieces = 1;
   p.slots = D > 128 ? 256 : 512;  // workgroups that run at once
-  const long most = std::min((long)width * page, 0x7fffffffl);  // keys
+  const long most = (long)width * page;  // keys
   if (few) {
     const long tiles = (long)B * Hkv * (std::max<long>(1, (most + FEW_KEYS - 1) / FEW_KEYS));
     p.few_blocks = (int)std::max(1l, std::min<long>(p.slots, tiles));
@@ -1060,7 +1060,7 @@ bool bad_shape(int T, int B, int Hq, int Hkv, int D) {
 extern "C" {
 
 size_t qmoe_paged_attention_workspace(int T, int B, int Hq, int Hkv, int D, int page, int table_width, int one_each) {
-  if (bad_shape(T, B, Hq, Hkv, D) || page < 1 || table_width < 0) return 0;
+  if (bad_shape(T, B, Hq, Hkv, D) || page < 1 || table_width < 0 || (long)table_width * page > TOKENS_MAX) return 0;
   const Plan p = plan_for(T, B, Hq, Hkv, D, page, table_width, one_each);
   return 4 * (p.few_floats + p.many_floats);
 }
@@ -1073,16 +1073,16 @@ int qmoe_paged_attention(const void* q, long q_token, long q_head, const void* k
   if (bad_shape(T, B, Hq, Hkv, D) || (type != QMOE_BF16 && type != QMOE_F16)) return QMOE_EINVAL;
   constexpr float LOG2E = 1.44269504088896341f;
   if (page < 1 || page > 1 << 30 || n_pages < 0 || table_width < 0 || table_ld < 0 || (!starts && T != B) ||
-      window < 0 || !std::isfinite(scale * LOG2E))
+      window < 0 || window > 1 << 30 || !std::isfinite(scale * LOG2E) || (long)table_width * page > TOKENS_MAX)
     return QMOE_EINVAL;
   if ((k_page | k_slot | k_head | v_page | v_slot | v_head) & 7) return QMOE_EINVAL;
   if ((reinterpret_cast<uintptr_t>(k_cache) | reinterpret_cast<uintptr_t>(v_cache)) & 15) return QMOE_EINVAL;
-  if (T == 0) return QMOE_OK;
-  if (!q || !out || missing(k_cache, v_cache, n_pages, table, table_width, lengths, B)) return QMOE_EINVAL;
   // bytes within a page, from page to page, and the list of the few-rows form are counted in 32 bits
   for (const long step : {k_page, v_page, k_slot * page, v_slot * page, k_head, v_head})
     if (step < 0 || step >= 1l << 30) return QMOE_EINVAL;
-  if ((long)B * Hkv * (std::min((long)table_width * page, 0x7fffffffl) / FEW_KEYS + 1 + LEAD) > 0x7fffff00l) return QMOE_EINVAL;
+  if ((long)B * Hkv * ((long)table_width * page / FEW_KEYS + 1 + LEAD) > 0x7fffff00l) return QMOE_EINVAL;
+  if (T == 0) return QMOE_OK;
+  if (!q || !out || missing(k_cache, v_cache, n_pages, table, table_width, lengths, B)) return QMOE_EINVAL;
   const Plan p = plan_for(T, B, Hq, Hkv, D, page, table_width, !starts);
   if (p.few_floats + p.many_floats &&
       (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15) || workspace_bytes < 4 * (p.few_floats + p.many_floats)))

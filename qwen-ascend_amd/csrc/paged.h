@@ -15,6 +15,9 @@ struct FastDiv {
   QMOE_HOST_DEV uint32_t div(uint32_t n) const { return (uint32_t)((((uint64_t)n * mul) >> 32) + n) >> shift; }
 };
 
+// Positions that a table can name (so that those of whole tiles beyond them are ints too).
+constexpr long TOKENS_MAX = 0x7ffff000l;
+
 // A cache tensor [pages, page, heads, D] as element steps; elements of a head are contiguous.
 struct CacheSteps {
   long page, slot, head;
@@ -43,7 +46,7 @@ struct Batch {
   QMOE_DEV int new_rows(int b) const { return starts ? max(start(b + 1) - start(b), 0) : 1; }
   // Cached tokens of sequence b, as many as its row of the table can hold.
   QMOE_DEV int length(int b) const {
-    const long most = n_pages ? min((long)width * page.d, 0x7fffffffl) : 0;
+    const long most = n_pages ? (long)width * page.d : 0;
     return (int)min(max((long)lengths[b], 0l), most);
   }
   // The page of position p in [0, length(b)), or -1 where the table names none of the cache's.

@@ -183,6 +183,10 @@ int launch_chunks(const RotateArgs& a, hipStream_t st) {
   const int items = a.rd / (2 * C) + (a.D - a.rd + 2 * C - 1) / (2 * C);
   if (items > 256) return launch_units<E, C, 8>(a, st);
   if (items > 64) return launch_units<E, C, 4>(a, st);
+  // Two of 64 where many waves look their tokens' places up (1, 2, 3, 4 of 64, us: 2246 tokens of 32 + 16 heads
+  // of 128 15.3, 14.2, 14.0, 14.5; 64 of 32 + 8 4.6, 4.9, 5.7, 6.2; without places, 8192 of 16 heads
+  // of 256 22.4, 23.4, 23.6, 26.2).
+  if (a.Hkv && (long)a.batch.T * a.heads * items > 64 * 8192) return launch_units<E, C, 2>(a, st);
   return launch_units<E, C, 1>(a, st);
 }
 
@@ -234,7 +238,7 @@ int qmoe_append_kv(const void* k, long k_token, long k_head, const void* v, long
   if (page < 1 || page > 1 << 30 || n_pages < 0 || table_width < 0 || table_ld < 0 || (!starts && T != B))
     return QMOE_EINVAL;
   if ((q == nullptr) != (q_out == nullptr) || (Hq > 0) != (q != nullptr)) return QMOE_EINVAL;
-  if ((long)Hq + 2l * Hkv > 1 << 20) return QMOE_EINVAL;
+  if ((long)Hq + 2l * Hkv > 1 << 20 || (long)table_width * page > TOKENS_MAX) return QMOE_EINVAL;
   if (T == 0) return QMOE_OK;
   if (!k || !v || (rd && !frequencies) || missing(k_cache, v_cache, n_pages, table, table_width, lengths, B)) return QMOE_EINVAL;
   RotateArgs a = {};

@@ -151,8 +151,8 @@ def paged_attention(q, k_cache, v_cache, table, lengths, *, starts=None, scale=N
     if (k_ptr | v_ptr) & 15 or not (contiguous or all(s % 8 == 0 for s in (*k_steps, *v_steps))):
         raise RuntimeError("cached heads must be 16-byte aligned")
     _check_batch(table, lengths, starts, T)
-    if window != int(window) or not 0 <= window < 1 << 31:
-        raise RuntimeError("window must be 0 (none) or a number of tokens")
+    if window != int(window) or not 0 <= window <= 1 << 30:
+        raise RuntimeError("window must be 0 (none) or a number of tokens up to 2^30")
     if not _lib.operands(q, k_cache, v_cache, table, lengths, starts):
         with torch.cuda.device(q.device):
             return paged_attention(q, k_cache, v_cache, table, lengths, starts=starts, scale=scale, window=window)

@@ -157,6 +157,13 @@ def test_large_scores(device, dtype, new):
     assert not paged_attention(q, *caches, table, lens, starts=starts, scale=1.0).any()
 
 
+@pytest.mark.parametrize("new,lengths,Hq,Hkv,D", [([8200], [8200], 32, 8, 64), ([40, 1, 3, 17, 0, 64] * 25, [90, 500, 3, 17, 5, 129] * 25, 4, 2, 128),
+                                                  ([2000, 1000, 3000, 2100], [2000, 1500, 3000, 9000], 32, 8, 64)])
+def test_many_tiles(device, new, lengths, Hq, Hkv, D):
+    """More tiles of rows than run at once, whole; more sequences than lanes."""
+    check(device, new, lengths, 16, Hq, Hkv, D, BF16, seed=5, padding=100)
+
+
 def test_layouts(device):
     """q as a slice of wider rows at any alignment, caches as views, scale 0 and below 0, tables of wider rows."""
     from qmoe import paged_attention

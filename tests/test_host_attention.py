@@ -69,7 +69,7 @@ def attend(x=None, kc=None, vc=None, table=None, lengths=None, **kw):
     (attend(t(3, 4, 36), t(4, 16, 2, 36), t(4, 16, 2, 36)), "multiple of 8"), (attend(t(3, 4, 264)), "multiple of 8"),
     (attend(t(3, 3, 32)), "cannot share"), (attend(t(3, 130, 32)), "cannot share"), (attend(t(3, 0, 32)), "cannot share"),
     (attend(kc=t(4, 16, 64)), "both alike"), (attend(kc=t(5, 16, 2, 32)), "both alike"), (attend(vc=t(4, 16, 2, 32, dtype=F16)), "type"),
-    (attend(window=-1), "window"), (attend(window=1.5), "window"), (attend(window=1 << 31), "window"),
+    (attend(window=-1), "window"), (attend(window=1.5), "window"), (attend(window=(1 << 30) + 1), "window"),
     (attend(lengths=torch.zeros(3)), "lengths must be"), (attend(starts=i(3)), "starts must be"),
     (attend(kc=t(4, 16, 2, 36)[..., :32], vc=t(4, 16, 2, 36)[..., :32]), "16-byte aligned"),
     (attend(kc=t(4 * 16 * 64 + 1)[1:].view(4, 16, 2, 32)), "16-byte aligned"),
@@ -113,7 +113,9 @@ def test_c_entries_refuse_before_any_launch():
     assert attend(T=0) == 0
     for kw in (dict(type=2), dict(T=-1), dict(B=-1), dict(Hq=3), dict(Hq=0), dict(Hkv=0), dict(Hq=130, Hkv=2), dict(D=36), dict(D=264),
                dict(D=0), dict(page=0), dict(pages=-1), dict(scale=math.inf), dict(window=-1), dict(k_slot=60), dict(kc=8),
-               dict(B=3, starts=None), dict(width=-1), dict(ld=-1), dict(Hq=8192, Hkv=4096)):
+               dict(B=3, starts=None), dict(width=-1), dict(ld=-1), dict(Hq=8192, Hkv=4096),
+               dict(window=(1 << 30) + 1), dict(width=1 << 20, page=1 << 11), dict(k_slot=1 << 28), dict(k_slot=-64),
+               dict(B=1 << 20, Hkv=4, width=1 << 20, page=16)):
         assert attend(**kw) == -1 and attend(**{"T": 0, **kw}) == -1, kw
     for kw in (dict(q=None), dict(kc=None), dict(table=None), dict(lengths=None), dict(out=None), dict(T=1 << 30, Hq=4)):
         assert attend(**kw) == -1, kw
