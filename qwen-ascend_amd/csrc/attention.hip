@@ -55,7 +55,7 @@ struct AttentionArgs {
   int negate;       // of a scale below 0
   int same_pages;   // 16 keys on 16 lie on one page
   int few;          // FEW, or 0: all sequences take the many-rows form
-  int few_blocks, few_rows, many_tiles, pieces, slots, join_few;
+  int few_blocks, few_from, few_rows, many_tiles, pieces, slots, join_few;
   float *few_part, *many_part;  // partial sums: rows of D, then pairs (maximum, sum)
 };
 
@@ -64,7 +64,7 @@ QMOE_DEV float2* few_tops(const AttentionArgs& a) {
   return reinterpret_cast<float2*>(a.few_part + 2l * a.few_blocks * a.few_rows * a.D);
 }
 QMOE_DEV float2* many_tops(const AttentionArgs& a) {
-  return reinterpret_cast<float2*>(a.many_part + 2l * (a.slots + 1) * ROWS * a.D);
+  return reinterpret_cast<float2*>(a.many_part + 2l * (2 * a.slots + 1) * ROWS * a.D);
 }
 
 // Inclusive sums over a wave's lanes.
@@ -394,17 +394,22 @@ struct ManyList {
   }
 };
 
-// Where tiles are few, each is cut into pieces of so many 64 keys that all pieces of the call make up about
-// as many as run at once. Tiles of a sequence count alike, with the most keys that one of them may see; in
-// the list of all tiles' keys (sequence, tile, head), a piece that starts in stretch u of that size is kept at
-// 2 u, or 2 u + 1 if it is the first of its tile: a tile in pieces is longer than a stretch, so these differ.
+// Where tiles are few, long ones are cut into pieces. Tiles of a sequence count alike, with the most keys that one
+// of them may see. Where all sequences' tiles are about as long, a piece is the part of all keys that one of the
+// workgroups that run at once gets; else half of it, in tiles of more than two such pieces, so that long
+// tiles do not outlast the rest. Shares and halves, us: 64 new tokens after 32768 70, 90 and after 65536 (heads
+// of 256) 156, 187; 8 sequences of up to 500 after up to 30000 450, 393, heads of 192 1203, 939.
+// In the list of all tiles' keys (sequence, tile, head), a piece that starts in stretch u of a piece's size is
+// kept at 2 u, or 2 u + 1 if it is the first of its tile: a tile in pieces is longer than a stretch, so these
+// differ.
 struct Pieces {
-  int size, start;  // in units of 64 keys: a piece; this tile's start in the list
+  int size, start, cut;  // in units of 64 keys: a piece; this tile's start in the list; tiles up to cut * size are whole
 };
 QMOE_DEV Pieces pieces_of(const AttentionArgs& a, const ManyTile& t, int h) {
   const int lane = threadIdx.x & 63, G = a.group.d;
   const Batch& batch = a.batch;
-  int total = 0, before = 0, of = 0;
+  int total = 0, count = 0, before = 0, of = 0;
+  uint32_t most = 0;
   for (int i = 0; i < batch.B; i += 64) {
     int tiles = 0, keys = 0;
     if (i + lane < batch.B) {
@@ -420,8 +425,15 @@ QMOE_DEV Pieces pieces_of(const AttentionArgs& a, const ManyTile& t, int h) {
     const int mine = tiles * keys * a.Hkv, upto = prefix_sum(mine);
     if (t.b >= i && t.b < i + 64) before = total + lane_of(upto - mine, t.b - i), of = lane_of(keys, t.b - i);
     total += lane_of(upto, 63);
+    count += lane_of(prefix_sum(tiles * a.Hkv), 63);
+    most = max(most, (uint32_t)lane_of((int)wave_max_u32_vec((uint32_t)keys), 0));
   }
-  return {max(8, (total + a.slots - 1) / a.slots), before + (t.r0 / ROWS * a.Hkv + h) * of};
+  const bool alike = 4l * most * count <= 5l * total;
+  const int stretches = alike ? a.slots : 2 * a.slots;
+  return {max(8, (total + stretches - 1) / stretches), before + (t.r0 / ROWS * a.Hkv + h) * of, alike ? 1 : 2};
+}
+QMOE_DEV int piece_count(const AttentionArgs& a, const Pieces& p, int tiles) {
+  return tiles > p.cut * p.size ? min((tiles + p.size - 1) / p.size, a.pieces) : 1;
 }
 QMOE_DEV long piece_at(const Pieces& p, int piece) { return 2l * ((p.start + piece * p.size) / p.size) + (piece == 0); }
 
@@ -447,11 +459,11 @@ QMOE_DEV void many_rows(const AttentionArgs& a, int block, unsigned char* lds) {
   if (a.pieces > 1) {
     if (piece * 8 >= max(mt.tiles, 1)) return;  // no piece is shorter
     pieces = pieces_of(a, mt, h);
-    const int count = min((mt.tiles + pieces.size - 1) / pieces.size, a.pieces);
-    if (piece >= max(count, 1)) return;
+    const int count = piece_count(a, pieces, mt.tiles);
+    if (piece >= count) return;
     cut = count > 1;
-    t0 = piece * pieces.size;
-    if (piece + 1 < count) t1 = t0 + pieces.size;
+    const int each = (mt.tiles + count - 1) / count;
+    t0 = min(piece * each, t1), t1 = min(t0 + each, t1);
   }
   const int G = a.group.d, b = mt.b, row0 = mt.row0, rows = mt.rows, r0 = mt.r0, before = mt.before, begin = mt.begin;
   const int end = min(before + (int)a.group.div(min(r0 + ROWS, rows) - 1) + 1, b < batch.B ? batch.length(b) : 0);
@@ -851,15 +863,17 @@ QMOE_DEV void few_rows(const AttentionArgs& a, int block, unsigned char* lds) {
   }
 }
 
-// Each form by itself, and both in one launch (the few-rows form in the first blocks).
+// Each form by itself, and both in one launch: few rows' equal shares in the last blocks, where they fill what
+// the other form's tiles leave (8 sequences of up to 500 after up to 30000 365 us, 393 in the first), or in the
+// first, where most sequences must be of few rows (16 of up to 5 tokens 24.5 us, 29.9 in the last).
 enum { MANY = 1, FEW_ROWS = 2 };
 template <typename E, int NK, bool FULL, int FORMS>
 __global__ __launch_bounds__(256, (NK <= 4 ? 2 : 1)) void attention_kernel(AttentionArgs a) {
   __shared__ __align__(16) unsigned char lds[Layout<NK>::LDS];
   if constexpr (FORMS == MANY) many_rows<E, NK, FULL>(a, blockIdx.x, lds);
   else if constexpr (FORMS == FEW_ROWS) few_rows<E, NK, FULL>(a, blockIdx.x, lds);
-  else if ((int)blockIdx.x < a.few_blocks) few_rows<E, NK, FULL>(a, blockIdx.x, lds);
-  else many_rows<E, NK, FULL>(a, blockIdx.x - a.few_blocks, lds);
+  else if (blockIdx.x - a.few_from < (unsigned)a.few_blocks) few_rows<E, NK, FULL>(a, blockIdx.x - a.few_from, lds);
+  else many_rows<E, NK, FULL>(a, blockIdx.x - (a.few_from ? 0 : a.few_blocks), lds);
 }
 
 // ---------------------------------------------------------------- joining
@@ -971,7 +985,7 @@ __global__ __launch_bounds__(256) void join_kernel(AttentionArgs a) {
     const ManyTile t = list.find(a, number);
     if (t.r0 < 0 || t.r0 >= t.rows || t.tiles <= 8) return;
     pieces = pieces_of(a, t, h);
-    count = min((t.tiles + pieces.size - 1) / pieces.size, a.pieces);
+    count = piece_count(a, pieces, t.tiles);
     if (count <= 1) return;
     rows = min(ROWS, t.rows - t.r0), row0 = t.row0, first = t.r0;
   }
@@ -1012,11 +1026,13 @@ Plan plan_for(int T, int B, int Hq, int Hkv, int D, int page, int width, bool on
     p.few_floats = 2l * p.few_blocks * p.few_rows * (D + 2);
   }
   if (many) {
-    p.many_tiles = (int)((long)T * G / ROWS) + B + 1;
-    const long items = (((long)T * G + ROWS - 1) / ROWS) * Hkv, units = (most + 63) / 64;
-    if (items < 4 * p.slots && ((long)p.many_tiles * Hkv + p.slots) * (units + 8) < 1l << 31)
+    // a tile for 128 rows, and one more that is not full for each such sequence and for the rows behind the last
+    const long rows = (long)T * G;
+    p.many_tiles = (int)(rows / ROWS + std::min<long>(B, few ? rows / (FEW + 1) : B) + 1);
+    const long items = (rows + ROWS - 1) / ROWS * Hkv, units = (most + 63) / 64;
+    if (items < 4 * p.slots && ((long)p.many_tiles * Hkv + 2 * p.slots) * (units + 8) < 1l << 31)
       p.pieces = (int)std::max<long>(1, std::min({units / 8, (long)PIECES_MAX, std::max(8l, 16l * p.slots / items)}));
-    if (p.pieces > 1) p.many_floats = 2l * (p.slots + 1) * ROWS * (D + 2);
+    if (p.pieces > 1) p.many_floats = 2l * (2 * p.slots + 1) * ROWS * (D + 2);
   }
   return p;
 }
@@ -1024,7 +1040,6 @@ Plan plan_for(int T, int B, int Hq, int Hkv, int D, int page, int width, bool on
 template <typename E, int NK, bool FULL>
 int launch(const AttentionArgs& a, hipStream_t st) {
   const long tiles = (long)a.many_tiles * a.Hkv, blocks = tiles * a.pieces + a.few_blocks;
-  if (blocks > 0x7fffffffl || tiles * JOIN > 0x7ffffffl) return QMOE_EINVAL;
   const dim3 grid((unsigned)blocks), threads(256);
   if (!a.few_blocks) hipLaunchKernelGGL((attention_kernel<E, NK, FULL, MANY>), grid, threads, 0, st, a);
   else if (!tiles) hipLaunchKernelGGL((attention_kernel<E, NK, FULL, FEW_ROWS>), grid, threads, 0, st, a);
@@ -1084,6 +1099,7 @@ int qmoe_paged_attention(const void* q, long q_token, long q_head, const void* k
   if (T == 0) return QMOE_OK;
   if (!q || !out || missing(k_cache, v_cache, n_pages, table, table_width, lengths, B)) return QMOE_EINVAL;
   const Plan p = plan_for(T, B, Hq, Hkv, D, page, table_width, !starts);
+  if ((long)p.many_tiles * Hkv * p.pieces > 0x7fff0000l) return QMOE_EINVAL;
   if (p.few_floats + p.many_floats &&
       (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15) || workspace_bytes < 4 * (p.few_floats + p.many_floats)))
     return QMOE_EWORKSPACE;
@@ -1100,6 +1116,7 @@ int qmoe_paged_attention(const void* q, long q_token, long q_head, const void* k
   a.same_pages = page % 16 == 0;
   a.few = p.few, a.few_blocks = p.few_blocks, a.few_rows = p.few_rows, a.many_tiles = p.many_tiles;
   a.pieces = p.pieces, a.slots = p.slots;
+  a.few_from = (long)T * (Hq / Hkv) <= (long)B * FEW ? 0 : p.many_tiles * Hkv * p.pieces;
   // (few heads: parts of a row beyond 64, a workgroup to each row)
   a.join_few = p.few_blocks > 48l * B * Hkv ? JOIN : JOIN_FEW;
   a.few_part = static_cast<float*>(workspace);
