@@ -55,7 +55,8 @@ struct AttentionArgs {
   int negate;       // of a scale below 0
   int same_pages;   // 16 keys on 16 lie on one page
   int few;          // FEW, or 0: all sequences take the many-rows form
-  int few_blocks, few_from, few_rows, many_tiles, pieces, slots, join_few;
+  int few_blocks, few_from, few_rows, many_tiles, pieces, slots;
+  int join_few, join_many;  // workgroups that share out the rows of a head of few rows, of a tile
   float *few_part, *many_part;  // partial sums: rows of D, then pairs (maximum, sum)
 };
 
@@ -882,7 +883,6 @@ __global__ __launch_bounds__(256, (NK <= 4 ? 2 : 1)) void attention_kernel(Atten
 // `from` and so on below `rows`. Up to 64 parts: a wave to a row; more: a workgroup to a row; `slots`
 // workgroups share the rows. The parts' scales first, then as many parts at once as threads make rows of D, eight of
 // them in flight each.
-constexpr int JOIN = 8, JOIN_FEW = 2;  // workgroups that share out the rows of a tile, of a head of few rows
 constexpr int PARTS_MAX = 520;
 template <typename E, typename At, typename Out>
 QMOE_DEV void join_rows(const float* sums, const float2* tops, At at, int count, int slot, int slots, int rows, Out out, int D) {
@@ -952,14 +952,14 @@ QMOE_DEV void join_rows(const float* sums, const float2* tops, At at, int count,
 }
 
 // Blocks [0, few_blocks) x join_few: the head inside whose tiles the first boundary is the one between the
-// shares of block - 1 and block. Behind them, where the many-rows form cuts keys into pieces, JOIN for
-// each tile and head.
+// shares of block - 1 and block. Behind them, where the many-rows form cuts keys into pieces, join_many
+// for each tile and head.
 template <typename E>
 __global__ __launch_bounds__(256) void join_kernel(AttentionArgs a) {
   const Batch& batch = a.batch;
   const int few = a.few_blocks * a.join_few, G = a.group.d;
   const bool is_few = (int)blockIdx.x < few;
-  const int slots = is_few ? a.join_few : JOIN, at = is_few ? blockIdx.x : blockIdx.x - few, block = at / slots, slot = at - block * slots;
+  const int slots = is_few ? a.join_few : a.join_many, at = is_few ? blockIdx.x : blockIdx.x - few, block = at / slots, slot = at - block * slots;
   const float *sums, *tops;
   int count, rows, row0, h, first;  // rows of the tile; its first token's row and its own first row
   Pieces pieces = {};
@@ -1045,7 +1045,7 @@ int launch(const AttentionArgs& a, hipStream_t st) {
   else if (!tiles) hipLaunchKernelGGL((attention_kernel<E, NK, FULL, FEW_ROWS>), grid, threads, 0, st, a);
   else hipLaunchKernelGGL((attention_kernel<E, NK, FULL, MANY | FEW_ROWS>), grid, threads, 0, st, a);
   const int rc = (int)hipGetLastError();
-  const long joins = (long)a.few_blocks * a.join_few + (a.pieces > 1 ? tiles * JOIN : 0);
+  const long joins = (long)a.few_blocks * a.join_few + (a.pieces > 1 ? tiles * a.join_many : 0);
   if (rc || joins == 0) return rc;
   hipLaunchKernelGGL((join_kernel<E>), dim3((unsigned)joins), threads, 0, st, a);
   return (int)hipGetLastError();
@@ -1117,8 +1117,13 @@ int qmoe_paged_attention(const void* q, long q_token, long q_head, const void* k
   a.few = p.few, a.few_blocks = p.few_blocks, a.few_rows = p.few_rows, a.many_tiles = p.many_tiles;
   a.pieces = p.pieces, a.slots = p.slots;
   a.few_from = (long)T * (Hq / Hkv) <= (long)B * FEW ? 0 : p.many_tiles * Hkv * p.pieces;
-  // (few heads: parts of a row beyond 64, a workgroup to each row)
-  a.join_few = p.few_blocks > 48l * B * Hkv ? JOIN : JOIN_FEW;
+  // few heads: parts of a row beyond 64, a workgroup to each row
+  a.join_few = p.few_blocks > 48l * B * Hkv ? 8 : 2;
+  // Few tiles: most are in pieces, and more workgroups join them sooner; many: most are not, and the workgroups
+  // are in the way. 4, 8, 16, 32 for each, us: 16 tiles 83, 69, 61, 59, 264 189, 177, 171, 176, 707 (none in
+  // pieces) 84, 88, 99, 118.
+  const long items = ((long)T * (Hq / Hkv) + ROWS - 1) / ROWS * Hkv;
+  a.join_many = items <= 32 ? 32 : items <= 384 ? 16 : items <= 640 ? 8 : 4;
   a.few_part = static_cast<float*>(workspace);
   a.many_part = a.few_part + p.few_floats;
   return type == QMOE_BF16 ? dispatch<ElemBF16>(a, (hipStream_t)stream) : dispatch<ElemF16>(a, (hipStream_t)stream);
