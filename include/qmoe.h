@@ -429,7 +429,7 @@ int qmoe_token_logprobs(const void* logits, long ld, int type, const void* token
  *      [B]: its tokens, the new ones among them; table int32 [B, table_width], rows table_ld apart:
  *      entry p / page names the page of position p. An entry outside [0, n_pages) is no page, and
  *      positions past the table have none. Nothing is read or written out of range whatever
- *      these hold; two tokens must not be stored at one place. */
+ *      these hold; two tokens must not be stored at one place. table_width * page is at most 0x7ffff000. */
 /* The first rd elements of every head turned by its token's position, the rest copied. Pair i is
  * (x[i], x[i + rd/2]), or (x[2i], x[2i+1]) for interleaved; frequencies: uint64 [rd/2], turns per
  * position times 2^64; cosine and sine are multiplied by `turn`. positions [T]: int32, or int64
@@ -454,8 +454,10 @@ int qmoe_append_kv(const void* k, long k_token, long k_head, const void* v, long
  * to `type` for the product with v). Query heads [h G, h G + G) share key head h, G = Hq / Hkv <= 64.
  * A row that sees no key, or only scores of -inf, and every row behind the last sequence gives 0;
  * what lies at places that a row does not see (NaN too) does not reach it. QMOE_BF16 or QMOE_F16; D <= 256 a
- * multiple of 8, cache steps too, caches 16-byte aligned. Workspace: qmoe_paged_attention_workspace()
- * bytes for the call's own sizes, 16-byte aligned (one_each: starts is NULL). */
+ * multiple of 8, cache steps too, caches 16-byte aligned; k_page, v_page, page * k_slot and page * v_slot
+ * below 2^30 elements, window at most 2^30, Hq at most 4096. Workspace: qmoe_paged_attention_workspace() bytes for the
+ * call's own sizes, up to about 140 MB, 16-byte aligned (one_each: starts is NULL); calls that may overlap need
+ * one each. */
 size_t qmoe_paged_attention_workspace(int T, int B, int Hq, int Hkv, int D, int page, int table_width, int one_each);
 int qmoe_paged_attention(const void* q, long q_token, long q_head, const void* k_cache, long k_page, long k_slot,
                          long k_head, const void* v_cache, long v_page, long v_slot, long v_head, int type,

@@ -41,6 +41,7 @@ typedef __attribute__((address_space(1))) const void global_void;
 constexpr int ROWS = 128;      // rows of a workgroup, many-rows form
 constexpr int FEW = 32;        // rows up to which a sequence takes the few-rows form
 constexpr int FEW_KEYS = 128;  // keys of a tile of that form
+constexpr int FEW_BLOCKS_MAX = 768;  // workgroups of that form, and parts of a row
 constexpr int D_MAX = 256, GROUP_MAX = 64;
 
 struct AttentionArgs {
@@ -132,7 +133,7 @@ struct Layout {
   QMOE_DEV static int v_swizzle(int row) { return DP == 64 ? 4 * ((row >> 1) & 1) : 4 * (row & 3); }
 };
 
-// The keys that a lane's row sees: [low, high], those present in the tile.
+// A lane's row sees the keys [low, high], of those that are present in a tile.
 struct Seen {
   int low, high;
 };
@@ -438,6 +439,17 @@ QMOE_DEV int piece_count(const AttentionArgs& a, const Pieces& p, int tiles) {
 }
 QMOE_DEV long piece_at(const Pieces& p, int piece) { return 2l * ((p.start + piece * p.size) / p.size) + (piece == 0); }
 
+// A workgroup: 128 rows against one piece of their keys, 64 at a time. K and V come to LDS by DMA, both
+// halves of a double buffer, and serve four waves of 32 rows, so that a CU's two workgroups draw 128 KB of
+// tiles for 256 rows' products; with heads of up to 128 two waves a SIMD hold q, the output's sums and the
+// scores in 256 registers each. What bounds it is issue: of a step of 64 keys (heads of 128) a wave
+// spends 4345 clocks, 1024 of them in its own 32 MFMAs, the rest in sharing the matrix pipe with the other
+// wave of its SIMD (busy 38 %), in the weights (224 vector operations a tile; the vector pipe is busy 40 %)
+// and in 450 at the wait and the barrier. 8192 tokens of 32 + 8 heads of 128, bf16: 590 us, 933 TFLOP/s, where a large
+// product reaches 1235. Not faster there, us (in turn with what was there then): K loaded a tile further ahead
+// than V (spills), instruction groups in fixed order 611 to 620 (606), wave priorities 632 (621), three
+// waves a SIMD over a single V buffer 819 (601), loads spread over the step 584 to 591 (580). Eight waves on
+// 256 rows 588 (604), which leaves fewer workgroups where rows are few.
 template <typename E, int NK, bool FULL>
 QMOE_DEV void many_rows(const AttentionArgs& a, int block, unsigned char* lds) {
   using L = Layout<NK>;
@@ -678,6 +690,12 @@ struct FewList {
 // it ends with and one that it goes on with.
 QMOE_DEV long part_of(int block, bool begins) { return 2l * block + (begins ? 1 : 0); }
 
+// A workgroup: its share of the list, tile by tile of 128 keys, each of its four waves 32 of them against all (up
+// to 32) rows, K and V loaded to the wave's own quarter of LDS, so that waves meet only where a head ends. Each
+// key is read once for all query heads of its group: bound by memory. 64 single tokens after up to 65536 (8 heads
+// of 128, 1.29 GB) 247 us, 5.2 TB/s, 4 after 131072 (2 heads of 256, 1.07 GB) 190 us, 5.6; a kernel that
+// only reads the same pages reached 5.6 to 6.0. 1 after 4096: 10 us, latency (a table entry, a key, sums), and 6
+// to join its parts.
 template <typename E, int NK, bool FULL>
 QMOE_DEV void few_rows(const AttentionArgs& a, int block, unsigned char* lds) {
   using L = Layout<NK>;
@@ -883,10 +901,10 @@ __global__ __launch_bounds__(256, (NK <= 4 ? 2 : 1)) void attention_kernel(Atten
 // `from` and so on below `rows`. Up to 64 parts: a wave to a row; more: a workgroup to a row; `slots`
 // workgroups share the rows. The parts' scales first, then as many parts at once as threads make rows of D, eight of
 // them in flight each.
-constexpr int PARTS_MAX = 520;
+static_assert(FEW_BLOCKS_MAX <= 3 * 256);
 template <typename E, typename At, typename Out>
 QMOE_DEV void join_rows(const float* sums, const float2* tops, At at, int count, int slot, int slots, int rows, Out out, int D) {
-  __shared__ float scale[PARTS_MAX], sum_of[4];
+  __shared__ float scale[FEW_BLOCKS_MAX], sum_of[4];
   __shared__ __align__(16) f32x4_v part[256];
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   const bool alone = count <= 64;  // a wave by itself
@@ -1022,7 +1040,9 @@ Plan plan_for(int T, int B, int Hq, int Hkv, int D, int page, int width, bool on
   const long most = (long)width * page;  // keys
   if (few) {
     const long tiles = (long)B * Hkv * (std::max<long>(1, (most + FEW_KEYS - 1) / FEW_KEYS));
-    p.few_blocks = (int)std::max(1l, std::min<long>(p.slots, tiles));
+    // Heads of 64 by themselves leave registers and LDS for three workgroups on a CU (4 tokens after 65536 128 us
+    // with two, 108 with three, 64 after up to 16384 83, 78); beside the other form's tiles they gain nothing.
+    p.few_blocks = (int)std::max(1l, std::min<long>(D == 64 && !many ? FEW_BLOCKS_MAX : p.slots, tiles));
     p.few_floats = 2l * p.few_blocks * p.few_rows * (D + 2);
   }
   if (many) {

@@ -67,6 +67,9 @@ struct Chunk {
 // U x 64 items of its heads, an item being two chunks of C elements that turn together (or are
 // copied); it has all its loads in flight while it works out the token's angles, a pair per lane,
 // which its lanes then share through LDS.
+// 8192 tokens of 16 heads of 256, 64 elements turned, 134 MB: 22.4 us, 6.0 TB/s (caches included); 2246 tokens of
+// 32 + 16 heads of 128 into a cache, 55 MB: 14.2 us, 3.9 TB/s, as a token's place is looked up before its
+// stores. Few tokens by launch and latency: one of 32 heads 2.9 us, 64 of 32 + 8 into a cache 4.5.
 template <typename E, int C, int U>
 __global__ __launch_bounds__(256) void rotate_kernel(RotateArgs a) {
   using raw = typename E::raw;

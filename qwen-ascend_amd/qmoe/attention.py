@@ -7,10 +7,10 @@ An attention layer calls, between its projections (q, k, v may be views of one p
 
 The caches are [pages, page, Hkv, D]. A batch of B sequences is described on the device, so a
 captured graph follows it: ``table`` int32 [B, width] names the page of positions [i * page, (i + 1) *
-page) of a sequence (an entry outside the cache, as -1, is no page); ``lengths`` int32 [B] counts its
-tokens with the new ones; ``starts`` int32 [B + 1], ascending from 0: rows [starts[b], starts[b + 1]) are
-its new tokens, the last ones of it. Without ``starts`` each sequence has one new token. Rows
-behind the last sequence are padding. HIP kernels ``qmoe_append_kv`` and ``qmoe_paged_attention`` of
+page) of a sequence (an entry outside the cache, as -1, is no page; width * page is at most 2^31 -
+4096); ``lengths`` int32 [B] counts its tokens with the new ones; ``starts`` int32 [B + 1], ascending
+from 0: rows [starts[b], starts[b + 1]) are its new tokens, the last ones of it. Without ``starts``
+each sequence has one new token. Rows behind the last sequence are padding. HIP kernels ``qmoe_append_kv`` and ``qmoe_paged_attention`` of
 libqmoe.so. Forward only: a tensor that requires a gradient is refused while gradients are
 recorded, and one with a forward-mode tangent.
 """
@@ -130,7 +130,7 @@ def paged_attention(q, k_cache, v_cache, table, lengths, *, starts=None, scale=N
     The caches hold the new tokens' keys and values too (:func:`append_kv`). The row of a token at
     position p sees the keys up to p, with a ``window`` > 0 only the last ``window`` of them, and
     none without a page. bfloat16 or float16; D <= 256 a multiple of 8; query heads [h G, (h + 1) G) share
-    key head h, G = Hq / Hkv <= 64. ``scale``: D^-0.5 if not given. Scores, softmax and the output's sums are
+    key head h, G = Hq / Hkv <= 64. A page of a cache spans fewer than 2^30 elements. ``scale``: D^-0.5 if not given. Scores, softmax and the output's sums are
     fp32; the weights e^(s - m) are rounded to q's type for their product with the values, each
     output once. A row that sees no key, or whose scores are all -inf, gives 0, and so do rows behind
     the last sequence; what lies at a place that a row does not see, NaN too, does not reach it."""
@@ -166,7 +166,8 @@ def paged_attention(q, k_cache, v_cache, table, lengths, *, starts=None, scale=N
     ws = q.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
     ptr = _lib.ptr
     _lib.check(L.qmoe_paged_attention(
-        q.data_ptr(), q_token, q_head, k_ptr, *k_steps, v_ptr, *v_steps, _TYPES[q.dtype], table.data_ptr(), table.stride(0), width, lengths.data_ptr(), ptr(starts),
+        q.data_ptr(), q_token, q_head, k_ptr, *k_steps, v_ptr, *v_steps, _TYPES[q.dtype], table.data_ptr(),
+        table.stride(0), width, lengths.data_ptr(), ptr(starts),
         out.data_ptr(), T, B, Hq, Hkv, D, page, k_cache.shape[0], D ** -0.5 if scale is None else float(scale), int(window),
         ptr(ws), nbytes, _lib.stream_of(q)), "paged_attention")
     return out

@@ -44,6 +44,13 @@ def test_single_tokens_long(device, lengths, Hq, Hkv, D):
     check(device, [1] * len(lengths), lengths, 16, Hq, Hkv, D, BF16, seed=len(lengths))
 
 
+@pytest.mark.parametrize("lengths", [[99000], [131072], [60000, 1, 45000]])
+@pytest.mark.parametrize("Hq,Hkv", [(8, 1), (1, 1), (6, 3)])
+def test_single_tokens_many_parts(device, lengths, Hq, Hkv):
+    """Heads of 64, one head's keys over nearly all workgroups."""
+    check(device, [1] * len(lengths), lengths, 64, Hq, Hkv, 64, BF16)
+
+
 @pytest.mark.parametrize("Hq,Hkv,D", SHAPES)
 @pytest.mark.parametrize("dtype,window", [(BF16, 0), (F16, 0), (BF16, 9), (F16, 130)])
 def test_several(device, Hq, Hkv, D, dtype, window):
