@@ -126,9 +126,11 @@ QMOE_DEV float half_sum(float v) {
 // each, rows of V 64 bytes each.
 template <int NK>
 struct Layout {
-  static constexpr int DC = 32 * NK, DP = NK <= 2 ? 64 : NK <= 4 ? 128 : 256, STRIDE = 2 * DP;
+  static constexpr int DC = 32 * NK, D_LEAST = NK == 2 ? 8 : NK == 3 ? 72 : NK == 4 ? 104 : NK == 6 ? 136 : 200;
+  static constexpr int DP = NK <= 2 ? 64 : NK <= 4 ? 128 : 256, STRIDE = 2 * DP;
   static constexpr int PIECES = DP / 8, RPI = 64 / PIECES;  // rows of a wave's load instruction
   static constexpr int TILE = 64 * STRIDE, LDS = 4 * TILE;
+  QMOE_DEV static constexpr bool always(int ks) { return 16 * ks + 15 < D_LEAST; }  // within every such head
   QMOE_DEV static int k_swizzle(int row) { return DP == 64 ? (row >> 1) & 7 : DP == 128 ? row & 15 : row & 7; }
   QMOE_DEV static int v_swizzle(int row) { return DP == 64 ? 4 * ((row >> 1) & 1) : 4 * (row & 3); }
 };
@@ -303,15 +305,19 @@ QMOE_DEV long read_lane(long v, int src) {
 }
 
 // COUNT runs of rows, one 16-byte piece per lane, straight to LDS: run g is rows src + g * EVERY of the
-// tile, whose offsets the lanes hold, to `to` + 1 KB * g * EVERY / RPI. Lanes past the head's elements load nothing
-// (FULL: there are none). A row that is not there is skipped, or zeroed. `run`: 16 rows on 16 lie one step
+// tile, whose offsets the lanes hold, to `to` + 1 KB * g * EVERY / RPI. Lanes past the head's elements load its
+// last piece again (FULL: there are none): such values of V only reach sums that are not stored, those of K are made 0 where
+// they are read. A load to LDS without some of its lanes takes several times as long. A row that is not there is skipped, or zeroed. `run`: 16 rows on 16 lie one step
 // apart, so that an offset of each 16, as a scalar, does for all of them.
 template <int NK, bool FULL, int COUNT, int EVERY, bool KEYS>
 QMOE_DEV void load_rows(unsigned char* to, const unsigned char* base, long offset, uint64_t present, bool whole, bool run,
                         int src, uint32_t step, int D) {
   using L = Layout<NK>;
   const int lane = threadIdx.x & 63, row = lane / L::PIECES;
-  auto piece_of = [&](int mine) { return (lane % L::PIECES) ^ (KEYS ? L::k_swizzle(mine) : L::v_swizzle(mine)); };
+  auto piece_of = [&](int mine) {
+    const int piece = (lane % L::PIECES) ^ (KEYS ? L::k_swizzle(mine) : L::v_swizzle(mine));
+    return FULL ? piece : min(piece, D / 8 - 1);
+  };
   if (whole && run) {
 #pragma unroll
     for (int g = 0; g < COUNT; ++g) {
@@ -320,9 +326,8 @@ QMOE_DEV void load_rows(unsigned char* to, const unsigned char* base, long offse
       uint64_t p = reinterpret_cast<uint64_t>(base) + read_lane(offset, from & ~15) + (from & 15) * step;
       asm volatile("" : "+s"(p));
       const int piece = piece_of(from + row);
-      if (FULL || 8 * piece < D)
-        __builtin_amdgcn_global_load_lds((global_void*)(p + (row * step + 16u * piece)),
-                                         (lds_void*)(to + g * (1024 * EVERY / L::RPI)), 16, 0, 0);
+      __builtin_amdgcn_global_load_lds((global_void*)(p + (row * step + 16u * piece)),
+                                       (lds_void*)(to + g * (1024 * EVERY / L::RPI)), 16, 0, 0);
     }
   } else {
 #pragma unroll 1
@@ -330,12 +335,10 @@ QMOE_DEV void load_rows(unsigned char* to, const unsigned char* base, long offse
       const int mine = src + g * EVERY + row, piece = piece_of(mine);
       unsigned char* at = to + g * (1024 * EVERY / L::RPI);
       const long from = __shfl(offset, mine);
-      if (FULL || 8 * piece < D) {
-        if ((present >> mine) & 1)
-          __builtin_amdgcn_global_load_lds((global_void*)(base + from + 16 * piece), (lds_void*)at, 16, 0, 0);
-        else if (!KEYS)
-          *reinterpret_cast<u32x4_v*>(at + 16 * lane) = (u32x4_v){0, 0, 0, 0};
-      }
+      if ((present >> mine) & 1)
+        __builtin_amdgcn_global_load_lds((global_void*)(base + from + 16 * piece), (lds_void*)at, 16, 0, 0);
+      else if (!KEYS)
+        *reinterpret_cast<u32x4_v*>(at + 16 * lane) = (u32x4_v){0, 0, 0, 0};
     }
   }
 }
@@ -520,10 +523,6 @@ QMOE_DEV void many_rows(const AttentionArgs& a, int block, unsigned char* lds) {
     return present;
   };
 
-  if (!FULL) {  // the elements behind a head's
-    for (int i = threadIdx.x; i < L::LDS / 16; i += 256) reinterpret_cast<u32x4_v*>(lds)[i] = (u32x4_v){0, 0, 0, 0};
-    __syncthreads();
-  }
   __shared__ int unusual;
   if (threadIdx.x == 0) unusual = 0;  // (before the first barrier of the loop, after which it may be set)
   __syncthreads();
@@ -558,8 +557,9 @@ QMOE_DEV void many_rows(const AttentionArgs& a, int block, unsigned char* lds) {
       for (int i = 0; i < 16; ++i) s[j][0][i] = 0.f;
 #pragma unroll
       for (int ks = 0; ks < 2 * NK; ++ks) {
-        const s16x8_v f = *reinterpret_cast<const s16x8_v*>(now + k_base + 32 * j * L::STRIDE + 16 * ((2 * ks + half) ^ k_swizzle));
-        s[j][0] = Mma<E>::mma(f, q[ks], s[j][0]);
+        u32x4_v f = *reinterpret_cast<const u32x4_v*>(now + k_base + 32 * j * L::STRIDE + 16 * ((2 * ks + half) ^ k_swizzle));
+        if (!(FULL || L::always(ks) || 16 * ks + 8 * half < a.D)) f = (u32x4_v){0, 0, 0, 0};
+        s[j][0] = Mma<E>::mma(__builtin_bit_cast(s16x8_v, f), q[ks], s[j][0]);
       }
     };
     const bool whole = present == ~0ull && first + 63 <= wave_first && (!a.window || first > wave_last - a.window);
@@ -741,7 +741,7 @@ QMOE_DEV void few_rows(const AttentionArgs& a, int block, unsigned char* lds) {
     Rows<E, NK, 1> acc;
     acc.clear();
 
-    const unsigned char* kb = static_cast<const unsigned char*>(a.k) + 2 * h * a.kc.head + 16 * half;
+    const unsigned char* kb = static_cast<const unsigned char*>(a.k) + 2 * h * a.kc.head;
     const unsigned char* vb = static_cast<const unsigned char*>(a.v) + 2 * h * a.vc.head;
     const int* table = batch.table + b * batch.table_ld;
     auto first_of = [&](int x) { return keys.begin + FEW_KEYS * x + 32 * wave; };
@@ -750,24 +750,21 @@ QMOE_DEV void few_rows(const AttentionArgs& a, int block, unsigned char* lds) {
       return x < x1 && key < keys.end ? table[batch.page.div(key)] : -1;
     };
     unsigned char* mine = lds + wave * 64 * L::STRIDE;  // two times 32 rows of V
+    auto within = [&](int ks) { return FULL || L::always(ks) || 16 * ks + 8 * half < a.D; };
     // K's rows go straight to registers (lane & 31 is the row of the first operand), V's to LDS
     s16x8_v k[2 * NK];
     auto load_k = [&](int x, int entry) {
       // (a key without a page: the cache's first, left out by its score)
       const unsigned char* row = kb + row_offset(a.kc, batch.page, entry, first_of(x) + (lane & 31));
-      if (FULL) {
 #pragma unroll
-        for (int ks = 0; ks < 2 * NK; ++ks) k[ks] = *reinterpret_cast<const s16x8_v*>(row + 32 * ks);
-      } else {
-#pragma unroll
-        for (int ks = 0; ks < 2 * NK; ++ks) {
-          const bool in = 16 * ks + 8 * half < a.D;
-          u32x4_v w = *reinterpret_cast<const u32x4_v*>(in ? row + 32 * ks : row);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) w[i] = in ? w[i] : 0;
-          k[ks] = __builtin_bit_cast(s16x8_v, w);
-        }
-      }
+      for (int ks = 0; ks < 2 * NK; ++ks) k[ks] = *reinterpret_cast<const s16x8_v*>(row + (within(ks) ? 32 * ks + 16 * half : 0));
+    };
+    // The elements behind a head's: others of its row, made 0 where they are used, as at the load that would
+    // wait for them.
+    auto key_part = [&](int ks) {
+      u32x4_v w = __builtin_bit_cast(u32x4_v, k[ks]);
+      if (!within(ks)) w = (u32x4_v){0, 0, 0, 0};
+      return __builtin_bit_cast(s16x8_v, w);
     };
     auto load_v = [&](int x, int entry, uint64_t present, unsigned char* to) {
       const long vo = row_offset(a.vc, batch.page, entry, first_of(x) + (lane & 31));
@@ -801,8 +798,8 @@ QMOE_DEV void few_rows(const AttentionArgs& a, int block, unsigned char* lds) {
       for (int i = 0; i < 16; ++i) s[0][i] = 0.f;
 #pragma unroll
       for (int ks = 0; ks < 2 * NK; ++ks) {
-        if constexpr (NK > 4) s[0] = Mma<E>::mma(k[ks], q_lds[ks * 64 + lane], s[0]);
-        else s[0] = Mma<E>::mma(k[ks], q[ks], s[0]);
+        if constexpr (NK > 4) s[0] = Mma<E>::mma(key_part(ks), q_lds[ks * 64 + lane], s[0]);
+        else s[0] = Mma<E>::mma(key_part(ks), q[ks], s[0]);
       }
       // The next keys take these registers (behind the last tile: the first row of the cache; a branch around
       // the loads would cost a wait for them where it ends).
