@@ -305,10 +305,12 @@ QMOE_DEV long read_lane(long v, int src) {
 }
 
 // COUNT runs of rows, one 16-byte piece per lane, straight to LDS: run g is rows src + g * EVERY of the
-// tile, whose offsets the lanes hold, to `to` + 1 KB * g * EVERY / RPI. Lanes past the head's elements load its
-// last piece again (FULL: there are none): such values of V only reach sums that are not stored, those of K are made 0 where
-// they are read. A load to LDS without some of its lanes takes several times as long. A row that is not there is skipped, or zeroed. `run`: 16 rows on 16 lie one step
-// apart, so that an offset of each 16, as a scalar, does for all of them.
+// tile, whose offsets the lanes hold, to `to` + 1 KB * g * EVERY / RPI. Lanes past a head's elements (FULL: there are
+// none) load its last piece again, as a load to LDS without some of its lanes takes several times as long (32 tokens
+// after up to 16384, 8 heads of 80: 226 us, so 62): such values of V only reach sums that are not stored, those
+// of K are made 0 where they are read. A row that is not there is skipped, or zeroed; the cache's first row in
+// its place, for all such rows of all tiles, took longer (8 sequences of up to 500 after up to 30000 369 us, 412).
+// `run`: 16 rows on 16 lie one step apart, so that an offset of each 16, as a scalar, does for all of them.
 template <int NK, bool FULL, int COUNT, int EVERY, bool KEYS>
 QMOE_DEV void load_rows(unsigned char* to, const unsigned char* base, long offset, uint64_t present, bool whole, bool run,
                         int src, uint32_t step, int D) {
@@ -448,7 +450,7 @@ QMOE_DEV long piece_at(const Pieces& p, int piece) { return 2l * ((p.start + pie
 // scores in 256 registers each. What bounds it is issue: of a step of 64 keys (heads of 128) a wave
 // spends 4345 clocks, 1024 of them in its own 32 MFMAs, the rest in sharing the matrix pipe with the other
 // wave of its SIMD (busy 38 %), in the weights (224 vector operations a tile; the vector pipe is busy 40 %)
-// and in 450 at the wait and the barrier. 8192 tokens of 32 + 8 heads of 128, bf16: 590 us, 933 TFLOP/s, where a large
+// and in 450 at the wait and the barrier. 8192 tokens of 32 + 8 heads of 128, bf16: 584 us, 941 TFLOP/s, where a large
 // product reaches 1235. Not faster there, us (in turn with what was there then): K loaded a tile further ahead
 // than V (spills), instruction groups in fixed order 611 to 620 (606), wave priorities 632 (621), three
 // waves a SIMD over a single V buffer 819 (601), loads spread over the step 584 to 591 (580). Eight waves on
