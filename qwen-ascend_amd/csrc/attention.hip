@@ -442,7 +442,11 @@ QMOE_DEV Pieces pieces_of(const AttentionArgs& a, const ManyTile& t, int h) {
 QMOE_DEV int piece_count(const AttentionArgs& a, const Pieces& p, int tiles) {
   return tiles > p.cut * p.size ? min((tiles + p.size - 1) / p.size, a.pieces) : 1;
 }
-QMOE_DEV long piece_at(const Pieces& p, int piece) { return 2l * ((p.start + piece * p.size) / p.size) + (piece == 0); }
+// (within the workspace also where sequences share rows against the rules, and their sums pass 32 bits)
+QMOE_DEV long piece_at(const AttentionArgs& a, const Pieces& p, int piece) {
+  const uint32_t stretch = ((uint32_t)p.start + (uint32_t)piece * (uint32_t)p.size) / (uint32_t)p.size;
+  return 2l * min(stretch, 2u * a.slots) + (piece == 0);
+}
 
 // A workgroup: 128 rows against one piece of their keys, 64 at a time. K and V come to LDS by DMA, both
 // halves of a double buffer, and serve four waves of 32 rows, so that a CU's two workgroups draw 128 KB of
@@ -609,7 +613,7 @@ QMOE_DEV void many_rows(const AttentionArgs& a, int block, unsigned char* lds) {
   const float l = half_sum(acc.l);
   if (!valid) return;
   if (cut) {
-    const long at = piece_at(pieces, piece) * ROWS + 32 * wave + (lane & 31);
+    const long at = piece_at(a, pieces, piece) * ROWS + 32 * wave + (lane & 31);
     if (half == 0) many_tops(a)[at] = make_float2(acc.m, l);
     float* to = a.many_part + at * a.D;
 #pragma unroll
@@ -1009,7 +1013,7 @@ __global__ __launch_bounds__(256) void join_kernel(AttentionArgs a) {
   sums = is_few ? a.few_part : a.many_part;
   tops = reinterpret_cast<const float*>(is_few ? few_tops(a) : many_tops(a));
   join_rows<E>(sums, reinterpret_cast<const float2*>(tops),
-               [&](int r, int c) { return is_few ? part_of(block - 1 + c, c == 0) * a.few_rows + r : piece_at(pieces, c) * ROWS + r; },
+               [&](int r, int c) { return is_few ? part_of(block - 1 + c, c == 0) * a.few_rows + r : piece_at(a, pieces, c) * ROWS + r; },
                count, slot, slots, rows,
                [&](int r) {
                  const int token = a.group.div(first + r);

@@ -175,3 +175,24 @@ def test_workspace(device):
         assert call(need) == 0
         assert torch.equal(out, paged_attention(q, *caches, table, lens, starts=None if one else starts))
         assert (ws[need:] == 171).all()
+
+
+@pytest.mark.parametrize("times,tokens,before", [(2, 300, 3000), (2500, 4096, 61440)])
+def test_starts_out_of_order(device, times, tokens, before):
+    """Sequences that share rows against the rules, once with more keys in all than 32 bits count: results mean nothing
+    then, but nothing is written outside of the output, and a call that keeps to the rules is right afterwards."""
+    from qmoe import paged_attention
+    log(f"starts out of order: {times} x {tokens}")
+    Hq, Hkv, D, page = 32, 8, 64, 64
+    n = normal(device, 5)
+    caches = [n(2, page, Hkv, D, dtype=torch.float16) for _ in range(2)]
+    B = 2 * times - 1
+    table = torch.zeros((B, (tokens + before) // page), dtype=torch.int32, device=device)
+    lens = torch.full((B,), tokens + before, dtype=torch.int32, device=device)
+    starts = torch.tensor([0, tokens] * times, dtype=torch.int32, device=device)
+    q = n(tokens, Hq, D, dtype=torch.float16)
+    assert paged_attention(q, *caches, table, lens, starts=starts).shape == q.shape
+    torch.cuda.synchronize()
+    few = torch.tensor([0, 40], dtype=torch.int32, device=device)
+    out = paged_attention(q[:40], *caches, table[:1], lens[:1], starts=few)
+    assert_close(out, *A.attention(q[:40], *caches, table[:1], lens[:1], few), "attention")
