@@ -409,8 +409,11 @@ struct ManyList {
 // In the list of all tiles' keys (sequence, tile, head), a piece that starts in stretch u of a piece's size is
 // kept at 2 u, or 2 u + 1 if it is the first of its tile: a tile in pieces is longer than a stretch, so these
 // differ.
+// 64 keys on 64 that are sooner done in one go than in pieces (joining takes as long as 10 of heads of 128; 128 tokens
+// after 1300)
+__host__ QMOE_DEV constexpr int whole_tiles(int D) { return D > 128 ? 12 : 24; }
 struct Pieces {
-  int size, start, cut;  // in units of 64 keys: a piece; this tile's start in the list; tiles up to cut * size are whole
+  int size, start, whole;  // in units of 64 keys: a piece; this tile's start in the list; tiles up to that length are not cut
 };
 QMOE_DEV Pieces pieces_of(const AttentionArgs& a, const ManyTile& t, int h) {
   const int lane = threadIdx.x & 63, G = a.group.d;
@@ -437,10 +440,11 @@ QMOE_DEV Pieces pieces_of(const AttentionArgs& a, const ManyTile& t, int h) {
   }
   const bool alike = 4l * most * count <= 5l * total;
   const int stretches = alike ? a.slots : 2 * a.slots;
-  return {max(8, (total + stretches - 1) / stretches), before + (t.r0 / ROWS * a.Hkv + h) * of, alike ? 1 : 2};
+  const int size = max(8, (total + stretches - 1) / stretches);
+  return {size, before + (t.r0 / ROWS * a.Hkv + h) * of, max(alike ? size : 2 * size, whole_tiles(a.D))};
 }
 QMOE_DEV int piece_count(const AttentionArgs& a, const Pieces& p, int tiles) {
-  return tiles > p.cut * p.size ? min((tiles + p.size - 1) / p.size, a.pieces) : 1;
+  return tiles > p.whole ? min((tiles + p.size - 1) / p.size, a.pieces) : 1;
 }
 // (within the workspace also where sequences share rows against the rules, and their sums pass 32 bits)
 QMOE_DEV long piece_at(const AttentionArgs& a, const Pieces& p, int piece) {
@@ -1004,7 +1008,7 @@ __global__ __launch_bounds__(256) void join_kernel(AttentionArgs a) {
     const ManyList list(a);
     if (number >= list.total) return;
     const ManyTile t = list.find(a, number);
-    if (t.r0 < 0 || t.r0 >= t.rows || t.tiles <= 8) return;
+    if (t.r0 < 0 || t.r0 >= t.rows || t.tiles <= whole_tiles(a.D)) return;
     pieces = pieces_of(a, t, h);
     count = piece_count(a, pieces, t.tiles);
     if (count <= 1) return;
@@ -1031,7 +1035,7 @@ struct Plan {
   size_t few_floats, many_floats;
 };
 constexpr int PIECES_MAX = 64;
-Plan plan_for(int T, int B, int Hq, int Hkv, int D, int page, int width, bool one_each) {
+Plan plan_for(int T, int B, int Hq, int Hkv, int D, int page, int width, int window, bool one_each) {
   const int G = Hq / Hkv;
   Plan p = {};
   const bool many = one_each ? G > FEW : (long)T * G > FEW;  // may there be sequences of many rows
@@ -1052,9 +1056,20 @@ Plan plan_for(int T, int B, int Hq, int Hkv, int D, int page, int width, bool on
     // a tile for 128 rows, and one more that is not full for each such sequence and for the rows behind the last
     const long rows = (long)T * G;
     p.many_tiles = (int)(rows / ROWS + std::min<long>(B, few ? rows / (FEW + 1) : B) + 1);
-    const long items = (rows + ROWS - 1) / ROWS * Hkv, units = (most + 63) / 64;
-    if (items < 4 * p.slots && ((long)p.many_tiles * Hkv + 2 * p.slots) * (units + 8) < 1l << 31)
-      p.pieces = (int)std::max<long>(1, std::min({units / 8, (long)PIECES_MAX, std::max(8l, 16l * p.slots / items)}));
+    const long items = (rows + ROWS - 1) / ROWS * Hkv;
+    const long units = (most + 63) / 64, seen = window ? std::min(units, (window + ROWS / G + 127l) / 64) : units;
+    // What pieces may save, in steps of a workgroup. One sequence: up to a tile on each workgroup, what all of them
+    // are short of the longest; more tiles, longest first, what the last round of the shortest is short of workgroups.
+    // us in pieces and whole: prompts of 1024 54, 34, of 2048 74, 64, of 4096 187, 164; 256 tokens after 2048 39, 61,
+    // 1024 after 8192 197, 226. (A window never adds pieces: the workspace is asked for without it.)
+    auto gain = [&](long longest, long shortest) {
+      if (B > 1) return longest;
+      return items <= p.slots ? longest - items * (longest + shortest) / (2 * p.slots)
+                              : shortest * ((p.slots - items % p.slots) % p.slots) / p.slots;
+    };
+    const long gains = std::min(gain(units, std::max(units - T / 64, 0l)), window ? gain(seen, seen) : units);
+    if (items < 4 * p.slots && gains > whole_tiles(D) && ((long)p.many_tiles * Hkv + 2 * p.slots) * (units + 8) < 1l << 31)
+      p.pieces = (int)std::max<long>(1, std::min({seen / 8, (long)PIECES_MAX, std::max(8l, 16l * p.slots / items)}));
     if (p.pieces > 1) p.many_floats = 2l * (2 * p.slots + 1) * ROWS * (D + 2);
   }
   return p;
@@ -1099,7 +1114,7 @@ extern "C" {
 
 size_t qmoe_paged_attention_workspace(int T, int B, int Hq, int Hkv, int D, int page, int table_width, int one_each) {
   if (bad_shape(T, B, Hq, Hkv, D) || page < 1 || table_width < 0 || (long)table_width * page > TOKENS_MAX) return 0;
-  const Plan p = plan_for(T, B, Hq, Hkv, D, page, table_width, one_each);
+  const Plan p = plan_for(T, B, Hq, Hkv, D, page, table_width, 0, one_each);
   return 4 * (p.few_floats + p.many_floats);
 }
 
@@ -1121,7 +1136,7 @@ int qmoe_paged_attention(const void* q, long q_token, long q_head, const void* k
   if ((long)B * Hkv * ((long)table_width * page / FEW_KEYS + 1 + LEAD) > 0x7fffff00l) return QMOE_EINVAL;
   if (T == 0) return QMOE_OK;
   if (!q || !out || missing(k_cache, v_cache, n_pages, table, table_width, lengths, B)) return QMOE_EINVAL;
-  const Plan p = plan_for(T, B, Hq, Hkv, D, page, table_width, !starts);
+  const Plan p = plan_for(T, B, Hq, Hkv, D, page, table_width, window, !starts);
   if ((long)p.many_tiles * Hkv * p.pieces > 0x7fff0000l) return QMOE_EINVAL;
   if (p.few_floats + p.many_floats &&
       (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15) || workspace_bytes < 4 * (p.few_floats + p.many_floats)))

@@ -196,3 +196,15 @@ def test_starts_out_of_order(device, times, tokens, before):
     few = torch.tensor([0, 40], dtype=torch.int32, device=device)
     out = paged_attention(q[:40], *caches, table[:1], lens[:1], starts=few)
     assert_close(out, *A.attention(q[:40], *caches, table[:1], lens[:1], few), "attention")
+
+
+@pytest.mark.parametrize("T,before,window", [(6000, 0, 4096), (3000, 0, 2000), (2600, 20000, 3000), (300, 9000, 0), (300, 9000, 5000),
+                                             (2100, 3000, 0)])
+def test_workspace_with_windows(device, T, before, window):
+    """One sequence, tiles in pieces or whole: the workspace, which is asked for without the window, is enough."""
+    from qmoe import paged_attention
+    log(f"window {window}: {T} after {before}")
+    caches, table, lens, starts = batch(device, 3, [T], [T + before], 16, 2, 64, BF16)
+    q = normal(device, 4)(T, 20, 64, std=2.0, dtype=BF16)
+    out = paged_attention(q, *caches, table, lens, starts=starts, window=window)
+    assert_close(out, *A.attention(q, *caches, table, lens, starts, None, window), "attention")
