@@ -409,9 +409,11 @@ struct ManyList {
 // In the list of all tiles' keys (sequence, tile, head), a piece that starts in stretch u of a piece's size is
 // kept at 2 u, or 2 u + 1 if it is the first of its tile: a tile in pieces is longer than a stretch, so these
 // differ.
-// 64 keys on 64 that are sooner done in one go than in pieces (joining takes as long as 10 of heads of 128; 128 tokens
-// after 1300)
-__host__ QMOE_DEV constexpr int whole_tiles(int D) { return D > 128 ? 12 : 24; }
+// Tiles of up to that many times 64 keys are sooner done in one go than in pieces and a joining launch. us whole and
+// in pieces: heads of 128, a prompt of 1024 (16) 34, 54, 64 tokens after 1024 (17) 32, 29, 256 after 2048 (36) 61, 39;
+// heads of 256, whose steps take twice as long, a prompt of 2048 (saves 16 at most) 109, 118, 64 tokens after
+// 1100 (19) 65, 45.
+__host__ QMOE_DEV constexpr int whole_tiles(int D) { return D > 128 ? 16 : 24; }
 struct Pieces {
   int size, start, whole;  // in units of 64 keys: a piece; this tile's start in the list; tiles up to that length are not cut
 };
