@@ -20,6 +20,7 @@
 //    share out the keys, 32 each at a time. All keys of all such sequences and heads make one list
 //    of tiles of 128, of which every workgroup takes an equal share, however the lengths differ.
 // What lies in pieces or crosses shares is joined by a second launch.
+#include "attention_layout.h"
 #include "paged.h"
 
 #include <algorithm>
@@ -120,20 +121,6 @@ QMOE_DEV float half_sum(float v) {
   const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
-
-// Heads of up to 32 * NK elements. In LDS rows are DP elements apart; the 16-byte pieces of a row are XOR'd with
-// its number, so that what one instruction reads of many rows spreads over the banks: rows of K one piece
-// each, rows of V 64 bytes each.
-template <int NK>
-struct Layout {
-  static constexpr int DC = 32 * NK, D_LEAST = NK == 2 ? 8 : NK == 3 ? 72 : NK == 4 ? 104 : NK == 6 ? 136 : 200;
-  static constexpr int DP = NK <= 2 ? 64 : NK <= 4 ? 128 : 256, STRIDE = 2 * DP;
-  static constexpr int PIECES = DP / 8, RPI = 64 / PIECES;  // rows of a wave's load instruction
-  static constexpr int TILE = 64 * STRIDE, LDS = 4 * TILE;
-  QMOE_DEV static constexpr bool always(int ks) { return 16 * ks + 15 < D_LEAST; }  // within every such head
-  QMOE_DEV static int k_swizzle(int row) { return DP == 64 ? (row >> 1) & 7 : DP == 128 ? row & 15 : row & 7; }
-  QMOE_DEV static int v_swizzle(int row) { return DP == 64 ? 4 * ((row >> 1) & 1) : 4 * (row & 3); }
-};
 
 // A lane's row sees the keys [low, high], of those that are present in a tile.
 struct Seen {
@@ -305,10 +292,10 @@ QMOE_DEV long read_lane(long v, int src) {
 }
 
 // COUNT runs of rows, one 16-byte piece per lane, straight to LDS: run g is rows src + g * EVERY of the
-// tile, whose offsets the lanes hold, to `to` + 1 KB * g * EVERY / RPI. Lanes past a head's elements (FULL: there are
-// none) load its last piece again, as a load to LDS without some of its lanes takes several times as long (32 tokens
+// tile, whose offsets the lanes hold, to `to` + 1 KB * g * EVERY / RPI. Lanes past a head's elements
+// load its last piece again, as a load to LDS without some of its lanes takes several times as long (32 tokens
 // after up to 16384, 8 heads of 80: 226 us, so 62): such values of V only reach sums that are not stored, those
-// of K are made 0 where they are read. A row that is not there is skipped, or zeroed; the cache's first row in
+// of K are made 0 where they are read, or not read. A row that is not there is skipped, or zeroed; the cache's first row in
 // its place, for all such rows of all tiles, took longer (8 sequences of up to 500 after up to 30000 369 us, 412).
 // `run`: 16 rows on 16 lie one step apart, so that an offset of each 16, as a scalar, does for all of them.
 template <int NK, bool FULL, int COUNT, int EVERY, bool KEYS>
@@ -316,10 +303,7 @@ QMOE_DEV void load_rows(unsigned char* to, const unsigned char* base, long offse
                         int src, uint32_t step, int D) {
   using L = Layout<NK>;
   const int lane = threadIdx.x & 63, row = lane / L::PIECES;
-  auto piece_of = [&](int mine) {
-    const int piece = (lane % L::PIECES) ^ (KEYS ? L::k_swizzle(mine) : L::v_swizzle(mine));
-    return FULL ? piece : min(piece, D / 8 - 1);
-  };
+  auto piece_of = [&](int mine) { return L::template piece_of<FULL, KEYS>(lane, mine, D); };
   if (whole && run) {
 #pragma unroll
     for (int g = 0; g < COUNT; ++g) {
@@ -1098,10 +1082,12 @@ int launch_heads(const AttentionArgs& a, hipStream_t st) {
 
 template <typename E>
 int dispatch(const AttentionArgs& a, hipStream_t st) {
-  if (a.D <= 64) return launch_heads<E, 2>(a, st);
-  if (a.D <= 96) return launch_heads<E, 3>(a, st);
-  if (a.D <= 128) return launch_heads<E, 4>(a, st);
-  if (a.D <= 192) return launch_heads<E, 6>(a, st);
+  switch (blocks_of(a.D)) {
+    case 2: return launch_heads<E, 2>(a, st);
+    case 3: return launch_heads<E, 3>(a, st);
+    case 4: return launch_heads<E, 4>(a, st);
+    case 6: return launch_heads<E, 6>(a, st);
+  }
   return launch_heads<E, 8>(a, st);
 }
 
