@@ -202,3 +202,19 @@ def test_planted_mistakes_are_seen():
     for w in wrong:
         with pytest.raises(AssertionError):
             R.assert_close(w.to(BF16), want, bound, "planted")
+
+
+def test_list_of_few_rows_fits_32_bits():
+    """Places of the list of single tokens' keys, with the up to 768 that equal shares are rounded up by, stay below
+    2^31: the C entry refuses more (a call that it takes asks for its workspace, before any launch)."""
+    from qmoe import _lib
+
+    def attend(B, tiles):  # tiles of 128 keys that a table names, two places a head beside them, and one more tile
+        return _lib.lib().qmoe_paged_attention(16, 128, 32, 16, 128 * 32, 32, 32, 16, 128 * 32, 32, 32, 0, 16, tiles, tiles, 16, None,
+                                               16, B, B, 1, 1, 32, 128, 3, 1.0, 0, None, 0, None)
+    most = 2 ** 31 - 1 - 768
+    B = 256
+    fits = most // B - 3
+    assert B * (fits + 1 + 3) <= 0x7fffff00  # within a rounder limit
+    assert attend(B, fits) == -2 and attend(B, fits + 1) == -1
+    assert attend(1 << 22, 1) == -2 and attend(1 << 22, 512) == -1
