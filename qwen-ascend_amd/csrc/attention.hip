@@ -615,6 +615,7 @@ QMOE_DEV void many_rows(const AttentionArgs& a, int block, unsigned char* lds) {
       }
     return;
   }
+  if (l == 0.f) acc.clear();  // (also of a sum that a weight of 0 made NaN)
   const float inv = l == 0.f ? 0.f : 1.f / l;
   uint16_t* to = static_cast<uint16_t*>(a.out) + row * a.D;
 #pragma unroll
@@ -860,6 +861,7 @@ QMOE_DEV void few_rows(const AttentionArgs& a, int block, unsigned char* lds) {
         total += l_of[w][at] * (m_of[w][at] == best ? 1.f : __builtin_amdgcn_exp2f(m_of[w][at] - best));
       }
       if (alone) {
+        if (total == 0.f) sum = (f32x4_v){0.f, 0.f, 0.f, 0.f};
         const float inv = total == 0.f ? 0.f : 1.f / total;
         const int tok = a.group.div(at);
         const long row = (long)(row0 + tok) * a.Hq + h * G + at - tok * G;
@@ -955,6 +957,7 @@ QMOE_DEV void join_rows(const float* sums, const float2* tops, At at, int count,
     meet();
     if (tid < quads) {
       for (int c = 1; c < streams; ++c) o += parts[c * quads + tid];
+      if (l == 0.f) o = (f32x4_v){0.f, 0.f, 0.f, 0.f};
       const float inv = l == 0.f ? 0.f : 1.f / l;
       reinterpret_cast<uint2*>(out(r))[tid] = make_uint2(Mma<E>::pack(o[0] * inv, o[1] * inv), Mma<E>::pack(o[2] * inv, o[3] * inv));
     }
