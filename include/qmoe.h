@@ -452,8 +452,9 @@ int qmoe_append_kv(const void* k, long k_token, long k_head, const void* v, long
  * with j > p - window) that lie on a page; out [T, Hq, D], contiguous, = sum e^(s_j - m) v_j / sum
  * e^(s_j - m), s_j = scale q.k_j, m = max s_j, in fp32 with one rounding (and the e^(s_j - m) rounded
  * to `type` for the product with v). Query heads [h G, h G + G) share key head h, G = Hq / Hkv <= 64.
- * A row that sees no key, or only scores of -inf, whatever the values, and every row behind the last sequence gives 0;
- * what lies at places that a row does not see (NaN too) does not reach it. QMOE_BF16 or QMOE_F16; D <= 256 a
+ * A row that sees no key, or only scores of -inf, and every row behind the last sequence gives 0, whatever the
+ * values; else an infinite value that it sees gives an infinity, or, as 0 times it, NaN where its key's score is
+ * -inf or its weight too small for `type`. What lies at places that a row does not see (NaN too) does not reach it. QMOE_BF16 or QMOE_F16; D <= 256 a
  * multiple of 8, cache steps too, caches 16-byte aligned; k_page, v_page, page * k_slot and page * v_slot
  * below 2^30 elements, window at most 2^30, Hq at most 4096. Workspace: qmoe_paged_attention_workspace() bytes for the
  * call's own sizes, up to about 155 MB, 16-byte aligned (one_each: starts is NULL); calls that may overlap need

@@ -81,6 +81,16 @@ QMOE_DEV int prefix_sum(int v) {
   return v;
 }
 QMOE_DEV int lane_of(int v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
+// A byte offset of lane `src` (wave-uniform) as a scalar.
+QMOE_DEV long read_lane(long v, int src) {
+  const uint32_t lo = __builtin_amdgcn_readlane((int)v, src), hi = __builtin_amdgcn_readlane((int)(v >> 32), src);
+  return (long)(((uint64_t)hi << 32) | lo);
+}
+// What lanes of a wave write to LDS, for the others of it.
+QMOE_DEV void wave_fence() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
 
 template <typename E>
 struct Mma;
@@ -223,21 +233,58 @@ struct Rows {
     }
   }
 
-  // The infinite and NaN values of one key, which were left out of its tile: o += v where the row sees it.
-  // v: its value row.
-  QMOE_DEV void add_unusual(const unsigned char* v, bool sees, int D) {
-    const int half = (threadIdx.x >> 5) & 1;
+  // The infinite and NaN values of 32 keys, which were left out of their tile: o += p v where the row sees the key (a
+  // bit of `there` each, the first one key `first`), p its weight, rounded as in whole tiles, so that a score of -inf
+  // gives NaN here as there. k + ko and v + vo: the row of key `lane & 31`; q(ks): the second operand of K Q^T;
+  // w: 4 KB of LDS that only this wave uses.
+  template <typename Q>
+  QMOE_DEV void add_unusual(const unsigned char* k, long ko, const unsigned char* v, long vo, uint32_t there, int first, Seen seen,
+                            float scale, Q q, float* w, int D) {
+    int lane = threadIdx.x & 63;
+    asm volatile("" : "+v"(lane));  // (no registers for sums of it, and below for loads ahead: the loop before needs them)
+    const int half = lane >> 5;
+    f32x16_v s;
 #pragma unroll
-    for (int dt = 0; dt < NK; ++dt)
+    for (int r = 0; r < 16; ++r) s[r] = 0.f;
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        const s16x4_v x = *reinterpret_cast<const s16x4_v*>(v + 2 * min(32 * dt + 8 * c + 4 * half, D - 4));
+    for (int ks = 0; ks < 2 * NK; ++ks) {
+      const bool within = L::always(ks) || 16 * ks + 8 * half < D;
+      u32x4_v f = *reinterpret_cast<const u32x4_v*>(k + ko + (within ? 32 * ks + 16 * half : 0));
+      if (!within) f = (u32x4_v){0, 0, 0, 0};
+      s = Mma<E>::mma(__builtin_bit_cast(s16x8_v, f), q(ks), s);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    const float base = m == -INFINITY ? 0.f : m;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float f = E::load((uint16_t)x[e]);
-          if (sees && !(f - f == 0.f)) o[dt][4 * c + e] += f;
+    for (int r = 0; r < 16; ++r) {
+      const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], scale, -base));
+      w[(key_of(0, r) + 4 * half) * 32 + (lane & 31)] = E::load((uint16_t)Mma<E>::pack(p, p));
+    }
+    wave_fence();
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll 1
+    for (int i = 0; i < 32; ++i) {
+      if (!((there >> i) & 1)) continue;
+      const unsigned char* row = v + read_lane(vo, i);
+      const bool sees = first + i >= seen.low && first + i <= seen.high;
+      const float p = sees ? w[i * 32 + (lane & 31)] : 0.f;
+      int last = D - 4;
+      asm volatile("" : "+s"(last));  // no offsets kept over the loop
+#pragma unroll
+      for (int dt = 0; dt < NK; ++dt) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const s16x4_v x = *reinterpret_cast<const s16x4_v*>(row + 2 * min(32 * dt + 8 * c + 4 * half, last));
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float f = E::load((uint16_t)x[e]);
+            o[dt][4 * c + e] += sees && !(f - f == 0.f) ? p * f : 0.f;
+          }
         }
+        __builtin_amdgcn_sched_barrier(0);
       }
+    }
+    wave_fence();
   }
 };
 
@@ -283,12 +330,6 @@ QMOE_DEV s16x8_v q_piece(const uint16_t* row, int at, int D, bool valid, int neg
 // Positions of a sequence's rows, as ints: what precedes its first new token, clamped.
 QMOE_DEV int tokens_before(const Batch& batch, int b, int n) {
   return (int)max((long)batch.lengths[b] - n, -0x40000000l);
-}
-
-// A byte offset of lane `src` (wave-uniform) as a scalar.
-QMOE_DEV long read_lane(long v, int src) {
-  const uint32_t lo = __builtin_amdgcn_readlane((int)v, src), hi = __builtin_amdgcn_readlane((int)(v >> 32), src);
-  return (long)(((uint64_t)hi << 32) | lo);
 }
 
 // COUNT runs of rows, one 16-byte piece per lane, straight to LDS: run g is rows src + g * EVERY of the
@@ -584,18 +625,19 @@ QMOE_DEV void many_rows(const AttentionArgs& a, int block, unsigned char* lds) {
     step(tile, now, next);
   }
   __syncthreads();
-  if (unusual) {
+  if (__builtin_expect(unusual, 0)) {
     for (int tile = t0; tile < t1; ++tile) {
       int e = entry_of(tile);
       if (e >= batch.n_pages) e = -1;
       const uint64_t present = __ballot(e >= 0);
       if (!partial(tile, present)) continue;
-      const long vo = row_offset(a.vc, batch.page, e, begin + 64 * tile + lane);
+      const int key = begin + 64 * tile + lane;
+      const long ko = row_offset(a.kc, batch.page, e, key), vo = row_offset(a.vc, batch.page, e, key);
 #pragma unroll 1
-      for (int i = 0; i < 64; ++i) {
-        const int key = begin + 64 * tile + i;
-        const bool sees = ((present >> i) & 1) && key >= seen.low && key <= seen.high;
-        acc.add_unusual(vb + ((present >> i) & 1 ? read_lane(vo, i) : 0), sees, FULL ? L::DC : a.D);
+      for (int j = 0; j < 2; ++j) {
+        const int from = 32 * j + (lane & 31);
+        acc.add_unusual(kb, __shfl(ko, from), vb, __shfl(vo, from), (uint32_t)(present >> (32 * j)), begin + 64 * tile + 32 * j, seen,
+                        a.scale, [&](int ks) { return q[ks]; }, reinterpret_cast<float*>(lds) + 1024 * wave, FULL ? L::DC : a.D);
       }
     }
   }
@@ -815,18 +857,15 @@ QMOE_DEV void few_rows(const AttentionArgs& a, int block, unsigned char* lds) {
       if (!whole(x, present) && clean<E, 32 / L::RPI>(v, 1)) unusual = true;
       step(x, v, next);
     }
-    if (unusual) {
+    if (__builtin_expect(unusual, 0)) {
       for (int x = x0; x < x1; ++x) {
         const int e = known(entry_of(x));
         const uint64_t there = __ballot(e >= 0);
         if (whole(x, there)) continue;
-        const long vo = row_offset(a.vc, batch.page, e, first_of(x) + (lane & 31));
-#pragma unroll 1
-        for (int i = 0; i < 32; ++i) {
-          const int key = first_of(x) + i;
-          const bool sees = ((there >> i) & 1) && key >= seen.low && key <= seen.high;
-          acc.add_unusual(vb + ((there >> i) & 1 ? read_lane(vo, i) : 0), sees, FULL ? L::DC : a.D);
-        }
+        const int key = first_of(x) + (lane & 31);
+        acc.add_unusual(kb, row_offset(a.kc, batch.page, e, key), vb, row_offset(a.vc, batch.page, e, key), (uint32_t)there,
+                        first_of(x), seen, a.scale, [&](int ks) { return NK > 4 ? q_lds[ks * 64 + lane] : q[NK > 4 ? 0 : ks]; },
+                        reinterpret_cast<float*>(mine), FULL ? L::DC : a.D);
       }
     }
 
@@ -908,12 +947,8 @@ QMOE_DEV void join_rows(const float* sums, const float2* tops, At at, int count,
   float* scales = alone ? scale + 64 * wave : scale;
   f32x4_v* parts = alone ? part + 64 * wave : part;
   auto meet = [&] {
-    if (alone) {
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-      __builtin_amdgcn_wave_barrier();
-    } else {
-      __syncthreads();
-    }
+    if (alone) wave_fence();
+    else __syncthreads();
   };
   for (int r = alone ? slot * 4 + wave : slot; r < rows; r += alone ? 4 * slots : slots) {
     float2 t[3];
@@ -935,9 +970,9 @@ QMOE_DEV void join_rows(const float* sums, const float2* tops, At at, int count,
 #pragma unroll
     for (int i = 0; i < 3; ++i)
       if ((i == 0 || !alone) && tid + 256 * i < count) {
-        const float f = t[i].y == 0.f ? 0.f : t[i].x == m ? 1.f : __builtin_amdgcn_exp2f(t[i].x - m);
+        const float f = t[i].x == m ? 1.f : __builtin_amdgcn_exp2f(t[i].x - m);
         scales[tid + 256 * i] = f;
-        l += t[i].y == 0.f ? 0.f : t[i].y * f;
+        l += t[i].y * f;
       }
     l = wave_sum_f32(l);
     if (!alone && lane == 0) sum_of[wave] = l;
@@ -951,7 +986,7 @@ QMOE_DEV void join_rows(const float* sums, const float2* tops, At at, int count,
         for (int i = 0; i < 8; ++i) x[i] = reinterpret_cast<const f32x4_v*>(sums + at(r, min(c + i * streams, count - 1)) * D)[quad];
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-          if (c + i * streams < count && scales[c + i * streams] != 0.f) o += x[i] * scales[c + i * streams];
+          if (c + i * streams < count) o += x[i] * scales[c + i * streams];
       }
     parts[tid] = o;
     meet();

@@ -133,7 +133,9 @@ def paged_attention(q, k_cache, v_cache, table, lengths, *, starts=None, scale=N
     key head h, G = Hq / Hkv <= 64. A page of a cache spans fewer than 2^30 elements. ``scale``: D^-0.5 if not given. Scores, softmax and the output's sums are
     fp32; the weights e^(s - m) are rounded to q's type for their product with the values, each
     output once. A row that sees no key, or whose scores are all -inf, gives 0, and so do rows behind
-    the last sequence; what lies at a place that a row does not see, NaN too, does not reach it."""
+    the last sequence; else an infinite value that it sees gives an infinity, or, as 0 times it, NaN where the key's
+    score is -inf or its weight too small for the type. What lies at a place that a row does not see, NaN
+    too, does not reach it."""
     if q.dtype not in (torch.bfloat16, torch.float16) or q.dim() != 3:
         raise RuntimeError("q must be [T, Hq, D] in bfloat16 or float16")
     T, Hq, D = q.shape
