@@ -63,6 +63,14 @@ struct Chunk {
   }
 };
 
+// (a cos - b sin, b cos + a sin), with one rounding order for all forms of the kernel: a head's bits then do not
+// depend on how many tokens a call has.
+QMOE_DEV void turn_pair(float& a, float& b, float c, float s) {
+  const float as = a * s;
+  a = __builtin_fmaf(a, c, -(b * s));
+  b = __builtin_fmaf(b, c, as);
+}
+
 // Memory bound: each element is read and written once. A wave takes one token and up to
 // U x 64 items of its heads, an item being two chunks of C elements that turn together (or are
 // copied); it has all its loads in flight while it works out the token's angles, a pair per lane,
@@ -134,15 +142,17 @@ __global__ __launch_bounds__(256) void rotate_kernel(RotateArgs a) {
       if (!a.interleaved || C == 1) {
 #pragma unroll
         for (int i = 0; i < C; ++i) {
-          const float f = E::load(x[u].e[i]), g = E::load(y[u].e[i]);
-          x[u].e[i] = E::store(f * c[i] - g * s[i]);
-          y[u].e[i] = E::store(g * c[i] + f * s[i]);
+          float f = E::load(x[u].e[i]), g = E::load(y[u].e[i]);
+          turn_pair(f, g, c[i], s[i]);
+          x[u].e[i] = E::store(f);
+          y[u].e[i] = E::store(g);
         }
       } else {
         auto turn = [&](raw& lo, raw& hi, int i) {
-          const float f = E::load(lo), g = E::load(hi);
-          lo = E::store(f * c[i] - g * s[i]);
-          hi = E::store(g * c[i] + f * s[i]);
+          float f = E::load(lo), g = E::load(hi);
+          turn_pair(f, g, c[i], s[i]);
+          lo = E::store(f);
+          hi = E::store(g);
         };
 #pragma unroll
         for (int i = 0; i < C / 2; ++i) turn(x[u].e[2 * i], x[u].e[2 * i + 1], i);
