@@ -14,6 +14,7 @@
 namespace {
 
 constexpr int D_MAX = 1024;
+constexpr unsigned GRID_X = 1 << 20;  // workgroups in a row of the grid: a dimension's threads are counted in 32 bits
 
 struct HeadRows {  // rows [T, heads, D]: element steps of a token and of a head
   const void* p;
@@ -83,9 +84,9 @@ __global__ __launch_bounds__(256) void rotate_kernel(RotateArgs a) {
   using raw = typename E::raw;
   __shared__ float cosine[4][D_MAX / 2], sine[4][D_MAX / 2];
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  const int unit = blockIdx.x * 4 + wave;
-  if (unit >= a.units) return;
-  const int t = a.groups.div(unit), first = (unit - t * (int)a.groups.d) * a.per_unit;
+  const unsigned unit = (blockIdx.y * GRID_X + blockIdx.x) * 4 + wave;
+  if (unit >= (unsigned)a.units) return;
+  const int t = a.groups.div(unit), first = ((int)unit - t * (int)a.groups.d) * a.per_unit;
   const int count = min(a.per_unit, a.heads - first) * (int)a.items.d;
 
   Chunk<E, C> x[U], y[U];
@@ -186,7 +187,8 @@ int launch_units(RotateArgs a, hipStream_t st) {
   const long units = (long)a.batch.T * groups;
   if (units > 0x7ffffff0l) return QMOE_EINVAL;
   a.units = (int)units;
-  hipLaunchKernelGGL((rotate_kernel<E, C, U>), dim3(host_ceil_div(units, 4)), dim3(256), 0, st, a);
+  const unsigned blocks = host_ceil_div(units, 4);
+  hipLaunchKernelGGL((rotate_kernel<E, C, U>), dim3(std::min(blocks, GRID_X), host_ceil_div(blocks, GRID_X)), dim3(256), 0, st, a);
   return (int)hipGetLastError();
 }
 

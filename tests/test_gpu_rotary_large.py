@@ -35,3 +35,43 @@ def test_bits_do_not_depend_on_the_call(device, heads, D, rd, dtype, layout):
     p = torch.arange(T, device=device)
     assert torch.equal(rotate(q, p, r), results[0][0])
     assert torch.equal(torch.cat([rotate(q[i:i + 7], p[i:i + 7], r) for i in range(0, 70, 7)]), results[0][0][:70])
+
+
+T = (1 << 26) + 5  # tokens of one head of 8, 64 threads each: past 2^32 in all
+STEP = 1 << 24
+
+
+def tokens(device, seed):
+    n = normal(device, seed)
+    return torch.cat([n(min(STEP, T - at), 1, 8) for at in range(0, T, STEP)])
+
+
+def test_rotate_past_a_row_of_the_grid(device):
+    from qmoe import Rotary, rotate
+    log(f"rotate T={T}")
+    x, p = tokens(device, 1), torch.arange(T, dtype=torch.int32, device=device)
+    for layout in ("half", "interleaved"):
+        r = Rotary(8, layout=layout, device=device)
+        out = rotate(x, p, r)
+        for at in range(0, T, STEP):
+            assert torch.equal(out[at:at + STEP], rotate(x[at:at + STEP], p[at:at + STEP], r)), at
+    assert rotate(x, p, r, inplace=True) is x and torch.equal(x, out)
+
+
+def test_append_past_a_row_of_the_grid(device):
+    from qmoe import Rotary, append_kv, rotate
+    log(f"append T={T}")
+    page = 4096
+    pages = -(-T // page)
+    k, v = tokens(device, 2), tokens(device, 3)
+    k_cache, v_cache = (torch.zeros((pages, page, 1, 8), dtype=torch.bfloat16, device=device) for _ in range(2))
+    table = torch.arange(pages, dtype=torch.int32, device=device)[None]
+    lengths = torch.tensor([T], dtype=torch.int32, device=device)
+    starts = torch.tensor([0, T], dtype=torch.int32, device=device)
+    r = Rotary(8, device=device)
+    q = append_kv(k, v, k_cache, v_cache, table, lengths, starts=starts, rotary=r, q=k)
+    p = torch.arange(T, dtype=torch.int32, device=device)
+    for at in range(0, T, STEP):
+        assert torch.equal(q[at:at + STEP], rotate(k[at:at + STEP], p[at:at + STEP], r)), at
+    assert torch.equal(k_cache.flatten(0, 1)[:T], q) and torch.equal(v_cache.flatten(0, 1)[:T], v)
+    assert not k_cache.flatten(0, 1)[T:].any()
