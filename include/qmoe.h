@@ -456,9 +456,9 @@ int qmoe_append_kv(const void* k, long k_token, long k_head, const void* v, long
  * values; else an infinite value that it sees gives an infinity, or, as 0 times it, NaN where its key's score is
  * -inf or its weight too small for `type`. What lies at places that a row does not see (NaN too) does not reach it. QMOE_BF16 or QMOE_F16; D <= 256 a
  * multiple of 8, cache steps too, caches 16-byte aligned; k_page, v_page, page * k_slot and page * v_slot
- * below 2^30 elements, window at most 2^30, Hq at most 4096. Workspace: qmoe_paged_attention_workspace() bytes for the
- * call's own sizes, up to about 155 MB, 16-byte aligned (one_each: starts is NULL); calls that may overlap need
- * one each. */
+ * below 2^30 elements, window at most 2^30, Hq at most 4096, T Hq below 2^31; with starts, T Hq / 128 + (B + 1) Hkv
+ * below 2^24 - 768. Workspace: qmoe_paged_attention_workspace() bytes for the call's own sizes, up to about 155 MB,
+ * 16-byte aligned (one_each: starts is NULL); calls that may overlap need one each. */
 size_t qmoe_paged_attention_workspace(int T, int B, int Hq, int Hkv, int D, int page, int table_width, int one_each);
 int qmoe_paged_attention(const void* q, long q_token, long q_head, const void* k_cache, long k_page, long k_slot,
                          long k_head, const void* v_cache, long v_page, long v_slot, long v_head, int type,

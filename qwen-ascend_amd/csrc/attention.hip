@@ -1164,7 +1164,8 @@ int qmoe_paged_attention(const void* q, long q_token, long q_head, const void* k
   if (T == 0) return QMOE_OK;
   if (!q || !out || missing(k_cache, v_cache, n_pages, table, table_width, lengths, B)) return QMOE_EINVAL;
   const Plan p = plan_for(T, B, Hq, Hkv, D, page, table_width, window, !starts);
-  if ((long)p.many_tiles * Hkv * p.pieces > 0x7fff0000l) return QMOE_EINVAL;
+  // a grid holds fewer than 2^32 threads
+  if ((long)p.many_tiles * Hkv * p.pieces + p.few_blocks >= (1l << 32) / 256) return QMOE_EINVAL;
   if (p.few_floats + p.many_floats &&
       (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15) || workspace_bytes < 4 * (p.few_floats + p.many_floats)))
     return QMOE_EWORKSPACE;

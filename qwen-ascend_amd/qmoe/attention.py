@@ -130,7 +130,8 @@ def paged_attention(q, k_cache, v_cache, table, lengths, *, starts=None, scale=N
     The caches hold the new tokens' keys and values too (:func:`append_kv`). The row of a token at
     position p sees the keys up to p, with a ``window`` > 0 only the last ``window`` of them, and
     none without a page. bfloat16 or float16; D <= 256 a multiple of 8; query heads [h G, (h + 1) G) share
-    key head h, G = Hq / Hkv <= 64. A page of a cache spans fewer than 2^30 elements. ``scale``: D^-0.5 if not given. Scores, softmax and the output's sums are
+    key head h, G = Hq / Hkv <= 64. A page of a cache spans fewer than 2^30 elements; with ``starts``,
+    T Hq / 128 + (B + 1) Hkv < 2^24 - 768. ``scale``: D^-0.5 if not given. Scores, softmax and the output's sums are
     fp32; the weights e^(s - m) are rounded to q's type for their product with the values, each
     output once. A row that sees no key, or whose scores are all -inf, gives 0, and so do rows behind
     the last sequence; else an infinite value that it sees gives an infinity, or, as 0 times it, NaN where the key's

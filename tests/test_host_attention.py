@@ -204,6 +204,18 @@ def test_planted_mistakes_are_seen():
             R.assert_close(w.to(BF16), want, bound, "planted")
 
 
+def test_grid_fits_32_bits():
+    """A grid holds fewer than 2^32 threads: the C entry refuses more (a call that it takes asks for its workspace,
+    before any launch)."""
+    from qmoe import _lib
+
+    def attend(T, B, Hq, Hkv):
+        return _lib.lib().qmoe_paged_attention(16, 8 * Hq, 8, 16, 16 * 8 * Hkv, 8 * Hkv, 8, 16, 16 * 8 * Hkv, 8 * Hkv, 8, 0, 16, 4, 4, 16, 16,
+                                               16, T, B, Hq, Hkv, 8, 16, 3, 1.0, 0, None, 0, None)
+    assert attend(1 << 24, 2, 64, 64) == -2 and attend((1 << 25) - 1, 2, 64, 64) == -1
+    assert attend(1 << 22, 1 << 16, 64, 64) == -2 and attend(1 << 24, 1 << 18, 64, 64) == -1
+
+
 def test_list_of_few_rows_fits_32_bits():
     """Places of the list of single tokens' keys, with the up to 768 that equal shares are rounded up by, stay below
     2^31: the C entry refuses more (a call that it takes asks for its workspace, before any launch)."""
