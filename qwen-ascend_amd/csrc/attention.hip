@@ -1160,7 +1160,7 @@ int qmoe_paged_attention(const void* q, long q_token, long q_head, const void* k
   // counted in 32 bits
   for (const long step : {k_page, v_page, k_slot * page, v_slot * page, k_head, v_head})
     if (step < 0 || step >= 1l << 30) return QMOE_EINVAL;
-  if ((long)B * Hkv * ((long)table_width * page / FEW_KEYS + 1 + LEAD) > 0x7fffffffl - FEW_BLOCKS_MAX) return QMOE_EINVAL;
+  if ((long)B * Hkv > (0x7fffffffl - FEW_BLOCKS_MAX) / ((long)table_width * page / FEW_KEYS + 1 + LEAD)) return QMOE_EINVAL;
   if (T == 0) return QMOE_OK;
   if (!q || !out || missing(k_cache, v_cache, n_pages, table, table_width, lengths, B)) return QMOE_EINVAL;
   const Plan p = plan_for(T, B, Hq, Hkv, D, page, table_width, window, !starts);

@@ -230,3 +230,13 @@ def test_list_of_few_rows_fits_32_bits():
     assert B * (fits + 1 + 3) <= 0x7fffff00  # within a rounder limit
     assert attend(B, fits) == -2 and attend(B, fits + 1) == -1
     assert attend(1 << 22, 1) == -2 and attend(1 << 22, 512) == -1
+
+
+def test_list_of_few_rows_past_64_bits():
+    """A batch whose places pass 64 bits is refused like any other that is too long."""
+    from qmoe import _lib
+
+    def attend(B, page):
+        return _lib.lib().qmoe_paged_attention(16, 4096 * 8, 8, 16, 4096 * 8, 0, 8, 16, 4096 * 8, 0, 8, 0, 16, 1, 1, 16, 16, 16, 1, B,
+                                               4096, 4096, 8, page, 3, 1.0, 0, None, 0, None)
+    assert attend(1 << 16, 16) == -2 and attend(1 << 28, 1 << 30) == -1 and attend((1 << 31) - 1, 1 << 30) == -1
