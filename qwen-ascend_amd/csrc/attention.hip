@@ -237,19 +237,22 @@ struct Rows {
   // bit of `there` each, the first one key `first`), p its weight, rounded as in whole tiles, so that a score of -inf
   // gives NaN here as there. k + ko and v + vo: the row of key `lane & 31`; q(ks): the second operand of K Q^T;
   // w: 4 KB of LDS that only this wave uses.
-  template <typename Q>
+  template <bool FULL, typename Q>
   QMOE_DEV void add_unusual(const unsigned char* k, long ko, const unsigned char* v, long vo, uint32_t there, int first, Seen seen,
                             float scale, Q q, float* w, int D) {
+    // (no registers for sums of the lane, offsets of elements or loads ahead: the loop before needs them)
     int lane = threadIdx.x & 63;
-    asm volatile("" : "+v"(lane));  // (no registers for sums of it, and below for loads ahead: the loop before needs them)
+    if (!FULL) asm volatile("" : "+v"(lane));
     const int half = lane >> 5;
+    int part = 16 * half, row_of = lane & 31;
+    asm volatile("" : "+v"(part), "+v"(row_of));
     f32x16_v s;
 #pragma unroll
     for (int r = 0; r < 16; ++r) s[r] = 0.f;
 #pragma unroll
     for (int ks = 0; ks < 2 * NK; ++ks) {
-      const bool within = L::always(ks) || 16 * ks + 8 * half < D;
-      u32x4_v f = *reinterpret_cast<const u32x4_v*>(k + ko + (within ? 32 * ks + 16 * half : 0));
+      const bool within = FULL || L::always(ks) || 16 * ks + 8 * half < D;
+      u32x4_v f = *reinterpret_cast<const u32x4_v*>(k + ko + (within ? 32 * ks + part : 0));
       if (!within) f = (u32x4_v){0, 0, 0, 0};
       s = Mma<E>::mma(__builtin_bit_cast(s16x8_v, f), q(ks), s);
       __builtin_amdgcn_sched_barrier(0);
@@ -258,31 +261,28 @@ struct Rows {
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
       const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], scale, -base));
-      w[(key_of(0, r) + 4 * half) * 32 + (lane & 31)] = E::load((uint16_t)Mma<E>::pack(p, p));
+      w[(key_of(0, r) + 4 * half) * 32 + row_of] = E::load((uint16_t)Mma<E>::pack(p, p));
     }
     wave_fence();
-    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll 1
     for (int i = 0; i < 32; ++i) {
-      if (!((there >> i) & 1)) continue;
-      const unsigned char* row = v + read_lane(vo, i);
-      const bool sees = first + i >= seen.low && first + i <= seen.high;
-      const float p = sees ? w[i * 32 + (lane & 31)] : 0.f;
+      const bool is = (there >> i) & 1, sees = is && first + i >= seen.low && first + i <= seen.high;
+      const unsigned char* row = v + (is ? read_lane(vo, i) : 0);
+      const float p = w[i * 32 + row_of];
       int last = D - 4;
-      asm volatile("" : "+s"(last));  // no offsets kept over the loop
+      if (!FULL) asm volatile("" : "+s"(last));
 #pragma unroll
-      for (int dt = 0; dt < NK; ++dt) {
+      for (int dt = 0; dt < NK; ++dt)
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          const s16x4_v x = *reinterpret_cast<const s16x4_v*>(row + 2 * min(32 * dt + 8 * c + 4 * half, last));
+          const int d = 32 * dt + 8 * c + 4 * half;
+          const s16x4_v x = *reinterpret_cast<const s16x4_v*>(row + 2 * (FULL ? d : min(d, last)));
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const float f = E::load((uint16_t)x[e]);
-            o[dt][4 * c + e] += sees && !(f - f == 0.f) ? p * f : 0.f;
+            if (sees && !(f - f == 0.f)) o[dt][4 * c + e] += p * f;
           }
         }
-        __builtin_amdgcn_sched_barrier(0);
-      }
     }
     wave_fence();
   }
@@ -636,8 +636,8 @@ QMOE_DEV void many_rows(const AttentionArgs& a, int block, unsigned char* lds) {
 #pragma unroll 1
       for (int j = 0; j < 2; ++j) {
         const int from = 32 * j + (lane & 31);
-        acc.add_unusual(kb, __shfl(ko, from), vb, __shfl(vo, from), (uint32_t)(present >> (32 * j)), begin + 64 * tile + 32 * j, seen,
-                        a.scale, [&](int ks) { return q[ks]; }, reinterpret_cast<float*>(lds) + 1024 * wave, FULL ? L::DC : a.D);
+        acc.template add_unusual<FULL>(kb, __shfl(ko, from), vb, __shfl(vo, from), (uint32_t)(present >> (32 * j)), begin + 64 * tile + 32 * j, seen,
+                        a.scale, [&](int ks) { return q[ks]; }, reinterpret_cast<float*>(lds) + 1024 * wave, a.D);
       }
     }
   }
@@ -863,9 +863,9 @@ QMOE_DEV void few_rows(const AttentionArgs& a, int block, unsigned char* lds) {
         const uint64_t there = __ballot(e >= 0);
         if (whole(x, there)) continue;
         const int key = first_of(x) + (lane & 31);
-        acc.add_unusual(kb, row_offset(a.kc, batch.page, e, key), vb, row_offset(a.vc, batch.page, e, key), (uint32_t)there,
+        acc.template add_unusual<FULL>(kb, row_offset(a.kc, batch.page, e, key), vb, row_offset(a.vc, batch.page, e, key), (uint32_t)there,
                         first_of(x), seen, a.scale, [&](int ks) { return NK > 4 ? q_lds[ks * 64 + lane] : q[NK > 4 ? 0 : ks]; },
-                        reinterpret_cast<float*>(mine), FULL ? L::DC : a.D);
+                        reinterpret_cast<float*>(mine), a.D);
       }
     }
 
@@ -919,9 +919,10 @@ QMOE_DEV void few_rows(const AttentionArgs& a, int block, unsigned char* lds) {
 // Each form by itself, and both in one launch: few rows' equal shares in the last blocks, where they fill what
 // the other form's tiles leave (8 sequences of up to 500 after up to 30000 365 us, 393 in the first), or in the
 // first, where most sequences must be of few rows (16 of up to 5 tokens 24.5 us, 29.9 in the last).
+// Heads of 64 in few rows alone: three workgroups on a CU, with 168 registers a wave.
 enum { MANY = 1, FEW_ROWS = 2 };
 template <typename E, int NK, bool FULL, int FORMS>
-__global__ __launch_bounds__(256, (NK <= 4 ? 2 : 1)) void attention_kernel(AttentionArgs a) {
+__global__ __launch_bounds__(256, (NK == 2 && FULL && FORMS == FEW_ROWS ? 3 : NK <= 4 ? 2 : 1)) void attention_kernel(AttentionArgs a) {
   __shared__ __align__(16) unsigned char lds[Layout<NK>::LDS];
   if constexpr (FORMS == MANY) many_rows<E, NK, FULL>(a, blockIdx.x, lds);
   else if constexpr (FORMS == FEW_ROWS) few_rows<E, NK, FULL>(a, blockIdx.x, lds);
