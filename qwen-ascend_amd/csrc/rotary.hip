@@ -4,9 +4,11 @@
 //   (a, b) -> turn * (a cos - b sin, b cos + a sin)
 // Pairs are (x_i, x_{i + rd/2}) or (x_2i, x_{2i+1}), i < rd/2; elements from rd on are copied.
 //
-// Frequencies come as 64-bit fractions of a turn, so that p f_i mod 1 is one integer product,
-// exact at any position; its leading 32 bits are the angle (2^-32 of a turn), and cosine and sine
-// are taken of it in fp32. One rounding per output.
+// Frequencies come as 64-bit fractions of a turn, so that p f_i mod 1 is one integer product, exact
+// at any position (the frequency itself is rounded once, to 53 bits where it was worked out in double
+// precision); its leading 32 bits are the angle (2^-32 of a turn), and cosine and sine are
+// taken of it in fp32, where the angle in half turns keeps 24 bits: fp32 outputs are off by 4.3e-8 of their norm,
+// with angles and their functions in 64 bits 3.3e-8. One rounding per output.
 #include "paged.h"
 
 #include <algorithm>
@@ -208,6 +210,8 @@ int launch_chunks(const RotateArgs& a, hipStream_t st) {
 template <typename E>
 int launch(const RotateArgs& a, hipStream_t st) {
   constexpr int C = 16 / sizeof(typename E::raw);
+  // Where a half of what turns is no whole pieces of 16 bytes, element by element: 8192 tokens of 32 heads of 96, 24
+  // turned, 72.8 us (1.4 TB/s), 96 turned 20.1 (5.0).
   if (a.rd % (2 * C) == 0 && a.D % C == 0) return launch_chunks<E, C>(a, st);
   return launch_chunks<E, 1>(a, st);
 }

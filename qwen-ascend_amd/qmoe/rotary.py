@@ -1,8 +1,8 @@
 """Rotary positions.
 
 Pair i of a head at position p turns by the angle p * f_i, with f_i = base^(-2i / dim). The
-frequencies are kept as 64-bit fractions of a turn, so an angle is one integer product, exact at
-any position; no table of cosines is kept. HIP kernel ``qmoe_rotate`` of libqmoe.so. Forward only: a
+frequencies, worked out in double precision, are kept as 64-bit fractions of a turn, so an angle is one
+integer product, which adds no error at any position; no table of cosines is kept. HIP kernel ``qmoe_rotate`` of libqmoe.so. Forward only: a
 tensor that requires a gradient is refused while gradients are recorded, and one with a
 forward-mode tangent.
 """
